@@ -1,0 +1,267 @@
+"""Matrices in microscaled 4-bit floating point against their definition in 64 bits.
+
+Quantising and going back are exact but for the one rounding that the definition names, so codes, scales and values are
+compared for equality.  A product's error is bounded by arithmetic:
+
+* its float32 sums: at most K additions, each off by a unit in the last place at most, 2^-23 of what has been summed so far:
+  K 2^-23 sum |x w|;
+* rows in bfloat16 or float32 are multiplied as they are; a kernel may hold them as whole multiples of a block's step, off by half a
+  step, at most 2^-16 (bfloat16) or 2^-22 (float32) of the block's largest entry: that times sum over the row of top |w|;
+* the one rounding to the output: half a step, 2^-8 (bfloat16) or 2^-24 (float32) of the value.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from plain import mx4_plain as plain
+from thing_htn_2026_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+ROW_STEP = {torch.bfloat16: 2.0 ** -16, torch.float32: 2.0 ** -22}
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+def as64(t):
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+def rows_of(rows, columns, dtype, seed, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((rows, columns), generator=g) * spread
+    x *= 2.0 ** torch.randint(-3, 4, (rows, columns), generator=g)
+    return x.to(dtype).cuda()
+
+
+def weight_of(n, k, seed):
+    """(the library's matrix, its values in float64)."""
+    g = np.random.default_rng(seed)
+    codes, scales = plain.quantize(g.standard_normal((n, k)) * np.exp2(g.integers(-6, 2, (n, 1))))
+    stored = torch.from_numpy(plain.stored(codes, k)).cuda()
+    return ops.mx4_from_parts(stored, torch.from_numpy(scales).cuda(), k), plain.values(codes, scales, k)
+
+
+def scale_bytes(q):
+    """[rows, blocks] of a matrix's scales."""
+    tiles = q.scales.cpu().numpy().reshape(q.scales.shape[0], q.scales.shape[1], 32, 4, 4)
+    flat = tiles.transpose(0, 3, 2, 1, 4).reshape(q.scales.shape[0] * 128, -1)      # row = 32 * (middle axis) + lane
+    return flat[:q.rows, :-(-q.columns // 32)]
+
+
+def check_quantized(x):
+    q = ops.quantize_mx4(x)
+    codes, scales = plain.quantize(as64(x))
+    assert np.array_equal(scale_bytes(q), scales)
+    got = q.codes.cpu().numpy()
+    want = np.zeros((q.rows, q.codes.shape[1]), dtype=np.uint8)
+    stored = plain.stored(codes, q.columns)
+    want[:, :stored.shape[1]] = stored
+    assert np.array_equal(got, want)
+    for dtype in DTYPES:
+        np.testing.assert_array_equal(as64(ops.dequantize_mx4(q, dtype)), plain.values(codes, scales, q.columns))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,columns", [(1, 1), (1, 32), (1, 2560), (3, 31), (5, 33), (37, 1000), (127, 128), (128, 136), (129, 264),
+                                          (300, 520), (2, 4099)])
+def test_quantized_matrix_is_the_definition(rows, columns, dtype):
+    check_quantized(rows_of(rows, columns, dtype, rows * 10007 + columns))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_midpoint_sign_and_scale(dtype):
+    """Blocks whose largest entry is 4 or 7.5 of their scale, with every midpoint between two magnitudes and its neighbours, over all
+    scales that the type reaches, zeros of both signs, subnormal numbers and blocks of zeros."""
+    eps = torch.finfo(dtype).eps
+    middle = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)
+    rows = []
+    for top in (4.0, 7.5):
+        for e in list(range(-133, -120)) + list(range(-5, 6)) + list(range(120, 126)):
+            row = torch.cat([torch.tensor([top, -0.0, 0.0, -6.0 if top > 6 else -3.0], dtype=torch.float64), middle, -middle,
+                             middle * (1 + eps), middle * (1 - eps)])
+            rows.append(row * 2.0 ** e)
+    x = torch.stack(rows + [torch.zeros(32, dtype=torch.float64), -torch.zeros(32, dtype=torch.float64)]).to(dtype).cuda()
+    assert torch.isfinite(x).all()
+    check_quantized(x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_a_block_with_a_number_that_is_not_finite(dtype, bad):
+    x = rows_of(4, 200, dtype, 5)
+    x[1, 40] = bad
+    x[3, 199] = bad
+    check_quantized(x)
+    values = as64(ops.dequantize_mx4(ops.quantize_mx4(x)))
+    gone = np.isnan(values)
+    assert gone[1, 32:64].all() and gone[3, 192:].all() and gone.sum() == 32 + 8
+
+
+@pytest.mark.parametrize("columns", [1, 31, 32, 95, 128, 1000])
+def test_stored_parts_keep_every_code_and_scale(columns):
+    g = np.random.default_rng(columns)
+    codes = g.integers(0, 16, (130, -(-columns // 32), 32), dtype=np.uint8)
+    scales = g.integers(0, 255, (130, -(-columns // 32)), dtype=np.uint8)
+    scales[7, 0] = 255
+    stored = plain.stored(codes, columns)
+    if columns % 2:
+        stored[:, -1] |= 0x50          # the half byte behind the last entry means nothing
+    q = ops.mx4_from_parts(torch.from_numpy(stored).cuda(), torch.from_numpy(scales).cuda(), columns)
+    assert q.shape == (130, columns)
+    with np.errstate(over="ignore"):
+        want = plain.values(codes, scales, columns).astype(np.float32)      # 6 * 2^127 is beyond float32
+    np.testing.assert_array_equal(ops.dequantize_mx4(q).cpu().numpy(), want)
+
+
+def bound(x, w, y, k, x_dtype, out_dtype, bias):
+    """How far a product may be off, entry by entry (see the top of this file)."""
+    sums = np.abs(x) @ np.abs(w).T
+    e = k * 2.0 ** -23 * (sums + (0 if bias is None else np.abs(bias)))
+    if x_dtype is not None:
+        e += ROW_STEP[x_dtype] * (plain.block_tops(x) @ np.abs(w).T)
+    return e + HALF_STEP[out_dtype] * (np.abs(y) + e)
+
+
+def check_product(m, n, k, x_dtype, out_dtype, with_bias=False, quantized=False, seed=0, spread=1.0):
+    x = rows_of(m, k, x_dtype, seed + 1, spread)
+    weight, w = weight_of(n, k, seed + 2)
+    bias = rows_of(1, n, x_dtype, seed + 3)[0] if with_bias else None
+    err = ops.new_error_word("cuda")
+    given = ops.quantize_mx4(x) if quantized else x
+    got = ops.linear_mx4(given, weight, out_dtype=out_dtype, bias=bias, err=err)
+    assert got.dtype == out_dtype and tuple(got.shape) == (m, n)
+    ops.raise_on_device_error(err, "test")
+    x64 = plain.values(*plain.quantize(as64(x)), k) if quantized else as64(x)
+    b64 = None if bias is None else as64(bias)
+    y = x64 @ w.T + (0 if bias is None else b64)
+    error = np.abs(as64(got) - y)
+    limit = bound(x64, w, y, k, None if quantized else x_dtype, out_dtype, b64)
+    assert (error <= limit).all(), (error / np.maximum(limit, 1e-300)).max()
+    return given, weight, got
+
+
+SIZES = [(1, 1, 1), (1, 128, 256), (1, 2560, 2560), (2, 100, 32), (3, 515, 1096), (5, 1333, 1000), (8, 640, 2432), (9, 129, 4100), (16, 256, 640),
+         (17, 384, 128), (31, 130, 384), (33, 257, 999), (42, 512, 256), (43, 512, 256), (64, 1000, 512), (77, 515, 1096), (100, 24, 8192),
+         (128, 128, 128), (129, 300, 1500), (200, 2000, 320), (257, 513, 130), (300, 256, 3000), (511, 260, 96)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_product_of_rows_as_they_are(m, n, k, dtype):
+    check_product(m, n, k, dtype, dtype, with_bias=(m + n) % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_product_of_quantized_rows(m, n, k, dtype):
+    check_product(m, n, k, dtype, dtype, with_bias=(m + n) % 2 == 0, quantized=True)
+
+
+@pytest.mark.parametrize("m", [4, 60, 300])
+@pytest.mark.parametrize("quantized", [False, True])
+def test_product_with_the_other_output_type(m, quantized):
+    check_product(m, 260, 500, torch.bfloat16, torch.float32, quantized=quantized)
+    check_product(m, 260, 500, torch.float32, torch.bfloat16, quantized=quantized)
+
+
+@pytest.mark.parametrize("spread", [2.0 ** -60, 2.0 ** 60])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [3, 150])
+def test_product_of_far_rows(m, dtype, spread):
+    check_product(m, 200, 700, dtype, dtype, spread=spread)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("m", [2, 40, 140, 300])
+def test_what_is_not_a_number_stays_in_its_row_and_column(m, quantized):
+    """A NaN or an infinity in a row of x makes that row NaN, one in a row of the weight that column; the rest is as without them."""
+    x = rows_of(m, 600, torch.bfloat16, 3)
+    g = torch.Generator().manual_seed(4)
+    w = torch.randn((200, 600), generator=g).cuda()
+    clean = ops.linear_mx4(ops.quantize_mx4(x) if quantized else x, ops.quantize_mx4(w))
+    x[1, 555] = float("nan")
+    w[130, 17] = float("inf")
+    got = ops.linear_mx4(ops.quantize_mx4(x) if quantized else x, ops.quantize_mx4(w))
+    assert torch.isnan(got[1]).all() and torch.isnan(got[:, 130]).all()
+    keep_rows = torch.arange(m, device="cuda") != 1
+    keep = torch.arange(200, device="cuda") != 130
+    assert torch.equal(got[keep_rows][:, keep], clean[keep_rows][:, keep])
+
+
+def test_no_rows():
+    weight, _ = weight_of(10, 64, 0)
+    x = torch.zeros((0, 64), dtype=torch.bfloat16, device="cuda")
+    assert ops.quantize_mx4(x).shape == (0, 64)
+    assert tuple(ops.dequantize_mx4(ops.quantize_mx4(x)).shape) == (0, 64)
+    assert tuple(ops.linear_mx4(x, weight).shape) == (0, 10)
+    assert tuple(ops.linear_mx4(ops.quantize_mx4(x), weight).shape) == (0, 10)
+
+
+def test_refusals():
+    weight, _ = weight_of(10, 64, 0)
+    x = torch.zeros((2, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ops.KernelError, match="dtype"):
+        ops.quantize_mx4(x.half())
+    with pytest.raises(ops.KernelError, match="contiguous"):
+        ops.quantize_mx4(x.t())
+    with pytest.raises(ops.KernelError, match="matrix"):
+        ops.quantize_mx4(x[0])
+    with pytest.raises(ops.KernelError, match="matrix"):
+        ops.quantize_mx4(x[:, :0].contiguous())
+    with pytest.raises(ops.KernelError, match="dtype"):
+        ops.dequantize_mx4(weight, torch.float16)
+    with pytest.raises(ops.KernelError, match="shapes"):
+        ops.linear_mx4(x[:, :32].contiguous(), weight)
+    with pytest.raises(ops.KernelError, match="shapes"):
+        ops.linear_mx4(ops.quantize_mx4(x[:, :32].contiguous()), weight)
+    with pytest.raises(ops.KernelError, match="contiguous"):
+        ops.linear_mx4(torch.zeros((64, 2), dtype=torch.bfloat16, device="cuda").t(), weight)
+    with pytest.raises(ops.KernelError, match="out_dtype"):
+        ops.linear_mx4(x, weight, out_dtype=torch.float16)
+    with pytest.raises(ops.KernelError, match="bias"):
+        ops.linear_mx4(x, weight, bias=torch.zeros(9, device="cuda"))
+    with pytest.raises(ops.KernelError, match="CUDA"):
+        ops.linear_mx4(x.cpu(), weight)
+    parts = torch.zeros((4, 32), dtype=torch.uint8, device="cuda")
+    with pytest.raises(ops.KernelError, match="codes"):
+        ops.mx4_from_parts(parts, torch.zeros((4, 3), dtype=torch.uint8, device="cuda"), 64)
+    with pytest.raises(ops.KernelError, match="codes"):
+        ops.mx4_from_parts(parts, torch.zeros((4, 2), dtype=torch.uint8, device="cuda"), 70)
+
+
+def test_another_stream_and_a_recorded_graph():
+    """Calls on a side stream, two recorded graphs that are replayed in turn with inputs of their own, and eager calls between."""
+    weight, w = weight_of(384, 512, 9)
+    inputs = [rows_of(m, 512, torch.bfloat16, 20 + m) for m in (2, 70)]
+    want = [ops.linear_mx4(x, weight) for x in inputs] + [ops.linear_mx4(ops.quantize_mx4(x), weight) for x in inputs]
+    static = [x.clone() for x in inputs]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = [ops.linear_mx4(x, weight) for x in static]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for x in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([ops.linear_mx4(x, weight), ops.linear_mx4(ops.quantize_mx4(x), weight)])
+        graphs.append(graph)
+    for _ in range(3):
+        for x in static:
+            x.zero_()
+        for graph in graphs:
+            graph.replay()
+        assert all((o == 0).all() for pair in outs for o in pair)
+        for x, source in zip(static, inputs):
+            x.copy_(source)
+        for graph in reversed(graphs):
+            graph.replay()
+        eager = ops.linear_mx4(inputs[0], weight)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0])
+        for i in range(2):
+            assert torch.equal(again[i], want[i])
+            assert torch.equal(outs[i][0], want[i]) and torch.equal(outs[i][1], want[2 + i])

@@ -149,6 +149,10 @@ _SIGNATURES = {
                                    c_int, c_int, c_int, c_void_p],
     "thn_delta_decode": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
+    "thn_mx4_quantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
+    "thn_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
+    "thn_mx4_arrange": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p],
+    "thn_mx4_linear": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "thn_gemm_f32": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "thn_linear_skinny_bf16": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "thn_linear_skinny_supported": [c_int, c_int],
@@ -981,6 +985,117 @@ def linear_batched(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     out = torch.empty((x.shape[0], x.shape[1], weight.shape[1]), dtype=torch.float32, device=x.device)
     for b in range(x.shape[0]):
         _call("thn_gemm_f32", _ptr(out[b]), _ptr(x[b]), _ptr(weight[b]), x.shape[1], weight.shape[1], x.shape[2], _stream())
+    return out
+
+
+# ------------------------------------------------------------------ microscaled 4-bit matrices
+
+
+@dataclass(frozen=True)
+class Mx4:
+    """A matrix ``[rows, columns]`` in microscaled 4-bit floating point: every 32 neighbouring entries of a row share a
+    scale, a power of two held in a byte (``2^(byte - 127)``; 255: the block is not a number), and an entry is one of 0, 1/2, 1, 3/2,
+    2, 3, 4, 6 with a sign, held in four bits.  ``codes`` and ``scales`` are laid out for the tensor cores
+    (``csrc/mx4.cuh``); :func:`quantize_mx4` makes one from numbers, :func:`mx4_from_parts` from stored codes and scales."""
+
+    codes: torch.Tensor      # uint8 [rows, padded columns / 2]
+    scales: torch.Tensor     # uint8 [ceil(rows / 128), padded columns / 128, 512]
+    rows: int
+    columns: int
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return (self.rows, self.columns)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def _on_current_device(t: torch.Tensor, what: str) -> None:
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _mx4_empty(rows: int, columns: int, device) -> Mx4:
+    padded = -(-columns // 128) * 128
+    return Mx4(torch.empty((rows, padded // 2), dtype=torch.uint8, device=device),
+               torch.empty((-(-rows // 128), padded // 128, 512), dtype=torch.uint8, device=device), rows, columns)
+
+
+def quantize_mx4(x: torch.Tensor) -> Mx4:
+    """``x [rows, columns]`` (bfloat16 or float32) in microscaled 4-bit floating point.  A block's scale is
+    ``2^(floor(log2 max|x|) - 2)``, at least 2^-127, and an entry becomes the nearest magnitude, of two equally near ones that with
+    the even code; what lies above 6 scales becomes 6.  A block that holds an infinity or a NaN is not a number as a whole."""
+    _need(x, "quantize_mx4 x")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise KernelError(f"quantize_mx4: a matrix with columns, please, not {tuple(x.shape)}")
+    code = _code(x, "quantize_mx4 x")
+    _on_current_device(x, "quantize_mx4 x")
+    out = _mx4_empty(x.shape[0], x.shape[1], x.device)
+    _call("thn_mx4_quantize", _ptr(out.codes), _ptr(out.scales), _ptr(x), x.shape[0], x.shape[1], code, _stream())
+    return out
+
+
+def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> Mx4:
+    """A matrix from what a file holds, row by row: ``codes`` uint8 ``[rows, ceil(columns / 2)]``, two entries a byte with the first in
+    the low half, and ``scales`` uint8 ``[rows, ceil(columns / 32)]``."""
+    _need(codes, "mx4_from_parts codes", torch.uint8)
+    _need(scales, "mx4_from_parts scales", torch.uint8)
+    columns = int(columns)
+    rows = codes.shape[0]
+    if columns < 1 or codes.dim() != 2 or tuple(codes.shape) != (rows, -(-columns // 2)) or tuple(scales.shape) != (rows, -(-columns // 32)):
+        raise KernelError(f"mx4_from_parts: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} for {columns} columns")
+    if scales.device != codes.device:
+        raise KernelError(f"mx4_from_parts: codes on {codes.device}, scales on {scales.device}")
+    _on_current_device(codes, "mx4_from_parts codes")
+    out = _mx4_empty(rows, columns, codes.device)
+    _call("thn_mx4_arrange", _ptr(out.codes), _ptr(out.scales), _ptr(codes), _ptr(scales), rows, columns, _stream())
+    return out
+
+
+def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The numbers ``[rows, columns]`` that ``q`` stands for, in float32 or bfloat16; both hold them exactly."""
+    if dtype not in DTYPE_CODE:
+        raise KernelError(f"dequantize_mx4: dtype {dtype} is not supported (float32 or bfloat16)")
+    _on_current_device(q.codes, "dequantize_mx4 q")
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    _call("thn_mx4_dequantize", _ptr(out), _ptr(q.codes), _ptr(q.scales), q.rows, q.columns, DTYPE_CODE[dtype], _stream())
+    return out
+
+
+def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x [M, K] @ weight[N, K]^T`` (+ ``bias [N]``) with a weight in 4 bits: float32 sums, one rounding to ``out_dtype`` (bfloat16 or
+    float32).  ``x`` is a tensor in bfloat16 or float32, which is multiplied as it is and whose type is the default
+    ``out_dtype``, or an :class:`Mx4` (default: bfloat16)."""
+    quantized = isinstance(x, Mx4)
+    if not quantized:
+        _need(x, "linear_mx4 x")
+        if x.dim() != 2:
+            raise KernelError(f"linear_mx4: x has {x.dim()} dimensions, not 2")
+    if x.shape[1] != weight.columns:
+        raise KernelError(f"linear_mx4: shapes x {tuple(x.shape)}, weight {weight.shape}")
+    if x.device != weight.device:
+        raise KernelError(f"linear_mx4: x on {x.device}, weight on {weight.device}")
+    data = x.codes if quantized else x
+    _on_current_device(data, "linear_mx4 x")
+    kind = 2 if quantized else _code(x, "linear_mx4 x")
+    out_dtype = out_dtype or (torch.bfloat16 if quantized else x.dtype)
+    if out_dtype not in DTYPE_CODE:
+        raise KernelError(f"linear_mx4: out_dtype {out_dtype} is not supported (float32 or bfloat16)")
+    if bias is not None:
+        _need(bias, "linear_mx4 bias")
+        if tuple(bias.shape) != (weight.rows,) or bias.device != data.device:
+            raise KernelError(f"linear_mx4: a bias {tuple(bias.shape)} on {bias.device} for {weight.rows} outputs on {data.device}")
+    bias_code = 0 if bias is None else _code(bias, "linear_mx4 bias")
+    out = torch.empty((x.shape[0], weight.rows), dtype=out_dtype, device=data.device)
+    _call("thn_mx4_linear", _ptr(out), DTYPE_CODE[out_dtype], _ptr(data), _ptr(x.scales) if quantized else None, kind, _ptr(weight.codes),
+          _ptr(weight.scales), _ptr(bias), bias_code, x.shape[0], weight.rows, weight.columns, _ptr(err), _stream())
     return out
 
 
