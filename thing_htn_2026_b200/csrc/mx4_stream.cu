@@ -1,0 +1,430 @@
+// out[M, N] = x[M, K] @ W[N, K]^T (+ bias) for few rows, W in microscaled 4-bit floating point (mx4.cuh): bound by reading W once.
+//
+//  * 128 rows of W are the wide operand of tcgen05.mma (kind::mxf8f6f4, scales applied by the tensor core), the rows of x its
+//    narrow one.  W comes by TMA, which spreads its 4-bit codes over 8-bit containers as it copies, so no thread touches a weight;
+//    its scales come as 512 bytes for 128 rows and 128 columns, in the order of tensor memory, and go there by tcgen05.cp.
+//  * Rows in bfloat16 or float32 become two or six terms of 8-bit floats in the kernel (mx4_tcgen05.cuh), a column of the narrow
+//    operand each; their sums are added at the end.  Rows in 4 bits are brought as W is.
+//  * A tile of 128 outputs is cut along K among the blocks of a cluster, whose partial sums meet in distributed shared memory
+//    and are added in ascending order: no scratch memory, no counters, the same result every time.
+//  * Two blocks a multiprocessor while the rows are few: the bytes in flight cover the memory's latency, and one block's
+//    start and end lie under the other's stream.
+//
+// Every wait on an mbarrier is bounded: after kWaitLimitNs the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, the
+// block's partial sums become NaN, and tensor memory is given back.  No wait depends on another block.
+#include "mx4_tcgen05.cuh"
+
+namespace {
+
+constexpr int BW = 128, BK = 128, UMMA_K = 32;
+constexpr int kThreads = 192;                          // warp 0: TMA, warp 1: products and tensor memory, warps 2-5: rows of x, then the sums
+constexpr uint32_t kWSmem = BW * BK, kWBytes = kWSmem / 2;     // in shared memory; as the barrier counts
+constexpr int kMaxStages = 12;
+constexpr int kMaxCluster = 8;
+
+// RT: how the rows come (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for
+template <typename RT, int MR>
+struct Shape {
+    static constexpr bool kQuantized = sizeof(RT) == 1;
+    static constexpr int kT = kQuantized ? 1 : kTerms<RT>;
+    static constexpr int NX = MR * kT < 16 ? 16 : MR * kT;           // columns of the product
+    static constexpr int kXAtoms = (NX + 127) / 128;
+    static constexpr uint32_t kXSmem = NX * BK;
+    static constexpr uint32_t kStageBytes = kWSmem + kXSmem + (1 + kXAtoms) * kMx4AtomBytes;
+    static constexpr uint32_t kStageStride = (kStageBytes + 1023) / 1024 * 1024;
+    static constexpr int kRecvFloats = (MR + kMaxCluster) * BW;      // [own row][sending block][output]
+    static constexpr size_t kFixed = kRecvFloats * 4 + 1024 /* alignment */ + 512 /* barriers */;
+    static constexpr size_t kBudget = 3 * kStageStride + kFixed <= 113 * 1024 ? 113 * 1024 : 226 * 1024;
+    static constexpr int kFit = (int)((kBudget - kFixed) / kStageStride);
+    static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+    static constexpr size_t kSmemBytes = kStages * kStageStride + kFixed;
+    static constexpr int kUsedCols = NX + 4 + 4 * kXAtoms;
+    static constexpr int kTmemCols = kUsedCols <= 32 ? 32 : kUsedCols <= 64 ? 64 : kUsedCols <= 128 ? 128 : 256;
+    static constexpr uint32_t kInstr = scaled_instr(kE2M1, kQuantized ? kE2M1 : kE4M3, BW, NX);
+};
+
+struct Args {
+    void* out;
+    const void* x;                // [M, K] of RT; 4 bits: its map
+    const uint8_t* x_scales;
+    const uint8_t* w_scales;
+    const void* bias;
+    int M, N, K, chunks, vector;  // vector: x's rows are whole aligned 16-byte pieces
+    int* err;
+    int skip_loads;               // the test of the bounded waits: nothing is loaded
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// *mine as it lies in block `rank` of the cluster <- v
+__device__ __forceinline__ void store_to_block(float* mine, uint32_t rank, float v) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(mine)), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
+
+// Eight neighbouring entries of a row as they lie in memory; what lies behind the last column is zero.
+template <typename RT>
+struct Eight {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const RT* row, int c, int K, bool vector) {
+        if (vector && c + 8 <= K) {
+            a = *reinterpret_cast<const uint4*>(row + c);
+            if constexpr (sizeof(RT) == 4) b = *reinterpret_cast<const uint4*>(row + c + 4);
+        } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = c + i < K ? __float_as_uint(to_f32<RT>(row[c + i])) : 0u;
+            if constexpr (sizeof(RT) == 4) {
+                a = make_uint4(w[0], w[1], w[2], w[3]);
+                b = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+                a = make_uint4(w[0] >> 16 | (w[1] & 0xffff0000u), w[2] >> 16 | (w[3] & 0xffff0000u), w[4] >> 16 | (w[5] & 0xffff0000u),
+                               w[6] >> 16 | (w[7] & 0xffff0000u));
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (sizeof(RT) == 4) {
+            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+        } else {
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+};
+
+template <typename RT, int MR, typename OutT, typename BiasT>
+__global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                              const Args a) {
+    using S = Shape<RT, MR>;
+    pdl_launch_dependents();
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* recv = reinterpret_cast<float*>(tiles + (size_t)S::kStages * S::kStageStride);
+    uint64_t* full = reinterpret_cast<uint64_t*>(recv + S::kRecvFloats);
+    uint64_t* empty = full + S::kStages;
+    uint64_t* acc_full = empty + S::kStages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+    volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank(), n_ranks = (int)cluster_size();
+    const int tile = blockIdx.x / n_ranks;
+    const int c0 = (int)((long long)a.chunks * rank / n_ranks), c1 = (int)((long long)a.chunks * (rank + 1) / n_ranks);
+
+    if (warp == 0) {
+        if (lane < S::kStages) mbar_init(full + lane, S::kQuantized ? 1 : 5);      // the copies, and the four warps that bring x
+        else if (lane < 2 * S::kStages) mbar_init(empty + (lane - S::kStages), 1);
+        else if (lane == 2 * S::kStages) mbar_init(acc_full, 1);
+        if (lane == 0) *give_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                     "r"(S::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    cluster_arrive();                          // this block has begun: the others may reach into it
+
+    if (warp == 0 && lane == 0) {
+        // ---- TMA producer: W of the first stages before the wait for the kernel that makes x
+        const int n = a.skip_loads ? 0 : c1 - c0;
+        const uint32_t bytes = kWBytes + kMx4AtomBytes + (S::kQuantized ? S::kXSmem / 2 + kMx4AtomBytes * S::kXAtoms : 0);
+        auto load_w = [&](int s, int c) {
+            unsigned char* dst = tiles + (size_t)s * S::kStageStride;
+            mbar_expect_tx(full + s, bytes);
+            tma_load_2d(dst, &map_w, full + s, c * BK, tile * BW);
+            bulk_load(dst + kWSmem + S::kXSmem, a.w_scales + ((long long)tile * a.chunks + c) * kMx4AtomBytes, kMx4AtomBytes, full + s);
+        };
+        auto load_x = [&](int s, int c) {
+            if constexpr (S::kQuantized) {
+                unsigned char* dst = tiles + (size_t)s * S::kStageStride;
+                tma_load_2d(dst + kWSmem, &map_x, full + s, c * BK, 0);
+                bulk_load(dst + kWSmem + S::kXSmem + kMx4AtomBytes, a.x_scales + (long long)c * kMx4AtomBytes, kMx4AtomBytes, full + s);
+            }
+        };
+        const int early = min(S::kStages, n);
+        for (int i = 0; i < early; ++i) load_w(i, c0 + i);
+        pdl_wait();
+        for (int i = 0; i < early; ++i) load_x(i, c0 + i);
+        for (int i = early; i < n && !*give_up; ++i) {
+            const int s = i % S::kStages;
+            if (!mbar_wait(empty + s, ((i / S::kStages) & 1) ^ 1)) {
+                if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                *give_up = 1;
+                break;
+            }
+            load_w(s, c0 + i);
+            load_x(s, c0 + i);
+        }
+    } else if (warp == 1 && lane == 0) {
+        // ---- the products
+        const uint32_t w_col = tmem_base + S::NX, x_col = w_col + 4;
+        bool ok = true;
+        for (int i = 0; i < c1 - c0 && ok && !*give_up; ++i) {
+            const int s = i % S::kStages;
+            ok = mbar_wait(full + s, (i / S::kStages) & 1);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride), scales = at + kWSmem + S::kXSmem;
+            scales_to_tmem(w_col, scale_desc(scales));
+#pragma unroll
+            for (int j = 0; j < S::kXAtoms; ++j) scales_to_tmem(x_col + 4 * j, scale_desc(scales + (1 + j) * kMx4AtomBytes));
+            const uint64_t w_desc = smem_desc(at), x_desc = smem_desc(at + kWSmem);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k)          // 32 bytes further along K: + 2 in the address field
+                mma_scaled(tmem_base, w_desc + 2 * k, x_desc + 2 * k, with_scale_byte(S::kInstr, k), w_col, x_col, (i | k) != 0);
+            umma_commit(empty + s);
+        }
+        if (!ok) {
+            if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+            *give_up = 1;
+            __threadfence_block();
+        }
+        umma_commit(acc_full);
+    } else if (warp >= 2) {
+        pdl_wait();
+        const int quarter = warp & 3;
+        if constexpr (!S::kQuantized) {
+            // ---- rows of x to terms: a thread takes eight columns of every eighth row
+            const int t = threadIdx.x - 64, piece = t & 15, first = t >> 4;
+            constexpr int kPasses = MR / 8;
+            Eight<RT> held[kPasses];
+            auto fetch = [&](int i) {
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    const int row = first + 8 * p;
+                    if (row < a.M) held[p].load(static_cast<const RT*>(a.x) + (long long)row * a.K, (c0 + i) * BK + piece * 8, a.K, a.vector);
+                }
+            };
+            if (c1 > c0) fetch(0);
+            for (int i = 0; i < c1 - c0 && !*give_up; ++i) {
+                const int s = i % S::kStages;
+                if (i >= S::kStages && !__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / S::kStages) & 1) ^ 1))) {
+                    if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                    *give_up = 1;
+                    break;
+                }
+                unsigned char* dst = tiles + (size_t)s * S::kStageStride + kWSmem;
+                unsigned char* scales = dst + S::kXSmem + kMx4AtomBytes;
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    const int row = first + 8 * p;
+                    if (8 * p >= a.M) break;                        // the same for all
+                    float v[8];
+                    if (row < a.M) {
+                        held[p].get(v);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+                    }
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (row >= a.M) continue;
+                    const uint32_t b = row_scale_byte(top);
+                    const float factor = __uint_as_float((254 - min(b, 253u)) << 23);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = b == 255 ? 0.f : v[j] * factor;
+#pragma unroll
+                    for (int term = 0; term < S::kT; ++term) {
+                        const uint32_t here = term_scale_byte(b, term), after = term_scale_byte(b, term + 1);
+                        const uint2 bytes = next_term(v, __uint_as_float((127 + here - after) << 23));
+                        const int column = term * MR + row;
+                        *reinterpret_cast<uint2*>(dst + column * BK + (((piece >> 1) ^ (column & 7)) << 4) + (piece & 1) * 8) = bytes;
+                        if ((piece & 3) == 0)
+                            scales[(column >> 7) * kMx4AtomBytes + (column & 31) * 16 + ((column & 127) >> 5) * 4 + (piece >> 2)] = (uint8_t)here;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + s);
+                if (i + 1 < c1 - c0) fetch(i + 1);
+            }
+        }
+        // ---- this block's partial sums, row by row, to the rows' owners
+        const int r = quarter * 32 + lane;
+        float acc[MR];
+#pragma unroll
+        for (int j = 0; j < MR; ++j) acc[j] = 0.f;
+        if (c1 > c0) {
+            if (__all_sync(0xffffffffu, mbar_wait(acc_full, 0))) {      // all lanes together before tcgen05.ld
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+                for (int j = 0; j < MR; j += 8) {
+                    float v[S::kT][8];
+#pragma unroll
+                    for (int term = 0; term < S::kT; ++term) tmem_load_8(taddr + term * MR + j, v[term]);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int term = S::kT - 1; term >= 0; --term)        // the smallest first
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) acc[j + e] += v[term][e];
+                }
+            } else {
+                if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                *give_up = 1;
+            }
+            if (*give_up) {
+#pragma unroll
+                for (int j = 0; j < MR; ++j) acc[j] = __uint_as_float(0x7fffffffu);
+            }
+        }
+        __syncwarp();
+        cluster_wait();                             // every block has begun
+        // row j goes to block j % n_ranks, as that block's row j / n_ranks, sender `rank`
+        int owner = 0, slot = rank;                 // slot = (j / n_ranks) * n_ranks + rank, kept without divisions
+#pragma unroll
+        for (int j = 0; j < MR; ++j) {
+            if (j < a.M) store_to_block(recv + slot * BW + r, (uint32_t)owner, acc[j]);
+            if (++owner == n_ranks) {
+                owner = 0;
+                slot += n_ranks;
+            }
+        }
+    }
+    __syncwarp();
+    if (warp < 2) cluster_wait();
+    cluster_arrive();
+    cluster_wait();                            // the partial sums are where they are added
+    if (warp >= 2) {
+        // ---- this block's rows, partial sums added in ascending order of K
+        const int r = (warp & 3) * 32 + lane;
+        const int n = tile * BW + r;
+        const float bias = a.bias && n < a.N ? to_f32<BiasT>(static_cast<const BiasT*>(a.bias)[n]) : 0.f;
+        for (int j = rank, own = 0; j < a.M; j += n_ranks, ++own) {
+            float v[kMaxCluster];
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q) v[q] = q < n_ranks ? recv[(own * n_ranks + q) * BW + r] : 0.f;
+            float sum = 0.f;
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q) sum += v[q];
+            if (n < a.N) static_cast<OutT*>(a.out)[(long long)j * a.N + n] = from_f32<OutT>(sum + bias);
+        }
+    }
+    if (*give_up) let_copies_land();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+    }
+}
+
+// The blocks of a cluster: as many as the resident blocks leave for a tile, two a multiprocessor where they fit, and no
+// more than there are pieces of K.
+template <typename RT, int MR>
+int cluster_for(int n_tiles, int chunks, int n_sms) {
+    const int resident = n_sms * (Shape<RT, MR>::kSmemBytes <= 113 * 1024 ? 2 : 1);
+    int c = resident / n_tiles;
+    if (c > kMaxCluster) c = kMaxCluster;
+    if (c > chunks) c = chunks;
+    return c < 1 ? 1 : c;
+}
+
+template <typename RT, int MR, typename OutT, typename BiasT>
+int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Args& args, cudaStream_t stream) {
+    using S = Shape<RT, MR>;
+    auto kernel = mx4_stream_kernel<RT, MR, OutT, BiasT>;
+    static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmemBytes);
+    if (configured != cudaSuccess) {
+        thn_set_error("mx4_stream: cannot reserve %zu bytes of shared memory: %s", S::kSmemBytes, cudaGetErrorString(configured));
+        return (int)configured;
+    }
+    int device = 0, n_sms = 0;
+    cudaGetDevice(&device);
+    cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
+    const int n_tiles = (args.N + BW - 1) / BW, c = cluster_for<RT, MR>(n_tiles, args.chunks, n_sms);
+    thn_launch_cluster(kernel, dim3((unsigned)(n_tiles * c)), dim3(kThreads), S::kSmemBytes, stream, dim3((unsigned)c, 1, 1), map_w, map_x, args);
+    return thn_launch_status("mx4_stream");
+}
+
+template <typename RT, int MR>
+int launch_rows(const Args& args, const void* codes, long long padded, int out_dtype, int bias_dtype, cudaStream_t stream) {
+    CUtensorMap map_w, map_x;
+    bool made = map_unpacked(&map_w, codes, args.N, padded, BW);
+    if (sizeof(RT) == 1) made = made && map_unpacked(&map_x, args.x, args.M, padded, Shape<RT, MR>::NX);
+    else map_x = map_w;
+    if (!made) {
+        thn_set_error("mx4_stream: cuTensorMapEncodeTiled failed for M=%d N=%d K=%d", args.M, args.N, args.K);
+        return THN_BAD_ARGUMENT;
+    }
+    if (out_dtype == THN_F32)
+        return bias_dtype == THN_F32 ? launch<RT, MR, float, float>(map_w, map_x, args, stream)
+                                     : launch<RT, MR, float, __nv_bfloat16>(map_w, map_x, args, stream);
+    return bias_dtype == THN_F32 ? launch<RT, MR, __nv_bfloat16, float>(map_w, map_x, args, stream)
+                                 : launch<RT, MR, __nv_bfloat16, __nv_bfloat16>(map_w, map_x, args, stream);
+}
+
+}  // namespace
+
+// How many rows of a type (THN_F32, THN_BF16, 2: 4 bits) thn_mx4_stream takes.
+THN_API int thn_mx4_stream_rows(int x_type) { return x_type == THN_F32 ? 32 : 64; }
+
+// out [M, N] of out_dtype = x [M, K] @ w [N, K]^T (+ bias [N] of bias_dtype, or null).
+//   x          [M, K] of x_type; 2: codes [M, padded / 2] with x_scales (mx4.cuh)
+//   codes, scales: W
+// All but bias and out 16-byte aligned; 4-bit codes 32-byte aligned.  err: device error word (THN_ERR_WAIT_TIMEOUT if a wait
+// gave up).  skip_loads: 0; otherwise no operand is loaded, so that the waits run out (for the test of the waits only).
+THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* x_scales, int x_type, const void* codes, const void* scales,
+                           const void* bias, int bias_dtype, int M, int N, int K, int skip_loads, int* err, cudaStream_t stream) {
+    THN_CHECK_ARG(x_type >= 0 && x_type <= 2 && (out_dtype == THN_F32 || out_dtype == THN_BF16) && (bias_dtype == THN_F32 || bias_dtype == THN_BF16),
+                  "mx4_stream: unknown type %d, %d or %d", x_type, out_dtype, bias_dtype);
+    THN_UNSUPPORTED_IF(M < 1 || M > thn_mx4_stream_rows(x_type) || N < 1 || K < 1 || K > (1 << 30), "mx4_stream: M=%d N=%d K=%d not supported", M, N, K);
+    THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 && (((uintptr_t)scales | (uintptr_t)x_scales) & 15) == 0,
+                  "mx4_stream: codes must be 32-byte and scales 16-byte aligned");
+    const long long padded = mx4_padded(K);
+    Args args = {};
+    args.out = out;
+    args.x = x;
+    args.x_scales = (const uint8_t*)x_scales;
+    args.w_scales = (const uint8_t*)scales;
+    args.bias = bias;
+    args.M = M;
+    args.N = N;
+    args.K = K;
+    args.chunks = (int)(padded / BK);
+    args.vector = ((uintptr_t)x & 15) == 0 && K % (x_type == THN_F32 ? 4 : 8) == 0;
+    args.err = err;
+    args.skip_loads = skip_loads;
+#define GO(RT, MR) return launch_rows<RT, MR>(args, codes, padded, out_dtype, bias_dtype, stream)
+    if (x_type == THN_F32) {
+        if (M <= 8) GO(float, 8);
+        if (M <= 16) GO(float, 16);
+        GO(float, 32);
+    }
+    if (x_type == THN_BF16) {
+        if (M <= 8) GO(__nv_bfloat16, 8);
+        if (M <= 16) GO(__nv_bfloat16, 16);
+        if (M <= 32) GO(__nv_bfloat16, 32);
+        GO(__nv_bfloat16, 64);
+    }
+    if (M <= 16) GO(uint8_t, 16);
+    if (M <= 32) GO(uint8_t, 32);
+    GO(uint8_t, 64);
+#undef GO
+}

@@ -1,0 +1,176 @@
+// What the block-scaled products on tensor memory share: barriers, copies, descriptors.
+#pragma once
+
+#include <cuda.h>
+
+#include "mx4.cuh"
+
+namespace {
+
+constexpr unsigned long long kWaitLimitNs = 20ull * 1000 * 1000;   // a wait gives up after 20 ms
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// Bounded wait for the phase with the given parity.  Returns false when it gave up.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
+    const uint32_t addr = smem_addr(bar);
+    WaitClock clock;
+    for (int spin = 0;; ++spin) {
+        uint32_t done;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((spin & 15) == 15 && clock.ran_out(kWaitLimitNs)) return false;
+    }
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(smem_addr(dst)), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");
+}
+
+// Shared-memory matrix descriptor of a K-major tile in rows of 128 bytes with the 128-byte swizzle (see gemm_tcgen05.cu).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// The same of 512 bytes of scales: 32 rows of 16 bytes, no swizzle, eight rows (128 bytes) a step.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// 512 bytes of scales to four columns of tensor memory, the same in all four quarters of its lanes.
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Element types of kind::mxf8f6f4
+constexpr uint32_t kE4M3 = 0, kE2M1 = 5;
+// Instruction descriptor of the block-scaled kinds: which of a word's four scale bytes at bits 4-5 (B) and 29-30 (A), element
+// types at 7 (A) and 10 (B), N / 8 at 17, scales that are powers of two (bit 23), M / 16 at 24; both operands K-major.
+__host__ __device__ constexpr uint32_t scaled_instr(uint32_t a_type, uint32_t b_type, int m, int n) {
+    return (a_type << 7) | (b_type << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t with_scale_byte(uint32_t instr, uint32_t k) { return instr | (k << 4) | (k << 29); }
+
+// 32 columns of the sum: D += A B with 8-bit containers, one scale byte a row
+__device__ __forceinline__ void mma_scaled(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instr, uint32_t a_scales,
+                                           uint32_t b_scales, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n"
+        "}\n"
+        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instr), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// 16 or 8 consecutive columns of this warp's 32 lanes; the caller waits with tmem_wait_load().
+__device__ __forceinline__ void tmem_load_8(uint32_t taddr, float* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// ---- rows as they are, as sums of 8-bit floats.
+//
+// A block of 32 entries with its largest magnitude in [2^e, 2^(e+1)) is brought to [2^7, 2^8) by the scale 2^(e-7); its entries
+// are rounded to e4m3 (four significant bits, down to 2^-9), what that leaves is brought up by 2^4 and rounded again, and so on.
+// Two terms hold a bfloat16 (eight bits) exactly down to 2^-13 of the block's largest entry, and below that to 2^-21 of it; six hold a
+// float32 (24 bits), down to 2^-13, and below that to 2^-37.  A term's products cost the tensor core half of a bfloat16's.
+template <typename T>
+constexpr int kTerms = sizeof(T) == 2 ? 2 : 6;
+
+// The scale byte of a block's first term, from its largest magnitude's bits; 255: not a number.
+__device__ __forceinline__ uint32_t row_scale_byte(uint32_t top_bits) {
+    const uint32_t field = top_bits >> 23;
+    return field == 255 ? 255 : field > 7 ? field - 7 : 0;
+}
+// The scale byte of term t: 2^-4 for each, as far as there are bytes.
+__device__ __forceinline__ uint32_t term_scale_byte(uint32_t first, int t) { return first == 255 ? 255 : first > 4u * t ? first - 4 * t : 0; }
+
+// Eight entries, scaled for a term, to that term's bytes; v becomes what is left, scaled by `next`.
+__device__ __forceinline__ uint2 next_term(float (&v)[8], float next) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint16_t pair;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+        uint32_t back;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(pair));
+        float lo, hi;
+        asm("{\n.reg .f16 a, b;\nmov.b32 {a, b}, %2;\ncvt.f32.f16 %0, a;\ncvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(back));
+        v[2 * i] = (v[2 * i] - lo) * next;
+        v[2 * i + 1] = (v[2 * i + 1] - hi) * next;
+        w[i >> 1] |= (uint32_t)pair << (16 * (i & 1));
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &result) != cudaSuccess ||
+            result != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return fn;
+}
+
+// Codes [rows][padded / 2] for boxes of 128 columns x box_rows, which arrive as 8-bit containers of 16 bytes for 16 entries, the
+// first eight of them filled (and counted by the barrier).
+inline bool map_unpacked(CUtensorMap* map, const void* codes, long long rows, long long padded, int box_rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)padded, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)padded / 2};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(codes), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Rows of `width` bytes for boxes of 128 bytes x box_rows.
+inline bool map_bytes(CUtensorMap* map, const void* base, long long rows, long long width, int box_rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)width};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace

@@ -153,6 +153,9 @@ _SIGNATURES = {
     "thn_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_arrange": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p],
     "thn_mx4_linear": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "thn_mx4_stream_rows": [c_int],
+    "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                       c_void_p],
     "thn_gemm_f32": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "thn_linear_skinny_bf16": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "thn_linear_skinny_supported": [c_int, c_int],
@@ -1094,6 +1097,10 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
             raise KernelError(f"linear_mx4: a bias {tuple(bias.shape)} on {bias.device} for {weight.rows} outputs on {data.device}")
     bias_code = 0 if bias is None else _code(bias, "linear_mx4 bias")
     out = torch.empty((x.shape[0], weight.rows), dtype=out_dtype, device=data.device)
+    if 0 < x.shape[0] <= lib().thn_mx4_stream_rows(kind) and weight.rows:
+        _call("thn_mx4_stream", _ptr(out), DTYPE_CODE[out_dtype], _ptr(data), _ptr(x.scales) if quantized else None, kind, _ptr(weight.codes),
+              _ptr(weight.scales), _ptr(bias), bias_code, x.shape[0], weight.rows, weight.columns, 0, _ptr(err), _stream())
+        return out
     _call("thn_mx4_linear", _ptr(out), DTYPE_CODE[out_dtype], _ptr(data), _ptr(x.scales) if quantized else None, kind, _ptr(weight.codes),
           _ptr(weight.scales), _ptr(bias), bias_code, x.shape[0], weight.rows, weight.columns, _ptr(err), _stream())
     return out
