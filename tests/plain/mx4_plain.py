@@ -44,11 +44,3 @@ def stored(codes, columns):
         flat = np.pad(flat, ((0, 0), (0, 1)))
     return (flat[:, 0::2] | flat[:, 1::2] << 4).astype(np.uint8)
 
-
-def block_tops(x):
-    """For every entry of float64 [rows, columns], the largest magnitude of its block."""
-    rows, columns = x.shape
-    v = np.zeros((rows, -(-columns // BLOCK) * BLOCK))
-    v[:, :columns] = np.abs(x)
-    top = v.reshape(rows, -1, BLOCK).max(axis=2)
-    return np.repeat(top, BLOCK, axis=1)[:, :columns]

@@ -36,11 +36,15 @@ def rows_of(rows, columns, dtype, seed, spread=1.0):
 
 
 def weight_of(n, k, seed):
-    """(the library's matrix, its values in float64)."""
-    g = np.random.default_rng(seed)
-    codes, scales = plain.quantize(g.standard_normal((n, k)) * np.exp2(g.integers(-6, 2, (n, 1))))
-    stored = torch.from_numpy(plain.stored(codes, k)).cuda()
-    return ops.mx4_from_parts(stored, torch.from_numpy(scales).cuda(), k), plain.values(codes, scales, k)
+    """(the library's matrix, its values in float64 on the device): any codes, scales of 2^-9 to 2^-1."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    blocks = -(-k // 32)
+    stored = torch.randint(0, 256, (n, -(-k // 2)), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.randint(118, 127, (n, blocks), generator=g, device="cuda", dtype=torch.uint8)
+    codes = torch.stack((stored & 15, stored >> 4), dim=-1).flatten(1)[:, :k].long()
+    values = torch.tensor(plain.MAGNITUDES, device="cuda")[codes & 7] * torch.where(codes >= 8, -1.0, 1.0).double()
+    values *= torch.exp2(scales.double() - 127).repeat_interleave(32, dim=1)[:, :k]
+    return ops.mx4_from_parts(stored, scales, k), values
 
 
 def scale_bytes(q):
@@ -115,13 +119,21 @@ def test_stored_parts_keep_every_code_and_scale(columns):
     np.testing.assert_array_equal(ops.dequantize_mx4(q).cpu().numpy(), want)
 
 
-def bound(x, w, y, k, x_dtype, out_dtype, bias):
+def tops(x):
+    """For every entry of float64 [rows, columns], the largest magnitude of its block."""
+    blocks = torch.nn.functional.pad(x.abs(), (0, -x.shape[1] % 32)).unflatten(1, (-1, 32))
+    return blocks.amax(dim=2).repeat_interleave(32, dim=1)[:, :x.shape[1]]
+
+
+def bound(x, w, y, x_dtype, out_dtype, bias):
     """How far a product may be off, entry by entry (see the top of this file)."""
-    sums = np.abs(x) @ np.abs(w).T
-    e = k * 2.0 ** -23 * (sums + (0 if bias is None else np.abs(bias)))
+    sums = x.abs() @ w.abs().t()
+    if bias is not None:
+        sums += bias.abs()
+    e = x.shape[1] * 2.0 ** -23 * sums
     if x_dtype is not None:
-        e += ROW_STEP[x_dtype] * (plain.block_tops(x) @ np.abs(w).T)
-    return e + HALF_STEP[out_dtype] * (np.abs(y) + e)
+        e += ROW_STEP[x_dtype] * (tops(x) @ w.abs().t())
+    return e + HALF_STEP[out_dtype] * (y.abs() + e)
 
 
 def check_product(m, n, k, x_dtype, out_dtype, with_bias=False, quantized=False, seed=0, spread=1.0):
@@ -133,13 +145,12 @@ def check_product(m, n, k, x_dtype, out_dtype, with_bias=False, quantized=False,
     got = ops.linear_mx4(given, weight, out_dtype=out_dtype, bias=bias, err=err)
     assert got.dtype == out_dtype and tuple(got.shape) == (m, n)
     ops.raise_on_device_error(err, "test")
-    x64 = plain.values(*plain.quantize(as64(x)), k) if quantized else as64(x)
-    b64 = None if bias is None else as64(bias)
-    y = x64 @ w.T + (0 if bias is None else b64)
-    error = np.abs(as64(got) - y)
-    limit = bound(x64, w, y, k, None if quantized else x_dtype, out_dtype, b64)
-    assert (error <= limit).all(), (error / np.maximum(limit, 1e-300)).max()
-    return given, weight, got
+    x64 = torch.from_numpy(plain.values(*plain.quantize(as64(x)), k)).cuda() if quantized else x.double()
+    b64 = None if bias is None else bias.double()
+    y = x64 @ w.t() + (0 if bias is None else b64)
+    error = (got.double() - y).abs()
+    limit = bound(x64, w, y, None if quantized else x_dtype, out_dtype, b64)
+    assert (error <= limit).all(), (error / limit.clamp(min=1e-300)).max()
 
 
 SIZES = [(1, 1, 1), (1, 128, 256), (1, 2560, 2560), (2, 100, 32), (3, 515, 1096), (5, 1333, 1000), (8, 640, 2432), (9, 129, 4100), (16, 256, 640),
@@ -164,6 +175,14 @@ def test_product_of_quantized_rows(m, n, k, dtype):
 def test_product_with_the_other_output_type(m, quantized):
     check_product(m, 260, 500, torch.bfloat16, torch.float32, quantized=quantized)
     check_product(m, 260, 500, torch.float32, torch.bfloat16, quantized=quantized)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 19100, 2050), (8, 19100, 1300), (3, 9700, 2600), (5, 200, 20000), (20, 19100, 700), (60, 9700, 1000)])
+def test_product_of_many_pieces_of_k_a_block(m, n, k, dtype):
+    """Blocks that go round their ring of stages several times."""
+    check_product(m, n, k, dtype, dtype)
+    check_product(m, n, k, dtype, dtype, quantized=True)
 
 
 @pytest.mark.parametrize("spread", [2.0 ** -60, 2.0 ** 60])
@@ -277,7 +296,7 @@ def test_a_wait_that_runs_out_is_reported(quantized):
     err = ops.new_error_word("cuda")
     data, scales, kind = (q.codes, q.scales, 2) if quantized else (x, None, 1)
     ops._call("thn_mx4_stream", out.data_ptr(), 0, data.data_ptr(), ops._ptr(scales), kind, weight.codes.data_ptr(), weight.scales.data_ptr(), None, 0,
-              5, 300, 640, 1, err.data_ptr(), ops._stream())
+              None, 0, 5, 300, 640, 1, err.data_ptr(), ops._stream())
     with pytest.raises(ops.KernelError, match="gave up"):
         ops.raise_on_device_error(err, "test")
     assert torch.isnan(out).all()

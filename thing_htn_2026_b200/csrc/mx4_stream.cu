@@ -3,8 +3,10 @@
 //  * 128 rows of W are the wide operand of tcgen05.mma (kind::mxf8f6f4, scales applied by the tensor core), the rows of x its
 //    narrow one.  W comes by TMA, which spreads its 4-bit codes over 8-bit containers as it copies, so no thread touches a weight;
 //    its scales come as 512 bytes for 128 rows and 128 columns, in the order of tensor memory, and go there by tcgen05.cp.
-//  * Rows in bfloat16 or float32 become two or six terms of 8-bit floats in the kernel (mx4_tcgen05.cuh), a column of the narrow
-//    operand each; their sums are added at the end.  Rows in 4 bits are brought as W is.
+//  * Rows in bfloat16 or float32 become two or six terms of 8-bit floats (mx4_tcgen05.cuh), a column of the narrow operand each;
+//    their sums are added at the end.  Up to kConverted rows this happens in the kernel, a half warp for a row's 128
+//    columns, beside the copies of W; more rows are prepared by a kernel of their own (mx4_terms_kernel), since every block would
+//    do it again, and come by TMA.  Rows in 4 bits are brought as W is.
 //  * A tile of 128 outputs is cut along K among the blocks of a cluster, whose partial sums meet in distributed shared memory
 //    and are added in ascending order: no scratch memory, no counters, the same result every time.
 //  * Two blocks a multiprocessor while the rows are few: the bytes in flight cover the memory's latency, and one block's
@@ -22,10 +24,12 @@ constexpr uint32_t kWSmem = BW * BK, kWBytes = kWSmem / 2;     // in shared memo
 constexpr int kMaxStages = 12;
 constexpr int kMaxCluster = 8;
 
-// RT: how the rows come (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for
+constexpr int kConverted = 8;                          // rows that the kernel itself brings to terms
+
+// RT: the rows' type (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for
 template <typename RT, int MR>
 struct Shape {
-    static constexpr bool kQuantized = sizeof(RT) == 1;
+    static constexpr bool kQuantized = sizeof(RT) == 1, kConverts = !kQuantized && MR <= kConverted;
     static constexpr int kT = kQuantized ? 1 : kTerms<RT>;
     static constexpr int NX = MR * kT < 16 ? 16 : MR * kT;           // columns of the product
     static constexpr int kXAtoms = (NX + 127) / 128;
@@ -45,8 +49,8 @@ struct Shape {
 
 struct Args {
     void* out;
-    const void* x;                // [M, K] of RT; 4 bits: its map
-    const uint8_t* x_scales;
+    const void* x;                // [M, K] of RT
+    const uint8_t* x_scales;      // 4 bits, and terms that were prepared
     const uint8_t* w_scales;
     const void* bias;
     int M, N, K, chunks, vector;  // vector: x's rows are whole aligned 16-byte pieces
@@ -73,43 +77,6 @@ __device__ __forceinline__ void store_to_block(float* mine, uint32_t rank, float
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
-// Eight neighbouring entries of a row as they lie in memory; what lies behind the last column is zero.
-template <typename RT>
-struct Eight {
-    uint4 a, b;
-    __device__ __forceinline__ void load(const RT* row, int c, int K, bool vector) {
-        if (vector && c + 8 <= K) {
-            a = *reinterpret_cast<const uint4*>(row + c);
-            if constexpr (sizeof(RT) == 4) b = *reinterpret_cast<const uint4*>(row + c + 4);
-        } else {
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = c + i < K ? __float_as_uint(to_f32<RT>(row[c + i])) : 0u;
-            if constexpr (sizeof(RT) == 4) {
-                a = make_uint4(w[0], w[1], w[2], w[3]);
-                b = make_uint4(w[4], w[5], w[6], w[7]);
-            } else {
-                a = make_uint4(w[0] >> 16 | (w[1] & 0xffff0000u), w[2] >> 16 | (w[3] & 0xffff0000u), w[4] >> 16 | (w[5] & 0xffff0000u),
-                               w[6] >> 16 | (w[7] & 0xffff0000u));
-            }
-        }
-    }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        if constexpr (sizeof(RT) == 4) {
-            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
-        } else {
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        }
-    }
-};
-
 template <typename RT, int MR, typename OutT, typename BiasT>
 __global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                               const Args a) {
@@ -130,7 +97,7 @@ __global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_const
     const int c0 = (int)((long long)a.chunks * rank / n_ranks), c1 = (int)((long long)a.chunks * (rank + 1) / n_ranks);
 
     if (warp == 0) {
-        if (lane < S::kStages) mbar_init(full + lane, S::kQuantized ? 1 : 5);      // the copies, and the four warps that bring x
+        if (lane < S::kStages) mbar_init(full + lane, S::kConverts ? 5 : 1);      // the copies, and the four warps that bring x
         else if (lane < 2 * S::kStages) mbar_init(empty + (lane - S::kStages), 1);
         else if (lane == 2 * S::kStages) mbar_init(acc_full, 1);
         if (lane == 0) *give_up = 0;
@@ -150,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_const
     if (warp == 0 && lane == 0) {
         // ---- TMA producer: W of the first stages before the wait for the kernel that makes x
         const int n = a.skip_loads ? 0 : c1 - c0;
-        const uint32_t bytes = kWBytes + kMx4AtomBytes + (S::kQuantized ? S::kXSmem / 2 + kMx4AtomBytes * S::kXAtoms : 0);
+        const uint32_t bytes = kWBytes + kMx4AtomBytes + (S::kConverts ? 0 : S::kXSmem / (S::kQuantized ? 2 : 1) + kMx4AtomBytes * S::kXAtoms);
         auto load_w = [&](int s, int c) {
             unsigned char* dst = tiles + (size_t)s * S::kStageStride;
             mbar_expect_tx(full + s, bytes);
@@ -158,10 +125,13 @@ __global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_const
             bulk_load(dst + kWSmem + S::kXSmem, a.w_scales + ((long long)tile * a.chunks + c) * kMx4AtomBytes, kMx4AtomBytes, full + s);
         };
         auto load_x = [&](int s, int c) {
-            if constexpr (S::kQuantized) {
+            if constexpr (!S::kConverts) {
                 unsigned char* dst = tiles + (size_t)s * S::kStageStride;
                 tma_load_2d(dst + kWSmem, &map_x, full + s, c * BK, 0);
-                bulk_load(dst + kWSmem + S::kXSmem + kMx4AtomBytes, a.x_scales + (long long)c * kMx4AtomBytes, kMx4AtomBytes, full + s);
+#pragma unroll
+                for (int j = 0; j < S::kXAtoms; ++j)
+                    bulk_load(dst + kWSmem + S::kXSmem + (1 + j) * kMx4AtomBytes, a.x_scales + ((long long)j * a.chunks + c) * kMx4AtomBytes,
+                              kMx4AtomBytes, full + s);
             }
         };
         const int early = min(S::kStages, n);
@@ -206,64 +176,54 @@ __global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_const
     } else if (warp >= 2) {
         pdl_wait();
         const int quarter = warp & 3;
-        if constexpr (!S::kQuantized) {
-            // ---- rows of x to terms: a thread takes eight columns of every eighth row
-            const int t = threadIdx.x - 64, piece = t & 15, first = t >> 4;
-            constexpr int kPasses = MR / 8;
-            Eight<RT> held[kPasses];
-            auto fetch = [&](int i) {
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
-                    const int row = first + 8 * p;
-                    if (row < a.M) held[p].load(static_cast<const RT*>(a.x) + (long long)row * a.K, (c0 + i) * BK + piece * 8, a.K, a.vector);
-                }
+        if constexpr (S::kConverts) {
+            // ---- rows of x to terms.  An item is a row's 128 columns of a chunk; the eight half warps take every eighth, a thread eight columns, and
+            // have kAhead of theirs under way.  All four warps go through every chunk, with an item of it or without, so that none is more than
+            // a round of the ring ahead of the products (a barrier's parity tells one round from the next, no more).
+            constexpr int kAhead = 4;
+            const int piece = threadIdx.x & 15, items = (c1 - c0) * a.M;
+            int item = (threadIdx.x - 64) >> 4;                      // this half warp's next one
+            Eight<RT> held[kAhead];
+            auto fetch = [&](int which, Eight<RT>& e) {
+                const int i = which / a.M, row = which - i * a.M;
+                if (which < items) e.load(static_cast<const RT*>(a.x) + (long long)row * a.K, (c0 + i) * BK + piece * 8, a.K, a.vector);
             };
-            if (c1 > c0) fetch(0);
-            for (int i = 0; i < c1 - c0 && !*give_up; ++i) {
+#pragma unroll
+            for (int h = 0; h < kAhead; ++h) fetch(item + 8 * h, held[h]);
+            for (int i = 0; i < c1 - c0; ++i) {
+                if (__any_sync(0xffffffffu, *give_up)) break;        // all lanes together
                 const int s = i % S::kStages;
                 if (i >= S::kStages && !__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / S::kStages) & 1) ^ 1))) {
                     if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
                     *give_up = 1;
                     break;
                 }
-                unsigned char* dst = tiles + (size_t)s * S::kStageStride + kWSmem;
-                unsigned char* scales = dst + S::kXSmem + kMx4AtomBytes;
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
-                    const int row = first + 8 * p;
-                    if (8 * p >= a.M) break;                        // the same for all
-                    float v[8];
-                    if (row < a.M) {
-                        held[p].get(v);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-                    }
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+                const bool there = item < (i + 1) * a.M;             // (at most one a chunk: no more than eight rows)
+                if (__any_sync(0xffffffffu, there)) {
+                    uint32_t top = there ? held[0].top() : 0;
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    if (row >= a.M) continue;
-                    const uint32_t b = row_scale_byte(top);
-                    const float factor = __uint_as_float((254 - min(b, 253u)) << 23);
+                    if (there) {
+                        unsigned char* dst = tiles + (size_t)s * S::kStageStride + kWSmem;
+                        const int row = item - i * a.M;
+                        const uint32_t b = row_scale_byte(top);
+                        held[0].terms(b, [&](int term, uint2 bytes) {
+                            const int column = term * MR + row;
+                            *reinterpret_cast<uint2*>(dst + column * BK + (((piece >> 1) ^ (column & 7)) << 4) + (piece & 1) * 8) = bytes;
+                            if ((piece & 3) == 0)
+                                dst[S::kXSmem + kMx4AtomBytes + (column & 31) * 16 + (column >> 5) * 4 + (piece >> 2)] = (uint8_t)term_scale_byte(b, term);
+                        });
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = b == 255 ? 0.f : v[j] * factor;
-#pragma unroll
-                    for (int term = 0; term < S::kT; ++term) {
-                        const uint32_t here = term_scale_byte(b, term), after = term_scale_byte(b, term + 1);
-                        const uint2 bytes = next_term(v, __uint_as_float((127 + here - after) << 23));
-                        const int column = term * MR + row;
-                        *reinterpret_cast<uint2*>(dst + column * BK + (((piece >> 1) ^ (column & 7)) << 4) + (piece & 1) * 8) = bytes;
-                        if ((piece & 3) == 0)
-                            scales[(column >> 7) * kMx4AtomBytes + (column & 31) * 16 + ((column & 127) >> 5) * 4 + (piece >> 2)] = (uint8_t)here;
+                        for (int h = 0; h + 1 < kAhead; ++h) held[h] = held[h + 1];
+                        fetch(item + 8 * kAhead, held[kAhead - 1]);
+                        item += 8;
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
                 if (lane == 0) mbar_arrive(full + s);
-                if (i + 1 < c1 - c0) fetch(i + 1);
             }
+            __syncwarp();
         }
         // ---- this block's partial sums, row by row, to the rows' owners
         const int r = quarter * 32 + lane;
@@ -335,6 +295,40 @@ __global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_const
     }
 }
 
+// Rows as terms of 8-bit floats: term t of row r at [t * plane + r], its scales as mx4.cuh lays out those of such a matrix.
+// A thread takes eight columns.
+template <typename RT>
+__global__ void __launch_bounds__(256) mx4_terms_kernel(uint8_t* __restrict__ bytes, uint8_t* __restrict__ scales, const RT* __restrict__ x, int M, int K,
+                                                        int padded, int plane, bool vector) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int pieces = padded / 8;
+    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int row = (int)(unit / pieces), piece = (int)(unit - (long long)row * pieces);
+    const bool there = row < M;
+    Eight<RT> e;
+    if (there) e.load(x + (long long)row * K, piece * 8, K, vector);
+    uint32_t top = there ? e.top() : 0;
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t b = row_scale_byte(top);
+    // the sixteen threads' four scale bytes of the first term as one word
+    uint32_t four = b << (8 * ((threadIdx.x >> 2) & 3));
+    four |= __shfl_xor_sync(0xffffffffu, four, 4);
+    four |= __shfl_xor_sync(0xffffffffu, four, 8);
+    if (!there) return;
+    e.terms(b, [&](int term, uint2 v) {
+        const long long at = (long long)term * plane + row;
+        *reinterpret_cast<uint2*>(bytes + at * padded + piece * 8) = v;
+        if ((threadIdx.x & 15) == 0) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w |= term_scale_byte(four >> (8 * i) & 255, term) << (8 * i);
+            *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(at, piece / 16, padded / kMx4Atom)) = w;
+        }
+    });
+}
+
 // The blocks of a cluster: as many as the resident blocks leave for a tile, two a multiprocessor where they fit, and no
 // more than there are pieces of K.
 template <typename RT, int MR>
@@ -363,12 +357,21 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Args& args,
     return thn_launch_status("mx4_stream");
 }
 
+// terms: for the rows' terms, kT * MR rows of `padded` bytes, then their scales (null where the kernel brings them itself)
 template <typename RT, int MR>
-int launch_rows(const Args& args, const void* codes, long long padded, int out_dtype, int bias_dtype, cudaStream_t stream) {
+int launch_rows(Args args, const void* codes, long long padded, void* terms, int out_dtype, int bias_dtype, cudaStream_t stream) {
+    using S = Shape<RT, MR>;
     CUtensorMap map_w, map_x;
     bool made = map_unpacked(&map_w, codes, args.N, padded, BW);
-    if (sizeof(RT) == 1) made = made && map_unpacked(&map_x, args.x, args.M, padded, Shape<RT, MR>::NX);
-    else map_x = map_w;
+    if constexpr (S::kQuantized) made = made && map_unpacked(&map_x, args.x, args.M, padded, S::NX);
+    else if constexpr (!S::kConverts) {
+        uint8_t* bytes = static_cast<uint8_t*>(terms);
+        uint8_t* scales = bytes + (long long)S::kT * MR * padded;
+        thn_launch(mx4_terms_kernel<RT>, (unsigned)(((long long)args.M * (padded / 8) + 255) / 256), 256, 0, stream, bytes, scales, (const RT*)args.x,
+                   args.M, args.K, (int)padded, MR, (bool)args.vector);
+        args.x_scales = scales;
+        made = made && map_bytes(&map_x, bytes, S::kT * MR, padded, S::NX);
+    } else map_x = map_w;
     if (!made) {
         thn_set_error("mx4_stream: cuTensorMapEncodeTiled failed for M=%d N=%d K=%d", args.M, args.N, args.K);
         return THN_BAD_ARGUMENT;
@@ -380,23 +383,36 @@ int launch_rows(const Args& args, const void* codes, long long padded, int out_d
                                  : launch<RT, MR, __nv_bfloat16, __nv_bfloat16>(map_w, map_x, args, stream);
 }
 
+// the rows that a block has room for
+int room_for(int M) { return M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+
 }  // namespace
 
 // How many rows of a type (THN_F32, THN_BF16, 2: 4 bits) thn_mx4_stream takes.
 THN_API int thn_mx4_stream_rows(int x_type) { return x_type == THN_F32 ? 32 : 64; }
 
+// The bytes of `terms` that M rows of a type need.
+THN_API long long thn_mx4_stream_scratch_bytes(int x_type, int M, int K) {
+    if (x_type == 2 || M <= kConverted) return 0;
+    const long long rows = (long long)room_for(M) * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
+    return rows * padded + (rows + 127) / 128 * (padded / kMx4Atom) * kMx4AtomBytes;
+}
+
 // out [M, N] of out_dtype = x [M, K] @ w [N, K]^T (+ bias [N] of bias_dtype, or null).
 //   x          [M, K] of x_type; 2: codes [M, padded / 2] with x_scales (mx4.cuh)
-//   codes, scales: W
-// All but bias and out 16-byte aligned; 4-bit codes 32-byte aligned.  err: device error word (THN_ERR_WAIT_TIMEOUT if a wait
-// gave up).  skip_loads: 0; otherwise no operand is loaded, so that the waits run out (for the test of the waits only).
+//   codes, scales: W;  terms: scratch of thn_mx4_stream_scratch_bytes
+// Scales and terms 16-byte, 4-bit codes 32-byte aligned.  err: device error word (THN_ERR_WAIT_TIMEOUT if a wait gave up).
+// skip_loads: 0; otherwise no operand is loaded, so that the waits run out (for the test of the waits only).
 THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* x_scales, int x_type, const void* codes, const void* scales,
-                           const void* bias, int bias_dtype, int M, int N, int K, int skip_loads, int* err, cudaStream_t stream) {
+                           const void* bias, int bias_dtype, void* terms, long long terms_bytes, int M, int N, int K, int skip_loads, int* err,
+                           cudaStream_t stream) {
     THN_CHECK_ARG(x_type >= 0 && x_type <= 2 && (out_dtype == THN_F32 || out_dtype == THN_BF16) && (bias_dtype == THN_F32 || bias_dtype == THN_BF16),
                   "mx4_stream: unknown type %d, %d or %d", x_type, out_dtype, bias_dtype);
-    THN_UNSUPPORTED_IF(M < 1 || M > thn_mx4_stream_rows(x_type) || N < 1 || K < 1 || K > (1 << 30), "mx4_stream: M=%d N=%d K=%d not supported", M, N, K);
-    THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 && (((uintptr_t)scales | (uintptr_t)x_scales) & 15) == 0,
-                  "mx4_stream: codes must be 32-byte and scales 16-byte aligned");
+    THN_UNSUPPORTED_IF(M < 1 || M > thn_mx4_stream_rows(x_type) || N < 1 || K < 1 || K > (1 << 24), "mx4_stream: M=%d N=%d K=%d not supported", M, N, K);
+    THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 &&
+                  (((uintptr_t)scales | (uintptr_t)x_scales | (uintptr_t)terms) & 15) == 0, "mx4_stream: codes must be 32-byte, scales and terms 16-byte aligned");
+    THN_CHECK_ARG(terms_bytes >= thn_mx4_stream_scratch_bytes(x_type, M, K), "mx4_stream: %lld bytes of scratch, %lld needed", terms_bytes,
+                  thn_mx4_stream_scratch_bytes(x_type, M, K));
     const long long padded = mx4_padded(K);
     Args args = {};
     args.out = out;
@@ -408,23 +424,24 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     args.N = N;
     args.K = K;
     args.chunks = (int)(padded / BK);
-    args.vector = ((uintptr_t)x & 15) == 0 && K % (x_type == THN_F32 ? 4 : 8) == 0;
+    args.vector = ((uintptr_t)x & 15) == 0 && K % 8 == 0;
     args.err = err;
     args.skip_loads = skip_loads;
-#define GO(RT, MR) return launch_rows<RT, MR>(args, codes, padded, out_dtype, bias_dtype, stream)
+#define GO(RT, MR) return launch_rows<RT, MR>(args, codes, padded, terms, out_dtype, bias_dtype, stream)
+    const int room = room_for(M);
     if (x_type == THN_F32) {
-        if (M <= 8) GO(float, 8);
-        if (M <= 16) GO(float, 16);
+        if (room == 8) GO(float, 8);
+        if (room == 16) GO(float, 16);
         GO(float, 32);
     }
     if (x_type == THN_BF16) {
-        if (M <= 8) GO(__nv_bfloat16, 8);
-        if (M <= 16) GO(__nv_bfloat16, 16);
-        if (M <= 32) GO(__nv_bfloat16, 32);
+        if (room == 8) GO(__nv_bfloat16, 8);
+        if (room == 16) GO(__nv_bfloat16, 16);
+        if (room == 32) GO(__nv_bfloat16, 32);
         GO(__nv_bfloat16, 64);
     }
-    if (M <= 16) GO(uint8_t, 16);
-    if (M <= 32) GO(uint8_t, 32);
+    if (room <= 16) GO(uint8_t, 16);
+    if (room == 32) GO(uint8_t, 32);
     GO(uint8_t, 64);
 #undef GO
 }

@@ -87,7 +87,7 @@ __device__ __forceinline__ void mma_scaled(uint32_t tmem_d, uint64_t a_desc, uin
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-// 16 or 8 consecutive columns of this warp's 32 lanes; the caller waits with tmem_wait_load().
+// Eight consecutive columns of this warp's 32 lanes; the caller waits with tmem_wait_load().
 __device__ __forceinline__ void tmem_load_8(uint32_t taddr, float* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
@@ -113,23 +113,105 @@ __device__ __forceinline__ uint32_t row_scale_byte(uint32_t top_bits) {
 // The scale byte of term t: 2^-4 for each, as far as there are bytes.
 __device__ __forceinline__ uint32_t term_scale_byte(uint32_t first, int t) { return first == 255 ? 255 : first > 4u * t ? first - 4 * t : 0; }
 
-// Eight entries, scaled for a term, to that term's bytes; v becomes what is left, scaled by `next`.
-__device__ __forceinline__ uint2 next_term(float (&v)[8], float next) {
-    uint32_t w[2] = {0, 0};
+// Eight neighbouring entries of a row, as they lie in memory.
+template <typename T>
+struct Eight;
+
+template <>
+struct Eight<__nv_bfloat16> {
+    uint4 raw;
+    // what lies behind the last column is zero; vector: the row is whole aligned 16-byte pieces
+    __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int K, bool vector) {
+        if (vector) {
+            raw = c < K ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+        } else {
+            const uint16_t* bits = reinterpret_cast<const uint16_t*>(row);
+            uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint16_t pair;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-        uint32_t back;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(pair));
-        float lo, hi;
-        asm("{\n.reg .f16 a, b;\nmov.b32 {a, b}, %2;\ncvt.f32.f16 %0, a;\ncvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(back));
-        v[2 * i] = (v[2 * i] - lo) * next;
-        v[2 * i + 1] = (v[2 * i + 1] - hi) * next;
-        w[i >> 1] |= (uint32_t)pair << (16 * (i & 1));
+            for (int i = 0; i < 4; ++i)
+                w[i] = (c + 2 * i < K ? bits[c + 2 * i] : 0u) | (c + 2 * i + 1 < K ? (uint32_t)bits[c + 2 * i + 1] << 16 : 0u);
+            raw = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
-    return make_uint2(w[0], w[1]);
-}
+    // the largest magnitude, as the bits of a float32
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, (&raw.x)[i] & 0x7fff7fffu);
+        return max(m << 16, m & 0xffff0000u);
+    }
+    // The terms: put(term, bytes).  Two-wide: the scaled entries and what their first term leaves are float16 numbers (eight bits below 2^8).
+    template <typename Put>
+    __device__ __forceinline__ void terms(uint32_t b, Put put) const {
+        const uint32_t up = (254 - min(b, 253u)) << 7, next = (15 + b - term_scale_byte(b, 1)) << 10;      // powers of two: bfloat16, float16
+        uint32_t t0[4], t1[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = (&raw.x)[i], half, back, rest;
+            uint16_t first, second;
+            asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(w), "r"(up | up << 16));
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(half) : "f"(__uint_as_float(w & 0xffff0000u)), "f"(__uint_as_float(w << 16)));
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(first) : "r"(half));
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(first));
+            asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(rest) : "r"(half), "r"(back));
+            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(rest) : "r"(rest), "r"(next | next << 16));
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(second) : "r"(rest));
+            t0[i] = first;
+            t1[i] = second;
+        }
+        const bool no = b == 255;
+        put(0, no ? make_uint2(0, 0) : make_uint2(t0[0] | t0[1] << 16, t0[2] | t0[3] << 16));
+        put(1, no ? make_uint2(0, 0) : make_uint2(t1[0] | t1[1] << 16, t1[2] | t1[3] << 16));
+    }
+};
+
+template <>
+struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* row, int c, int K, bool vector) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+            if (vector) {
+                const float4 q = c + h < K ? *reinterpret_cast<const float4*>(row + c + h) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[h] = q.x; v[h + 1] = q.y; v[h + 2] = q.z; v[h + 3] = q.w;
+            } else {
+#pragma unroll
+                for (int i = h; i < h + 4; ++i) v[i] = c + i < K ? row[c + i] : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        return m;
+    }
+    template <typename Put>
+    __device__ __forceinline__ void terms(uint32_t b, Put put) const {
+        const float up = __uint_as_float((254 - min(b, 253u)) << 23);
+        float rest[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rest[i] = b == 255 ? 0.f : v[i] * up;
+#pragma unroll
+        for (int term = 0; term < kTerms<float>; ++term) {
+            const float next = __uint_as_float((127 + term_scale_byte(b, term) - term_scale_byte(b, term + 1)) << 23);
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint16_t pair;
+                uint32_t back;
+                float lo, hi;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(rest[2 * i + 1]), "f"(rest[2 * i]));
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(pair));
+                asm("{\n.reg .f16 a, b;\nmov.b32 {a, b}, %2;\ncvt.f32.f16 %0, a;\ncvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(back));
+                rest[2 * i] = (rest[2 * i] - lo) * next;
+                rest[2 * i + 1] = (rest[2 * i + 1] - hi) * next;
+                w[i >> 1] |= (uint32_t)pair << (16 * (i & 1));
+            }
+            put(term, make_uint2(w[0], w[1]));
+        }
+    }
+};
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,

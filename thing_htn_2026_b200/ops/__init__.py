@@ -154,8 +154,9 @@ _SIGNATURES = {
     "thn_mx4_arrange": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p],
     "thn_mx4_linear": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     "thn_mx4_stream_rows": [c_int],
-    "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
-                       c_void_p],
+    "thn_mx4_stream_scratch_bytes": [c_int, c_int, c_int],
+    "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
+                       c_int, c_void_p, c_void_p],
     "thn_gemm_f32": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "thn_linear_skinny_bf16": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "thn_linear_skinny_supported": [c_int, c_int],
@@ -250,7 +251,8 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # (torch.cuda.current_stream() makes an object first: 3.2 us a call against 0.3)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _need(t: torch.Tensor, what: str, dtype=None) -> torch.Tensor:
@@ -994,17 +996,33 @@ def linear_batched(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
 # ------------------------------------------------------------------ microscaled 4-bit matrices
 
 
-@dataclass(frozen=True)
 class Mx4:
     """A matrix ``[rows, columns]`` in microscaled 4-bit floating point: every 32 neighbouring entries of a row share a
     scale, a power of two held in a byte (``2^(byte - 127)``; 255: the block is not a number), and an entry is one of 0, 1/2, 1, 3/2,
-    2, 3, 4, 6 with a sign, held in four bits.  ``codes`` and ``scales`` are laid out for the tensor cores
-    (``csrc/mx4.cuh``); :func:`quantize_mx4` makes one from numbers, :func:`mx4_from_parts` from stored codes and scales."""
+    2, 3, 4, 6 with a sign, held in four bits.  :func:`quantize_mx4` makes one from numbers, :func:`mx4_from_parts` from stored codes
+    and scales.  ``data`` holds the codes and behind them the scales, laid out for the tensor cores (``csrc/mx4.cuh``)."""
 
-    codes: torch.Tensor      # uint8 [rows, padded columns / 2]
-    scales: torch.Tensor     # uint8 [ceil(rows / 128), padded columns / 128, 512]
-    rows: int
-    columns: int
+    __slots__ = ("data", "rows", "columns", "code_bytes")
+
+    def __init__(self, data: torch.Tensor, rows: int, columns: int):
+        self.data, self.rows, self.columns = data, rows, columns
+        self.code_bytes = rows * (-(-columns // 128) * 64)
+
+    @classmethod
+    def empty(cls, like: torch.Tensor, rows: int, columns: int) -> "Mx4":
+        """Room for a matrix on the device of ``like``."""
+        atoms = -(-columns // 128)
+        return cls(like.new_empty((rows * 64 + (-(-rows // 128)) * 512) * atoms, dtype=torch.uint8), rows, columns)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """uint8 ``[rows, padded columns / 2]``."""
+        return self.data[:self.code_bytes].view(self.rows, -(-self.columns // 128) * 64)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """uint8 ``[ceil(rows / 128), padded columns / 128, 512]``."""
+        return self.data[self.code_bytes:].view(-(-self.rows // 128), -(-self.columns // 128), 512)
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -1012,22 +1030,20 @@ class Mx4:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.data.device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.data.numel()
+
+    def _pointers(self) -> Tuple[int, int]:
+        at = self.data.data_ptr()
+        return at, at + self.code_bytes
 
 
 def _on_current_device(t: torch.Tensor, what: str) -> None:
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():
         raise KernelError(f"{what}: tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _mx4_empty(rows: int, columns: int, device) -> Mx4:
-    padded = -(-columns // 128) * 128
-    return Mx4(torch.empty((rows, padded // 2), dtype=torch.uint8, device=device),
-               torch.empty((-(-rows // 128), padded // 128, 512), dtype=torch.uint8, device=device), rows, columns)
 
 
 def quantize_mx4(x: torch.Tensor) -> Mx4:
@@ -1039,8 +1055,10 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
         raise KernelError(f"quantize_mx4: a matrix with columns, please, not {tuple(x.shape)}")
     code = _code(x, "quantize_mx4 x")
     _on_current_device(x, "quantize_mx4 x")
-    out = _mx4_empty(x.shape[0], x.shape[1], x.device)
-    _call("thn_mx4_quantize", _ptr(out.codes), _ptr(out.scales), _ptr(x), x.shape[0], x.shape[1], code, _stream())
+    rows, columns = x.shape
+    out = Mx4.empty(x, rows, columns)
+    codes, scales = out._pointers()
+    _call("thn_mx4_quantize", codes, scales, x.data_ptr(), rows, columns, code, _stream())
     return out
 
 
@@ -1056,8 +1074,9 @@ def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> M
     if scales.device != codes.device:
         raise KernelError(f"mx4_from_parts: codes on {codes.device}, scales on {scales.device}")
     _on_current_device(codes, "mx4_from_parts codes")
-    out = _mx4_empty(rows, columns, codes.device)
-    _call("thn_mx4_arrange", _ptr(out.codes), _ptr(out.scales), _ptr(codes), _ptr(scales), rows, columns, _stream())
+    out = Mx4.empty(codes, rows, columns)
+    to_codes, to_scales = out._pointers()
+    _call("thn_mx4_arrange", to_codes, to_scales, codes.data_ptr(), scales.data_ptr(), rows, columns, _stream())
     return out
 
 
@@ -1065,9 +1084,10 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The numbers ``[rows, columns]`` that ``q`` stands for, in float32 or bfloat16; both hold them exactly."""
     if dtype not in DTYPE_CODE:
         raise KernelError(f"dequantize_mx4: dtype {dtype} is not supported (float32 or bfloat16)")
-    _on_current_device(q.codes, "dequantize_mx4 q")
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    _call("thn_mx4_dequantize", _ptr(out), _ptr(q.codes), _ptr(q.scales), q.rows, q.columns, DTYPE_CODE[dtype], _stream())
+    _on_current_device(q.data, "dequantize_mx4 q")
+    out = q.data.new_empty(q.shape, dtype=dtype)
+    codes, scales = q._pointers()
+    _call("thn_mx4_dequantize", out.data_ptr(), codes, scales, q.rows, q.columns, DTYPE_CODE[dtype], _stream())
     return out
 
 
@@ -1075,34 +1095,45 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [M, K] @ weight[N, K]^T`` (+ ``bias [N]``) with a weight in 4 bits: float32 sums, one rounding to ``out_dtype`` (bfloat16 or
     float32).  ``x`` is a tensor in bfloat16 or float32, which is multiplied as it is and whose type is the default
-    ``out_dtype``, or an :class:`Mx4` (default: bfloat16)."""
-    quantized = isinstance(x, Mx4)
-    if not quantized:
+    ``out_dtype``, or an :class:`Mx4` (default: bfloat16).  A row of ``x`` that holds an infinity or a NaN comes out as NaN, and so does the
+    column of a weight row that does.  ``err``: the step's device error word for the kernel's bounded waits."""
+    if isinstance(x, Mx4):
+        kind, data, (at, x_scales) = 2, x.data, x._pointers()
+        m, k = x.rows, x.columns
+    else:
         _need(x, "linear_mx4 x")
         if x.dim() != 2:
             raise KernelError(f"linear_mx4: x has {x.dim()} dimensions, not 2")
-    if x.shape[1] != weight.columns:
-        raise KernelError(f"linear_mx4: shapes x {tuple(x.shape)}, weight {weight.shape}")
-    if x.device != weight.device:
-        raise KernelError(f"linear_mx4: x on {x.device}, weight on {weight.device}")
-    data = x.codes if quantized else x
+        kind, data, at, x_scales = _code(x, "linear_mx4 x"), x, x.data_ptr(), None
+        m, k = x.shape
+    n = weight.rows
+    if k != weight.columns:
+        raise KernelError(f"linear_mx4: shapes x {(m, k)}, weight {weight.shape}")
+    if data.get_device() != weight.data.get_device():
+        raise KernelError(f"linear_mx4: x on {data.device}, weight on {weight.device}")
     _on_current_device(data, "linear_mx4 x")
-    kind = 2 if quantized else _code(x, "linear_mx4 x")
-    out_dtype = out_dtype or (torch.bfloat16 if quantized else x.dtype)
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if kind == 2 else x.dtype
     if out_dtype not in DTYPE_CODE:
         raise KernelError(f"linear_mx4: out_dtype {out_dtype} is not supported (float32 or bfloat16)")
+    bias_code = 0
     if bias is not None:
         _need(bias, "linear_mx4 bias")
-        if tuple(bias.shape) != (weight.rows,) or bias.device != data.device:
-            raise KernelError(f"linear_mx4: a bias {tuple(bias.shape)} on {bias.device} for {weight.rows} outputs on {data.device}")
-    bias_code = 0 if bias is None else _code(bias, "linear_mx4 bias")
-    out = torch.empty((x.shape[0], weight.rows), dtype=out_dtype, device=data.device)
-    if 0 < x.shape[0] <= lib().thn_mx4_stream_rows(kind) and weight.rows:
-        _call("thn_mx4_stream", _ptr(out), DTYPE_CODE[out_dtype], _ptr(data), _ptr(x.scales) if quantized else None, kind, _ptr(weight.codes),
-              _ptr(weight.scales), _ptr(bias), bias_code, x.shape[0], weight.rows, weight.columns, 0, _ptr(err), _stream())
+        if tuple(bias.shape) != (n,) or bias.get_device() != data.get_device():
+            raise KernelError(f"linear_mx4: a bias {tuple(bias.shape)} on {bias.device} for {n} outputs on {data.device}")
+        bias_code = _code(bias, "linear_mx4 bias")
+    out = data.new_empty((m, n), dtype=out_dtype)
+    if m == 0 or n == 0:
         return out
-    _call("thn_mx4_linear", _ptr(out), DTYPE_CODE[out_dtype], _ptr(data), _ptr(x.scales) if quantized else None, kind, _ptr(weight.codes),
-          _ptr(weight.scales), _ptr(bias), bias_code, x.shape[0], weight.rows, weight.columns, _ptr(err), _stream())
+    codes, scales = weight._pointers()
+    if m <= (32 if kind == 0 else 64):
+        size = 0 if kind == 2 or m <= 8 else lib().thn_mx4_stream_scratch_bytes(kind, m, k)
+        terms = data.new_empty(size, dtype=torch.uint8) if size else None
+        _call("thn_mx4_stream", out.data_ptr(), DTYPE_CODE[out_dtype], at, x_scales, kind, codes, scales, _ptr(bias), bias_code, _ptr(terms), size,
+              m, n, k, 0, _ptr(err), _stream())
+        return out
+    _call("thn_mx4_linear", out.data_ptr(), DTYPE_CODE[out_dtype], at, x_scales, kind, codes, scales, _ptr(bias), bias_code, m, n, k, _ptr(err),
+          _stream())
     return out
 
 
