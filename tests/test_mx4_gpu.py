@@ -286,17 +286,19 @@ def test_another_stream_and_a_recorded_graph():
             assert torch.equal(outs[i][0], want[i]) and torch.equal(outs[i][1], want[2 + i])
 
 
+@pytest.mark.parametrize("m,entry", [(5, "thn_mx4_stream"), (60, "thn_mx4_stream"), (200, "thn_mx4_pair")])
 @pytest.mark.parametrize("quantized", [False, True])
-def test_a_wait_that_runs_out_is_reported(quantized):
+def test_a_wait_that_runs_out_is_reported(m, entry, quantized):
     """Nothing is loaded: the waits for it end, the error word says so, the result is no number."""
     weight, _ = weight_of(300, 640, 1)
-    x = rows_of(5, 640, torch.bfloat16, 2)
+    x = rows_of(m, 640, torch.bfloat16, 2)
     q = ops.quantize_mx4(x)
-    out = torch.zeros((5, 300), dtype=torch.float32, device="cuda")
+    out = torch.zeros((m, 300), dtype=torch.float32, device="cuda")
     err = ops.new_error_word("cuda")
     data, scales, kind = (q.codes, q.scales, 2) if quantized else (x, None, 1)
-    ops._call("thn_mx4_stream", out.data_ptr(), 0, data.data_ptr(), ops._ptr(scales), kind, weight.codes.data_ptr(), weight.scales.data_ptr(), None, 0,
-              None, 0, 5, 300, 640, 1, err.data_ptr(), ops._stream())
+    room = torch.empty(getattr(ops.lib(), entry + "_scratch_bytes")(kind, m, 640) or 16, dtype=torch.uint8, device="cuda")
+    ops._call(entry, out.data_ptr(), 0, data.data_ptr(), ops._ptr(scales), kind, weight.codes.data_ptr(), weight.scales.data_ptr(), None, 0,
+              room.data_ptr(), room.numel(), m, 300, 640, 1, err.data_ptr(), ops._stream())
     with pytest.raises(ops.KernelError, match="gave up"):
         ops.raise_on_device_error(err, "test")
     assert torch.isnan(out).all()

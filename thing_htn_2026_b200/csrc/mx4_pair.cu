@@ -1,0 +1,418 @@
+// out[M, N] = x[M, K] @ W[N, K]^T (+ bias) for many rows, W in microscaled 4-bit floating point (mx4.cuh), on pairs of
+// multiprocessors (tcgen05 with cta_group::2, the scales applied by the tensor core).
+//
+//  * A pair's tile is 256 rows of W (the accumulator's lanes, 128 a block) by up to kCols rows of x (its columns, of which each block
+//    brings half), so that a multiprocessor brings half of what a block alone would for the same products.
+//  * Rows in 4 bits (kQuantized): both operands as they lie, 256 columns of the sum in 128 bytes a row, kind::mxf4, four times
+//    the rate of bfloat16.
+//  * Rows in bfloat16 or float32 (kRows2, kRows6): two or six terms of 8-bit floats (mx4_tcgen05.cuh) that mx4_terms_kernel has
+//    prepared, 128 columns of the sum at a time, kind::mxf8f6f4; W's codes are spread over 8-bit containers by TMA as they are
+//    copied.  Two terms at twice the rate of bfloat16 cost what a bfloat16 product costs; W is a quarter of the bytes.
+//  * Scales: 512 bytes for 128 rows and 128 columns, by TMA like the operands, to tensor memory by tcgen05.cp just ahead of the
+//    products that use them.  A tile's rows of x begin at a multiple of 64, two columns of scales.
+//
+// A row's result depends on its own entries and its place in a tile alone.  Every wait on an mbarrier is bounded: after
+// kWaitLimitNs the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, what is left to store becomes NaN, and tensor
+// memory is given back.  A pair's two blocks are one cluster and always resident together; no wait depends on another pair.
+#include "mx4_tcgen05.cuh"
+
+namespace {
+
+enum Mode { kQuantized, kRows2, kRows6 };
+
+constexpr int kFeatures = 256;                             // of a pair
+constexpr int kEpilogueWarps = 16, kThreads = 64 + 32 * kEpilogueWarps;      // warp 0: TMA, warp 1: products and tensor memory
+
+template <int MODE>
+struct Shape {
+    static constexpr int kT = MODE == kQuantized ? 1 : MODE == kRows2 ? 2 : 6;
+    static constexpr int kCols = 192, kBuffers = 2;                          // columns of an accumulator; accumulators
+    static constexpr int kSteps = MODE == kQuantized ? 2 : 1;                // pieces of 128 columns of the sum that a stage holds
+    static constexpr int kAtoms = (kCols + 64 + 127) / 128;                  // of scales that a tile's rows of x can touch
+    static constexpr uint32_t kASmem = 128 * 128, kBSmem = kCols / 2 * 128;  // of one block, a term
+    static constexpr uint32_t kScaleBytes = kSteps * (1 + kT * kAtoms) * kMx4AtomBytes;
+    static constexpr uint32_t kStageStride = kASmem + kT * kBSmem + (kScaleBytes + 1023) / 1024 * 1024;
+    static constexpr int kFit = (int)((226 * 1024 - 2048) / kStageStride);
+    static constexpr int kStages = kFit < 8 ? kFit : 8;
+    static constexpr size_t kSmemBytes = kStages * kStageStride + 1024 /* alignment */ + 512 /* barriers */;
+    static constexpr uint32_t kScaleCol = kCols * kBuffers;                  // W's scales, then x's
+    static_assert(kScaleCol + kSteps * 4 * (1 + kT * kAtoms) <= 512, "tensor memory");
+    static_assert(kStages >= 2, "shared memory");
+};
+
+struct Args {
+    void* out;
+    const void* bias;
+    int M, N, atoms;                // atoms: pieces of 128 columns of the sum
+    int cuts, size, n_tiles;        // the rows of x in equal tiles
+    int plane_atoms;                // rows of a term's plane / 128
+    int* err;
+    int skip_loads;                 // the test of the bounded waits: nothing is loaded
+};
+
+__device__ __forceinline__ uint32_t block_in_pair() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// the address, as a cluster sees it, of the leading block's copy of something in shared memory
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
+    return a;
+}
+__device__ __forceinline__ void pair_barrier() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// A tile to this block's shared memory, its bytes counted by the leading block's barrier.
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(smem_addr(dst)), "l"(map), "r"(leader_bar), "r"(x), "r"(y)
+        : "memory");
+}
+// 512 bytes of scales in each block's shared memory to four columns of its tensor memory.
+__device__ __forceinline__ void pair_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int MODE>
+__device__ __forceinline__ void pair_mma(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t instr, uint32_t a_scales, uint32_t b_scales,
+                                         uint32_t accumulate) {
+    if constexpr (MODE == kQuantized)
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "}\n"
+            ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instr), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "}\n"
+            ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(instr), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+            : "memory");
+}
+// The barrier at this place in both blocks hears of the products issued so far.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_addr(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Rows [row0, row0 + here) of x by features from `feature` on; columns: the rows rounded up to 64.
+struct Tile {
+    int row0, here, columns, feature;
+};
+
+template <int MODE, typename OutT, typename BiasT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pair_kernel(
+    const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w_scales, const __grid_constant__ CUtensorMap map_x,
+    const __grid_constant__ CUtensorMap map_x_scales, const Args a) {
+    using S = Shape<MODE>;
+    pdl_launch_dependents();
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + (size_t)S::kStages * S::kStageStride);
+    uint64_t* empty = full + S::kStages;
+    uint64_t* acc_full = empty + S::kStages;               // accumulator ready to be stored
+    uint64_t* acc_empty = acc_full + S::kBuffers;          // accumulator read by both blocks (the leader's counts)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kBuffers);
+    volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)block_in_pair(), pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+    const int n_k = (a.atoms + S::kSteps - 1) / S::kSteps;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, 1);
+        }
+        for (int i = 0; i < S::kBuffers; ++i) {
+            mbar_init(acc_full + i, 1);
+            mbar_init(acc_empty + i, 2 * kEpilogueWarps);
+        }
+        *give_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {   // the same warp of both blocks allocates
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    pair_barrier();                            // both blocks' barriers stand
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    pdl_wait();
+
+    // Neighbouring tiles share their rows of W: the tiles of rows run fastest.
+    auto tile_of = [&](int i) {
+        Tile t;
+        const int f = i / a.cuts, cut = i - f * a.cuts;
+        t.row0 = cut * a.size;
+        t.here = min(a.size, a.M - t.row0);
+        t.columns = (t.here + 63) / 64 * 64;
+        t.feature = f * kFeatures;
+        return t;
+    };
+
+    if (warp == 0 && lane == 0) {
+        // ---- TMA producer
+        int it = 0;
+        for (int i = pair; i < a.n_tiles && !*give_up; i += n_pairs) {
+            const Tile t = tile_of(i);
+            const int half = t.columns / 2, b_row = t.row0 + rank * half, a_row = t.feature + rank * 128;
+            const int x_atom = t.row0 >> 7, x_atoms = ((t.row0 & 127) + t.columns + 127) >> 7;
+            const uint32_t bytes = (MODE == kQuantized ? S::kASmem : S::kASmem / 2) + S::kT * (half * 128 + S::kSteps * x_atoms * kMx4AtomBytes) +
+                                   S::kSteps * kMx4AtomBytes;
+            for (int kb = 0; kb < n_k && !a.skip_loads; ++kb, ++it) {
+                const int s = it % S::kStages;
+                if (!mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1)) {
+                    if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                    *give_up = 1;
+                    break;
+                }
+                unsigned char* dst = tiles + (size_t)s * S::kStageStride;
+                unsigned char* scales = dst + S::kASmem + S::kT * S::kBSmem;
+                const uint32_t bar = leader_addr(full + s);
+                if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
+                load_tile(dst, &map_w, bar, kb * 128, a_row);          // (bytes of codes, or entries)
+                load_tile(scales, &map_w_scales, bar, 0, (a_row >> 7) * a.atoms + kb * S::kSteps);
+#pragma unroll
+                for (int term = 0; term < S::kT; ++term) {
+                    unsigned char* b = dst + S::kASmem + term * S::kBSmem;
+                    for (int r = 0; r < half; r += 32) load_tile(b + r * 128, &map_x, bar, kb * 128, term * a.plane_atoms * 128 + b_row + r);
+                    for (int j = 0; j < x_atoms; ++j)
+                        load_tile(scales + S::kSteps * (1 + term * S::kAtoms + j) * kMx4AtomBytes, &map_x_scales, bar, 0,
+                                  (term * a.plane_atoms + x_atom + j) * a.atoms + kb * S::kSteps);
+                }
+            }
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        // ---- the leading block issues the pair's products
+        const uint32_t w_col = tmem_base + S::kScaleCol, x_col = w_col + 4 * S::kSteps;
+        int it = 0, local = 0;
+        for (int i = pair; i < a.n_tiles && !*give_up; i += n_pairs, ++local) {
+            const Tile t = tile_of(i);
+            const uint32_t instr = MODE == kQuantized ? scaled_instr(1, 1, kFeatures, t.columns) : scaled_instr(kE2M1, kE4M3, kFeatures, t.columns);
+            const int x_atoms = ((t.row0 & 127) + t.columns + 127) >> 7;
+            const uint32_t first = (t.row0 & 127) >> 5;          // the tile's first column of scales
+            const int buf = local % S::kBuffers;
+            bool ok = mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t tmem_d = tmem_base + buf * S::kCols;
+            for (int kb = 0; kb < n_k && ok; ++kb, ++it) {
+                const int s = it % S::kStages;
+                ok = mbar_wait(full + s, (it / S::kStages) & 1);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride), scales = at + S::kASmem + S::kT * S::kBSmem;
+#pragma unroll
+                for (int p = 0; p < S::kSteps; ++p) pair_scales(w_col + 4 * p, scale_desc(scales + p * kMx4AtomBytes));
+                const uint64_t a_desc = smem_desc(at);
+#pragma unroll
+                for (int term = 0; term < S::kT; ++term) {
+                    const uint32_t from = scales + S::kSteps * (1 + term * S::kAtoms) * kMx4AtomBytes, to = x_col + term * S::kSteps * S::kAtoms * 4;
+                    for (int j = 0; j < x_atoms; ++j)
+#pragma unroll
+                        for (int p = 0; p < S::kSteps; ++p)
+                            pair_scales(to + (p * S::kAtoms + j) * 4, scale_desc(from + (j * S::kSteps + p) * kMx4AtomBytes));
+                    const uint64_t b_desc = smem_desc(at + S::kASmem + term * S::kBSmem);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {          // 32 bytes further along K: + 2 in the address field
+                        if constexpr (MODE == kQuantized) {        // 64 entries, two of a piece's four scales
+                            if (k >= 2 && kb * 2 + 1 >= a.atoms) break;
+                            pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, (k & 1) * 2), w_col + 4 * (k >> 1),
+                                           to + (k >> 1) * S::kAtoms * 4 + first, (kb | k) != 0);
+                        } else {                                   // 32 entries, one scale
+                            pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, k), w_col, to + first,
+                                           (kb | k | term) != 0);
+                        }
+                    }
+                }
+                pair_commit(empty + s);                    // the stage is free in both blocks when these products are done
+            }
+            if (ok) {
+                pair_commit(acc_full + buf);
+            } else {                                       // (the warps that wait for this accumulator, in both blocks, give up by themselves)
+                if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                *give_up = 1;
+            }
+        }
+    } else if (warp >= 2) {
+        // ---- epilogue: a warp reads tensor-memory lanes 32 * (warp % 4) .. + 31 (= features), every fourth chunk of 32 columns (= rows)
+        const int quarter = warp & 3, group = (warp - 2) >> 2;
+        int local = 0;
+        bool dead = false;
+        for (int i = pair; i < a.n_tiles; i += n_pairs, ++local) {
+            const Tile t = tile_of(i);
+            const int buf = local % S::kBuffers;
+            const int feature = t.feature + rank * 128 + quarter * 32 + lane;
+            const bool there = feature < a.N;
+            const float bias = a.bias && there ? to_f32<BiasT>(static_cast<const BiasT*>(a.bias)[feature]) : 0.f;
+            if (!dead) {
+                const bool came = mbar_wait(acc_full + buf, (local / S::kBuffers) & 1);
+                dead = !__all_sync(0xffffffffu, came && !*give_up);      // all lanes together before tcgen05.ld
+                if (dead) {
+                    if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                    *give_up = 1;
+                }
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t taddr = tmem_base + buf * S::kCols + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+            for (int c = 32 * group; c < t.here; c += 32 * (kEpilogueWarps / 4)) {
+                float v[32];
+                if (dead) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7fffffffu);
+                } else {
+                    tmem_load_32(taddr + c, v);
+                }
+                if (there) {
+                    OutT* out = static_cast<OutT*>(a.out) + (long long)(t.row0 + c) * a.N + feature;
+                    if (c + 32 <= t.here) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j, out += a.N) *out = from_f32<OutT>(v[j] + bias);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j, out += a.N)
+                            if (c + j < t.here) *out = from_f32<OutT>(v[j] + bias);
+                    }
+                }
+                __syncwarp();
+            }
+            // this warp has read its share of the accumulator: the leader may fill it again
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(acc_empty + buf)) : "memory");
+        }
+    }
+    if (*give_up) let_copies_land();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    pair_barrier();                            // neither block leaves while the other may reach into it
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    }
+}
+
+// Scales as rows of 512 bytes, `pieces` of them a box.
+bool map_scales(CUtensorMap* map, const void* scales, long long rows, int pieces) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[2] = {kMx4AtomBytes / 4, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {kMx4AtomBytes};
+    const cuuint32_t box[2] = {kMx4AtomBytes / 4, (cuuint32_t)pieces};
+    const cuuint32_t elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int MODE, typename OutT, typename BiasT>
+int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) {
+    auto kernel = mx4_pair_kernel<MODE, OutT, BiasT>;
+    static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE>::kSmemBytes);
+    if (configured != cudaSuccess) {
+        thn_set_error("mx4_pair: cannot reserve %zu bytes of shared memory: %s", Shape<MODE>::kSmemBytes, cudaGetErrorString(configured));
+        return (int)configured;
+    }
+    int device = 0, n_sms = 0;
+    cudaGetDevice(&device);
+    cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
+    const int pairs = args.n_tiles < n_sms / 2 ? args.n_tiles : n_sms / 2;
+    thn_launch(kernel, dim3((unsigned)(2 * pairs)), kThreads, Shape<MODE>::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], args);
+    return thn_launch_status("mx4_pair");
+}
+
+template <int MODE>
+int run(Args args, const void* codes, const void* scales, const void* x, const void* x_scales, int out_dtype, int bias_dtype, cudaStream_t stream) {
+    using S = Shape<MODE>;
+    const long long padded = (long long)args.atoms * kMx4Atom;
+    args.cuts = (args.M + S::kCols - 1) / S::kCols;
+    args.size = ((args.M + args.cuts - 1) / args.cuts + 63) / 64 * 64;
+    args.cuts = (args.M + args.size - 1) / args.size;
+    const long long n_tiles = (long long)args.cuts * ((args.N + kFeatures - 1) / kFeatures);
+    THN_UNSUPPORTED_IF(n_tiles > 0x3fffffff, "mx4_pair: M=%d N=%d are too many tiles", args.M, args.N);
+    args.n_tiles = (int)n_tiles;
+    args.plane_atoms = (args.M + 127) / 128;
+    CUtensorMap maps[4];
+    bool made = map_scales(&maps[1], scales, (long long)((args.N + 127) / 128) * args.atoms, S::kSteps) &&
+                map_scales(&maps[3], x_scales, (long long)S::kT * args.plane_atoms * args.atoms, S::kSteps);
+    if (MODE == kQuantized)
+        made = made && map_bytes(&maps[0], codes, args.N, padded / 2, 128) && map_bytes(&maps[2], x, args.M, padded / 2, 32);
+    else
+        made = made && map_unpacked(&maps[0], codes, args.N, padded, 128) && map_bytes(&maps[2], x, (long long)S::kT * args.plane_atoms * 128, padded, 32);
+    if (!made) {
+        thn_set_error("mx4_pair: cuTensorMapEncodeTiled failed for M=%d N=%d and %d pieces of K", args.M, args.N, args.atoms);
+        return THN_BAD_ARGUMENT;
+    }
+    if (out_dtype == THN_F32)
+        return bias_dtype == THN_F32 ? launch<MODE, float, float>(maps, args, stream) : launch<MODE, float, __nv_bfloat16>(maps, args, stream);
+    return bias_dtype == THN_F32 ? launch<MODE, __nv_bfloat16, float>(maps, args, stream)
+                                 : launch<MODE, __nv_bfloat16, __nv_bfloat16>(maps, args, stream);
+}
+
+}  // namespace
+
+// The bytes of `terms` that M rows of a type need.
+THN_API long long thn_mx4_pair_scratch_bytes(int x_type, int M, int K) {
+    if (x_type == 2) return 0;
+    const long long atoms = (long long)((M + 127) / 128) * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
+    return atoms * 128 * padded + atoms * (padded / kMx4Atom) * kMx4AtomBytes;
+}
+
+// out [M, N] of out_dtype = x [M, K] @ w [N, K]^T (+ bias [N] of bias_dtype, or null).
+//   x          [M, K] of x_type; 2: codes [M, padded / 2] with x_scales (mx4.cuh)
+//   codes, scales: W;  terms: scratch of thn_mx4_pair_scratch_bytes
+// Scales and terms 16-byte, 4-bit codes 32-byte aligned.  err: device error word (THN_ERR_WAIT_TIMEOUT if a wait gave up).
+// skip_loads: 0; otherwise no operand is loaded, so that the waits run out (for the test of the waits only).
+THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_scales, int x_type, const void* codes, const void* scales,
+                         const void* bias, int bias_dtype, void* terms, long long terms_bytes, int M, int N, int K, int skip_loads, int* err,
+                         cudaStream_t stream) {
+    THN_CHECK_ARG(x_type >= 0 && x_type <= 2 && (out_dtype == THN_F32 || out_dtype == THN_BF16) && (bias_dtype == THN_F32 || bias_dtype == THN_BF16),
+                  "mx4_pair: unknown type %d, %d or %d", x_type, out_dtype, bias_dtype);
+    THN_UNSUPPORTED_IF(M < 1 || M > (1 << 24) || N < 1 || N > (1 << 24) || K < 1 || K > (1 << 24), "mx4_pair: M=%d N=%d K=%d not supported", M, N, K);
+    THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 &&
+                  (((uintptr_t)scales | (uintptr_t)x_scales | (uintptr_t)terms) & 15) == 0, "mx4_pair: codes must be 32-byte, scales and terms 16-byte aligned");
+    THN_CHECK_ARG(terms_bytes >= thn_mx4_pair_scratch_bytes(x_type, M, K), "mx4_pair: %lld bytes of scratch, %lld needed", terms_bytes,
+                  thn_mx4_pair_scratch_bytes(x_type, M, K));
+    Args args = {};
+    args.out = out;
+    args.bias = bias;
+    args.M = M;
+    args.N = N;
+    args.atoms = (int)(mx4_padded(K) / kMx4Atom);
+    args.err = err;
+    args.skip_loads = skip_loads;
+    THN_UNSUPPORTED_IF((long long)(N + 127) / 128 * args.atoms > 0x7fffffff || (long long)(M + 127) / 128 * 6 * args.atoms > 0x7fffffff,
+                       "mx4_pair: M=%d N=%d K=%d: too many scales", M, N, K);
+    if (x_type == 2) return run<kQuantized>(args, codes, scales, x, x_scales, out_dtype, bias_dtype, stream);
+    const int plane = (M + 127) / 128 * 128;
+    uint8_t* bytes = static_cast<uint8_t*>(terms);
+    uint8_t* term_scales = bytes + (long long)plane * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>) * mx4_padded(K);
+    const int status = mx4_terms(bytes, term_scales, x, x_type, M, K, plane, stream);
+    if (status != THN_OK) return status;
+    if (x_type == THN_F32) return run<kRows6>(args, codes, scales, bytes, term_scales, out_dtype, bias_dtype, stream);
+    return run<kRows2>(args, codes, scales, bytes, term_scales, out_dtype, bias_dtype, stream);
+}

@@ -367,8 +367,8 @@ int launch_rows(Args args, const void* codes, long long padded, void* terms, int
     else if constexpr (!S::kConverts) {
         uint8_t* bytes = static_cast<uint8_t*>(terms);
         uint8_t* scales = bytes + (long long)S::kT * MR * padded;
-        thn_launch(mx4_terms_kernel<RT>, (unsigned)(((long long)args.M * (padded / 8) + 255) / 256), 256, 0, stream, bytes, scales, (const RT*)args.x,
-                   args.M, args.K, (int)padded, MR, (bool)args.vector);
+        const int status = mx4_terms(bytes, scales, args.x, sizeof(RT) == 4 ? THN_F32 : THN_BF16, args.M, args.K, MR, stream);
+        if (status != THN_OK) return status;
         args.x_scales = scales;
         made = made && map_bytes(&map_x, bytes, S::kT * MR, padded, S::NX);
     } else map_x = map_w;
@@ -387,6 +387,18 @@ int launch_rows(Args args, const void* codes, long long padded, void* terms, int
 int room_for(int M) { return M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64; }
 
 }  // namespace
+
+int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K, int plane, cudaStream_t stream) {
+    const long long padded = mx4_padded(K), blocks = ((long long)M * (padded / 8) + 255) / 256;
+    THN_UNSUPPORTED_IF(blocks > 0x7fffffff, "mx4_terms: %d rows of %d entries are too many", M, K);
+    const bool vector = ((uintptr_t)x & 15) == 0 && K % 8 == 0;
+    if (x_type == THN_F32)
+        thn_launch(mx4_terms_kernel<float>, (unsigned)blocks, 256, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const float*)x, M, K, (int)padded, plane, vector);
+    else
+        thn_launch(mx4_terms_kernel<__nv_bfloat16>, (unsigned)blocks, 256, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const __nv_bfloat16*)x, M, K,
+                   (int)padded, plane, vector);
+    return thn_launch_status("mx4_terms");
+}
 
 // How many rows of a type (THN_F32, THN_BF16, 2: 4 bits) thn_mx4_stream takes.
 THN_API int thn_mx4_stream_rows(int x_type) { return x_type == THN_F32 ? 32 : 64; }

@@ -152,7 +152,9 @@ _SIGNATURES = {
     "thn_mx4_quantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_arrange": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p],
-    "thn_mx4_linear": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+    "thn_mx4_pair_scratch_bytes": [c_int, c_int, c_int],
+    "thn_mx4_pair": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
+                     c_int, c_void_p, c_void_p],
     "thn_mx4_stream_rows": [c_int],
     "thn_mx4_stream_scratch_bytes": [c_int, c_int, c_int],
     "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
@@ -1126,14 +1128,14 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     if m == 0 or n == 0:
         return out
     codes, scales = weight._pointers()
-    if m <= (32 if kind == 0 else 64):
+    few = m <= (32 if kind == 0 else 64)
+    if few:
         size = 0 if kind == 2 or m <= 8 else lib().thn_mx4_stream_scratch_bytes(kind, m, k)
-        terms = data.new_empty(size, dtype=torch.uint8) if size else None
-        _call("thn_mx4_stream", out.data_ptr(), DTYPE_CODE[out_dtype], at, x_scales, kind, codes, scales, _ptr(bias), bias_code, _ptr(terms), size,
-              m, n, k, 0, _ptr(err), _stream())
-        return out
-    _call("thn_mx4_linear", out.data_ptr(), DTYPE_CODE[out_dtype], at, x_scales, kind, codes, scales, _ptr(bias), bias_code, m, n, k, _ptr(err),
-          _stream())
+    else:
+        size = 0 if kind == 2 else lib().thn_mx4_pair_scratch_bytes(kind, m, k)
+    terms = data.new_empty(size, dtype=torch.uint8) if size else None
+    _call("thn_mx4_stream" if few else "thn_mx4_pair", out.data_ptr(), DTYPE_CODE[out_dtype], at, x_scales, kind, codes, scales, _ptr(bias), bias_code,
+          _ptr(terms), size, m, n, k, 0, _ptr(err), _stream())
     return out
 
 
