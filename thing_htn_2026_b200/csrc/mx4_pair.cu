@@ -30,13 +30,14 @@ struct Shape {
     static constexpr int kSteps = MODE == kQuantized ? 2 : 1;                // pieces of 128 columns of the sum that a stage holds
     static constexpr int kAtoms = (kCols + 64 + 127) / 128;                  // of scales that a tile's rows of x can touch
     static constexpr uint32_t kASmem = 128 * 128, kBSmem = kCols / 2 * 128;  // of one block, a term
-    static constexpr uint32_t kScaleBytes = kSteps * (1 + kT * kAtoms) * kMx4AtomBytes;
+    static constexpr uint32_t kScaleBytes = kSteps * (1 + kT * kAtoms) * kMx4AtomBytes;      // W's, then x's: [term][128 rows][piece]
     static constexpr uint32_t kStageStride = kASmem + kT * kBSmem + (kScaleBytes + 1023) / 1024 * 1024;
     static constexpr int kFit = (int)((226 * 1024 - 2048) / kStageStride);
     static constexpr int kStages = kFit < 8 ? kFit : 8;
     static constexpr size_t kSmemBytes = kStages * kStageStride + 1024 /* alignment */ + 512 /* barriers */;
     static constexpr uint32_t kScaleCol = kCols * kBuffers;                  // W's scales, then x's
-    static_assert(kScaleCol + kSteps * 4 * (1 + kT * kAtoms) <= 512, "tensor memory");
+    static constexpr uint32_t kScaleCols = kSteps * 4 * (1 + kT * kAtoms);   // of a stage; two stages' in turn
+    static_assert(kScaleCol + 2 * kScaleCols <= 512, "tensor memory");
     static_assert(kStages >= 2, "shared memory");
 };
 
@@ -64,11 +65,23 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
 __device__ __forceinline__ void pair_barrier() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
-// A tile to this block's shared memory, its bytes counted by the leading block's barrier.
-__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
+// A box to this block's shared memory, its bytes counted by the leading block's barrier.
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(smem_addr(dst)), "l"(map), "r"(leader_bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_addr(dst)), "l"(map), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_addr(dst)), "l"(map), "r"(leader_bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 // 512 bytes of scales in each block's shared memory to four columns of its tensor memory.
@@ -179,10 +192,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
         int it = 0;
         for (int i = pair; i < a.n_tiles && !*give_up; i += n_pairs) {
             const Tile t = tile_of(i);
-            const int half = t.columns / 2, b_row = t.row0 + rank * half, a_row = t.feature + rank * 128;
-            const int x_atom = t.row0 >> 7, x_atoms = ((t.row0 & 127) + t.columns + 127) >> 7;
-            const uint32_t bytes = (MODE == kQuantized ? S::kASmem : S::kASmem / 2) + S::kT * (half * 128 + S::kSteps * x_atoms * kMx4AtomBytes) +
-                                   S::kSteps * kMx4AtomBytes;
+            const int b_row = t.row0 + rank * (t.columns / 2), a_row = t.feature + rank * 128;
+            // (a last tile of fewer columns brings what a whole one does)
+            constexpr uint32_t kBytes = (MODE == kQuantized ? S::kASmem : S::kASmem / 2) + S::kT * S::kBSmem + S::kScaleBytes;
             for (int kb = 0; kb < n_k && !a.skip_loads; ++kb, ++it) {
                 const int s = it % S::kStages;
                 if (!mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1)) {
@@ -193,57 +205,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                 unsigned char* dst = tiles + (size_t)s * S::kStageStride;
                 unsigned char* scales = dst + S::kASmem + S::kT * S::kBSmem;
                 const uint32_t bar = leader_addr(full + s);
-                if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
-                load_tile(dst, &map_w, bar, kb * 128, a_row);          // (bytes of codes, or entries)
-                load_tile(scales, &map_w_scales, bar, 0, (a_row >> 7) * a.atoms + kb * S::kSteps);
-#pragma unroll
-                for (int term = 0; term < S::kT; ++term) {
-                    unsigned char* b = dst + S::kASmem + term * S::kBSmem;
-                    for (int r = 0; r < half; r += 32) load_tile(b + r * 128, &map_x, bar, kb * 128, term * a.plane_atoms * 128 + b_row + r);
-                    for (int j = 0; j < x_atoms; ++j)
-                        load_tile(scales + S::kSteps * (1 + term * S::kAtoms + j) * kMx4AtomBytes, &map_x_scales, bar, 0,
-                                  (term * a.plane_atoms + x_atom + j) * a.atoms + kb * S::kSteps);
-                }
+                if (rank == 0) mbar_expect_tx(full + s, 2 * kBytes);
+                load_box(dst, &map_w, bar, kb * 128, a_row);           // (bytes of codes, or entries)
+                load_box(dst + S::kASmem, &map_x, bar, kb * 128, b_row, 0);
+                load_box(scales, &map_w_scales, bar, 0, kb * S::kSteps, a_row >> 7, 0);
+                load_box(scales + S::kSteps * kMx4AtomBytes, &map_x_scales, bar, 0, kb * S::kSteps, t.row0 >> 7, 0);
             }
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
         // ---- the leading block issues the pair's products
-        const uint32_t w_col = tmem_base + S::kScaleCol, x_col = w_col + 4 * S::kSteps;
         int it = 0, local = 0;
         for (int i = pair; i < a.n_tiles && !*give_up; i += n_pairs, ++local) {
             const Tile t = tile_of(i);
             const uint32_t instr = MODE == kQuantized ? scaled_instr(1, 1, kFeatures, t.columns) : scaled_instr(kE2M1, kE4M3, kFeatures, t.columns);
-            const int x_atoms = ((t.row0 & 127) + t.columns + 127) >> 7;
             const uint32_t first = (t.row0 & 127) >> 5;          // the tile's first column of scales
             const int buf = local % S::kBuffers;
+            // scales of a stage to its half of their columns: W's, then x's, [term][piece of K][128 rows]
+            auto bring_scales = [&](int it) {
+                const uint32_t from = smem_addr(tiles + (size_t)(it % S::kStages) * S::kStageStride) + S::kASmem + S::kT * S::kBSmem;
+                const uint32_t to = tmem_base + S::kScaleCol + (it & 1) * S::kScaleCols;
+#pragma unroll
+                for (int p = 0; p < S::kSteps; ++p) pair_scales(to + 4 * p, scale_desc(from + p * kMx4AtomBytes));
+#pragma unroll
+                for (int term = 0; term < S::kT; ++term)
+#pragma unroll
+                    for (int j = 0; j < S::kAtoms; ++j)
+#pragma unroll
+                        for (int p = 0; p < S::kSteps; ++p)
+                            pair_scales(to + 4 * (S::kSteps + (term * S::kSteps + p) * S::kAtoms + j),
+                                        scale_desc(from + (S::kSteps + (term * S::kAtoms + j) * S::kSteps + p) * kMx4AtomBytes));
+            };
             bool ok = mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + buf * S::kCols;
+            bool ahead = false;                                  // this stage has come, and its scales are on their way
             for (int kb = 0; kb < n_k && ok; ++kb, ++it) {
                 const int s = it % S::kStages;
-                ok = mbar_wait(full + s, (it / S::kStages) & 1);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride), scales = at + S::kASmem + S::kT * S::kBSmem;
-#pragma unroll
-                for (int p = 0; p < S::kSteps; ++p) pair_scales(w_col + 4 * p, scale_desc(scales + p * kMx4AtomBytes));
+                if (!ahead) {
+                    ok = mbar_wait(full + s, (it / S::kStages) & 1);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    bring_scales(it);
+                }
+                // the next stage's scales go first, if they are here: they are copied under this stage's products
+                ahead = kb + 1 < n_k && mbar_here(full + (it + 1) % S::kStages, ((it + 1) / S::kStages) & 1);
+                if (ahead) {
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    bring_scales(it + 1);
+                }
+                const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride);
+                const uint32_t w_col = tmem_base + S::kScaleCol + (it & 1) * S::kScaleCols, x_col = w_col + 4 * S::kSteps + first;
                 const uint64_t a_desc = smem_desc(at);
 #pragma unroll
                 for (int term = 0; term < S::kT; ++term) {
-                    const uint32_t from = scales + S::kSteps * (1 + term * S::kAtoms) * kMx4AtomBytes, to = x_col + term * S::kSteps * S::kAtoms * 4;
-                    for (int j = 0; j < x_atoms; ++j)
-#pragma unroll
-                        for (int p = 0; p < S::kSteps; ++p)
-                            pair_scales(to + (p * S::kAtoms + j) * 4, scale_desc(from + (j * S::kSteps + p) * kMx4AtomBytes));
                     const uint64_t b_desc = smem_desc(at + S::kASmem + term * S::kBSmem);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {          // 32 bytes further along K: + 2 in the address field
                         if constexpr (MODE == kQuantized) {        // 64 entries, two of a piece's four scales
                             if (k >= 2 && kb * 2 + 1 >= a.atoms) break;
                             pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, (k & 1) * 2), w_col + 4 * (k >> 1),
-                                           to + (k >> 1) * S::kAtoms * 4 + first, (kb | k) != 0);
+                                           x_col + (k >> 1) * S::kAtoms * 4, (kb | k) != 0);
                         } else {                                   // 32 entries, one scale
-                            pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, k), w_col, to + first,
+                            pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, k), w_col, x_col + term * S::kAtoms * 4,
                                            (kb | k | term) != 0);
                         }
                     }
@@ -317,16 +340,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     }
 }
 
-// Scales as rows of 512 bytes, `pieces` of them a box.
-bool map_scales(CUtensorMap* map, const void* scales, long long rows, int pieces) {
+// A tensor map of up to four dimensions, the strides in bytes from the second on.
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, int n, const void* base, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3],
+              const cuuint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
     const EncodeTiled encode = encode_tiled();
     if (encode == nullptr) return false;
-    const cuuint64_t dims[2] = {kMx4AtomBytes / 4, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {kMx4AtomBytes};
-    const cuuint32_t box[2] = {kMx4AtomBytes / 4, (cuuint32_t)pieces};
-    const cuuint32_t elem[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    return encode(map, type, n, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Scales [planes][rows / 128][pieces of K][512 bytes] for boxes of `steps` pieces for 128 `box_atoms` rows of each plane.
+bool map_scales(CUtensorMap* map, const void* scales, long long atoms, long long row_atoms, int planes, int steps, int box_atoms) {
+    const cuuint64_t row = (cuuint64_t)atoms * kMx4AtomBytes;
+    return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, scales, {kMx4AtomBytes / 4, (cuuint64_t)atoms, (cuuint64_t)row_atoms, (cuuint64_t)planes},
+                    {kMx4AtomBytes, row, row * (cuuint64_t)row_atoms}, {kMx4AtomBytes / 4, (cuuint32_t)steps, (cuuint32_t)box_atoms, (cuuint32_t)planes},
+                    CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+// Bytes [planes][rows][width] for boxes of 128 bytes of box_rows rows of each plane, 128-byte swizzle.
+bool map_planes(CUtensorMap* map, const void* base, long long width, long long rows, int planes, int box_rows) {
+    return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, {(cuuint64_t)width, (cuuint64_t)rows, (cuuint64_t)planes, 1},
+                    {(cuuint64_t)width, (cuuint64_t)(width * rows), 0}, {128, (cuuint32_t)box_rows, (cuuint32_t)planes, 1}, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int MODE, typename OutT, typename BiasT>
@@ -357,12 +390,13 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
     args.n_tiles = (int)n_tiles;
     args.plane_atoms = (args.M + 127) / 128;
     CUtensorMap maps[4];
-    bool made = map_scales(&maps[1], scales, (long long)((args.N + 127) / 128) * args.atoms, S::kSteps) &&
-                map_scales(&maps[3], x_scales, (long long)S::kT * args.plane_atoms * args.atoms, S::kSteps);
+    bool made = map_scales(&maps[1], scales, args.atoms, (args.N + 127) / 128, 1, S::kSteps, 1) &&
+                map_scales(&maps[3], x_scales, args.atoms, args.plane_atoms, S::kT, S::kSteps, S::kAtoms);
     if (MODE == kQuantized)
-        made = made && map_bytes(&maps[0], codes, args.N, padded / 2, 128) && map_bytes(&maps[2], x, args.M, padded / 2, 32);
+        made = made && map_bytes(&maps[0], codes, args.N, padded / 2, 128) && map_planes(&maps[2], x, padded / 2, args.M, 1, S::kCols / 2);
     else
-        made = made && map_unpacked(&maps[0], codes, args.N, padded, 128) && map_bytes(&maps[2], x, (long long)S::kT * args.plane_atoms * 128, padded, 32);
+        made = made && map_unpacked(&maps[0], codes, args.N, padded, 128) &&
+               map_planes(&maps[2], x, padded, (long long)args.plane_atoms * 128, S::kT, S::kCols / 2);
     if (!made) {
         thn_set_error("mx4_pair: cuTensorMapEncodeTiled failed for M=%d N=%d and %d pieces of K", args.M, args.N, args.atoms);
         return THN_BAD_ARGUMENT;
