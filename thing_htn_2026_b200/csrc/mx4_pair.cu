@@ -149,7 +149,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kBuffers);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)block_in_pair(), pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     const int n_k = (a.atoms + S::kSteps - 1) / S::kSteps;
 
@@ -173,7 +173,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     __syncthreads();
     pair_barrier();                            // both blocks' barriers stand
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_base = *tmem_slot;
+    constexpr uint32_t tmem_base = 0;          // all columns are this pair's
     pdl_wait();
 
     // Neighbouring tiles share their rows of W: the tiles of rows run fastest.
@@ -212,10 +212,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                 load_box(scales + S::kSteps * kMx4AtomBytes, &map_x_scales, bar, 0, kb * S::kSteps, t.row0 >> 7, 0);
             }
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // ---- the leading block issues the pair's products
+    } else if (warp == 1 && rank == 0) {
+        // ---- the leading block issues the pair's products: a whole warp walks, one thread of it issues
+        const bool issues = elect_one();
         int it = 0, local = 0;
-        for (int i = pair; i < a.n_tiles && !*give_up; i += n_pairs, ++local) {
+        for (int i = pair; i < a.n_tiles && !__any_sync(0xffffffffu, *give_up); i += n_pairs, ++local) {
             const Tile t = tile_of(i);
             const uint32_t instr = MODE == kQuantized ? scaled_instr(1, 1, kFeatures, t.columns) : scaled_instr(kE2M1, kE4M3, kFeatures, t.columns);
             const uint32_t first = (t.row0 & 127) >> 5;          // the tile's first column of scales
@@ -235,27 +236,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                             pair_scales(to + 4 * (S::kSteps + (term * S::kSteps + p) * S::kAtoms + j),
                                         scale_desc(from + (S::kSteps + (term * S::kAtoms + j) * S::kSteps + p) * kMx4AtomBytes));
             };
-            bool ok = mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1);
+            bool ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + buf * S::kCols;
             bool ahead = false;                                  // this stage has come, and its scales are on their way
             for (int kb = 0; kb < n_k && ok; ++kb, ++it) {
                 const int s = it % S::kStages;
                 if (!ahead) {
-                    ok = mbar_wait(full + s, (it / S::kStages) & 1);
+                    ok = __all_sync(0xffffffffu, mbar_wait(full + s, (it / S::kStages) & 1));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    bring_scales(it);
+                    if (issues) bring_scales(it);
                 }
                 // the next stage's scales go first, if they are here: they are copied under this stage's products
-                ahead = kb + 1 < n_k && mbar_here(full + (it + 1) % S::kStages, ((it + 1) / S::kStages) & 1);
+                ahead = kb + 1 < n_k && __all_sync(0xffffffffu, mbar_here(full + (it + 1) % S::kStages, ((it + 1) / S::kStages) & 1));
                 if (ahead) {
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    bring_scales(it + 1);
+                    if (issues) bring_scales(it + 1);
                 }
                 const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride);
                 const uint32_t w_col = tmem_base + S::kScaleCol + (it & 1) * S::kScaleCols, x_col = w_col + 4 * S::kSteps + first;
                 const uint64_t a_desc = smem_desc(at);
+                if (issues) {
 #pragma unroll
                 for (int term = 0; term < S::kT; ++term) {
                     const uint64_t b_desc = smem_desc(at + S::kASmem + term * S::kBSmem);
@@ -272,13 +274,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                     }
                 }
                 pair_commit(empty + s);                    // the stage is free in both blocks when these products are done
+                }
+                __syncwarp();
             }
             if (ok) {
-                pair_commit(acc_full + buf);
+                if (issues) pair_commit(acc_full + buf);
             } else {                                       // (the warps that wait for this accumulator, in both blocks, give up by themselves)
-                if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
                 *give_up = 1;
             }
+            __syncwarp();
         }
     } else if (warp >= 2) {
         // ---- epilogue: a warp reads tensor-memory lanes 32 * (warp % 4) .. + 31 (= features), every fourth chunk of 32 columns (= rows)
@@ -336,7 +341,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     pair_barrier();                            // neither block leaves while the other may reach into it
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512) : "memory");
     }
 }
 

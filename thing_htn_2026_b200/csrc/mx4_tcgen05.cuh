@@ -15,6 +15,17 @@ constexpr unsigned long long kWaitLimitNs = 20ull * 1000 * 1000;   // a wait giv
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// The warp of this thread, as a number that the compiler knows to be the same for the whole warp.  What a warp computes from such
+// numbers alone stands in uniform registers, where the tensor core's instructions want their operands: with a single thread's
+// numbers an instruction took 55 to 75 clocks to issue, most of it on the way of its operands there.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+// One thread of a whole warp says yes.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
+}
+
 __device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count));
 }
