@@ -7,23 +7,23 @@
 //    their sums are added at the end.  Up to kConverted rows this happens in the kernel, a half warp for a row's 128
 //    columns, beside the copies of W; more rows are prepared by a kernel of their own (mx4_terms_kernel), since every block would
 //    do it again, and come by TMA.  Rows in 4 bits are brought as W is.
-//  * A tile of 128 outputs is cut along K among the blocks of a cluster, whose partial sums meet in distributed shared memory
-//    and are added in ascending order: no scratch memory, no counters, the same result every time.
-//  * Two blocks a multiprocessor while the rows are few: the bytes in flight cover the memory's latency, and one block's
-//    start and end lie under the other's stream.
+//  * Few tiles of 128 outputs: each is cut along K among the blocks of a cluster, whose partial sums meet in distributed shared
+//    memory and are added in ascending order: no scratch memory, no counters, the same result every time.  More tiles: a block
+//    alone walks several, and brings the next one's while the last one's sums are stored.
+//  * Two blocks a multiprocessor while the rows are few: the bytes in flight cover the memory's latency.
 //
 // Every wait on an mbarrier is bounded: after kWaitLimitNs the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, the
 // block's partial sums become NaN, and tensor memory is given back.  No wait depends on another block.
+#include <array>
+
 #include "mx4_tcgen05.cuh"
 
 namespace {
 
 constexpr int BW = 128, BK = 128, UMMA_K = 32;
-constexpr int kThreads = 192;                          // warp 0: TMA, warp 1: products and tensor memory, warps 2-5: rows of x, then the sums
 constexpr uint32_t kWSmem = BW * BK, kWBytes = kWSmem / 2;     // in shared memory; as the barrier counts
 constexpr int kMaxStages = 12;
 constexpr int kMaxCluster = 8;
-
 constexpr int kConverted = 8;                          // rows that the kernel itself brings to terms
 
 // RT: the rows' type (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for
@@ -32,18 +32,22 @@ struct Shape {
     static constexpr bool kQuantized = sizeof(RT) == 1, kConverts = !kQuantized && MR <= kConverted;
     static constexpr int kT = kQuantized ? 1 : kTerms<RT>;
     static constexpr int NX = MR * kT < 16 ? 16 : MR * kT;           // columns of the product
+    static constexpr int kThreads = 192 + (kConverts ? 128 : 0);     // warp 0: TMA, warp 1: products and tensor memory, 2-5: sums, 6-9: rows to terms
     static constexpr int kXAtoms = (NX + 127) / 128;
     static constexpr uint32_t kXSmem = NX * BK;
     static constexpr uint32_t kStageBytes = kWSmem + kXSmem + (1 + kXAtoms) * kMx4AtomBytes;
     static constexpr uint32_t kStageStride = (kStageBytes + 1023) / 1024 * 1024;
     static constexpr int kRecvFloats = (MR + kMaxCluster) * BW;      // [own row][sending block][output]
     static constexpr size_t kFixed = kRecvFloats * 4 + 1024 /* alignment */ + 512 /* barriers */;
-    static constexpr size_t kBudget = 3 * kStageStride + kFixed <= 113 * 1024 ? 113 * 1024 : 226 * 1024;
+    static constexpr size_t kBudget = 4 * kStageStride + kFixed <= 113 * 1024 ? 113 * 1024 : 226 * 1024;
     static constexpr int kFit = (int)((kBudget - kFixed) / kStageStride);
     static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
+    static_assert(kStages >= 4, "four warps bring rows to terms in turn: a warp must be within a round of the ring");
     static constexpr size_t kSmemBytes = kStages * kStageStride + kFixed;
-    static constexpr int kUsedCols = NX + 4 + 4 * kXAtoms;
-    static constexpr int kTmemCols = kUsedCols <= 32 ? 32 : kUsedCols <= 64 ? 64 : kUsedCols <= 128 ? 128 : 256;
+    static constexpr int kScaleCols = 4 + 4 * kXAtoms;               // of a stage; two stages' in turn, behind the two accumulators
+    static constexpr int kUsedCols = 2 * NX + 2 * kScaleCols;
+    static constexpr int kTmemCols = kUsedCols <= 64 ? 64 : kUsedCols <= 128 ? 128 : kUsedCols <= 256 ? 256 : 512;
+    static_assert(kUsedCols <= 512, "tensor memory");
     static constexpr uint32_t kInstr = scaled_instr(kE2M1, kQuantized ? kE2M1 : kE4M3, BW, NX);
 };
 
@@ -53,7 +57,7 @@ struct Args {
     const uint8_t* x_scales;      // 4 bits, and terms that were prepared
     const uint8_t* w_scales;
     const void* bias;
-    int M, N, K, chunks, vector;  // vector: x's rows are whole aligned 16-byte pieces
+    int M, N, K, chunks, n_tiles, vector;      // vector: x's rows are whole aligned 16-byte pieces
     int* err;
     int skip_loads;               // the test of the bounded waits: nothing is loaded
 };
@@ -78,8 +82,8 @@ __device__ __forceinline__ void store_to_block(float* mine, uint32_t rank, float
 }
 
 template <typename RT, int MR, typename OutT, typename BiasT>
-__global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                                                              const Args a) {
+__global__ void __launch_bounds__(Shape<RT, MR>::kThreads) mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                                             const __grid_constant__ CUtensorMap map_x, const Args a) {
     using S = Shape<RT, MR>;
     pdl_launch_dependents();
     extern __shared__ unsigned char smem_raw[];
@@ -87,204 +91,269 @@ __global__ void __launch_bounds__(kThreads) mx4_stream_kernel(const __grid_const
     float* recv = reinterpret_cast<float*>(tiles + (size_t)S::kStages * S::kStageStride);
     uint64_t* full = reinterpret_cast<uint64_t*>(recv + S::kRecvFloats);
     uint64_t* empty = full + S::kStages;
-    uint64_t* acc_full = empty + S::kStages;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+    uint64_t* acc_full = empty + S::kStages;   // [2] accumulator ready to be summed
+    uint64_t* acc_empty = acc_full + 2;        // [2] accumulator read
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), n_ranks = (int)cluster_size();
-    const int tile = blockIdx.x / n_ranks;
-    const int c0 = (int)((long long)a.chunks * rank / n_ranks), c1 = (int)((long long)a.chunks * (rank + 1) / n_ranks);
+    // A cluster of several blocks has one tile; a block alone walks tiles first, first + grid, ...
+    const int first_tile = blockIdx.x / n_ranks, step = gridDim.x / n_ranks;
+    const int c0 = (int)((long long)a.chunks * rank / n_ranks), n = (int)((long long)a.chunks * (rank + 1) / n_ranks) - c0;
+    auto give_up_at = [&] {
+        if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+        *give_up = 1;
+    };
 
-    if (warp == 0) {
-        if (lane < S::kStages) mbar_init(full + lane, S::kConverts ? 5 : 1);      // the copies, and the four warps that bring x
-        else if (lane < 2 * S::kStages) mbar_init(empty + (lane - S::kStages), 1);
-        else if (lane == 2 * S::kStages) mbar_init(acc_full, 1);
-        if (lane == 0) *give_up = 0;
+    auto load_w = [&](int s, int tile, int c) {
+        constexpr uint32_t kBytes = kWBytes + kMx4AtomBytes + (S::kConverts ? 0 : S::kXSmem / (S::kQuantized ? 2 : 1) + kMx4AtomBytes * S::kXAtoms);
+        unsigned char* dst = tiles + (size_t)s * S::kStageStride;
+        mbar_expect_tx(full + s, kBytes);
+        tma_load_2d(dst, &map_w, full + s, c * BK, tile * BW);
+        bulk_load(dst + kWSmem + S::kXSmem, a.w_scales + ((long long)tile * a.chunks + c) * kMx4AtomBytes, kMx4AtomBytes, full + s);
+    };
+    const int early = a.skip_loads ? 0 : min(S::kStages, n);
+    if (warp == 0 && elect_one()) {
+        // W of the first stages, before anything else: nobody but this thread need know of the barriers yet
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(full + s, S::kConverts ? 2 : 1);     // the copies, and the warp that brings x
+            mbar_init(empty + s, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(acc_full + i, 1);
+            mbar_init(acc_empty + i, 4);
+        }
+        *give_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int i = 0; i < early; ++i) load_w(i, first_tile, c0 + i);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                      "r"(S::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_base = *tmem_slot;
-    cluster_arrive();                          // this block has begun: the others may reach into it
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    if (n_ranks > 1) cluster_arrive();         // this block has begun: the others may reach into it
 
-    if (warp == 0 && lane == 0) {
-        // ---- TMA producer: W of the first stages before the wait for the kernel that makes x
-        const int n = a.skip_loads ? 0 : c1 - c0;
-        const uint32_t bytes = kWBytes + kMx4AtomBytes + (S::kConverts ? 0 : S::kXSmem / (S::kQuantized ? 2 : 1) + kMx4AtomBytes * S::kXAtoms);
-        auto load_w = [&](int s, int c) {
-            unsigned char* dst = tiles + (size_t)s * S::kStageStride;
-            mbar_expect_tx(full + s, bytes);
-            tma_load_2d(dst, &map_w, full + s, c * BK, tile * BW);
-            bulk_load(dst + kWSmem + S::kXSmem, a.w_scales + ((long long)tile * a.chunks + c) * kMx4AtomBytes, kMx4AtomBytes, full + s);
-        };
-        auto load_x = [&](int s, int c) {
-            if constexpr (!S::kConverts) {
-                unsigned char* dst = tiles + (size_t)s * S::kStageStride;
-                tma_load_2d(dst + kWSmem, &map_x, full + s, c * BK, 0);
+    if (warp == 0) {
+        // ---- the copies
+        if (elect_one()) {
+            auto load_x = [&](int s, int c) {
+                if constexpr (!S::kConverts) {
+                    unsigned char* dst = tiles + (size_t)s * S::kStageStride;
+                    tma_load_2d(dst + kWSmem, &map_x, full + s, c * BK, 0);
 #pragma unroll
-                for (int j = 0; j < S::kXAtoms; ++j)
-                    bulk_load(dst + kWSmem + S::kXSmem + (1 + j) * kMx4AtomBytes, a.x_scales + ((long long)j * a.chunks + c) * kMx4AtomBytes,
-                              kMx4AtomBytes, full + s);
-            }
-        };
-        const int early = min(S::kStages, n);
-        for (int i = 0; i < early; ++i) load_w(i, c0 + i);
-        pdl_wait();
-        for (int i = 0; i < early; ++i) load_x(i, c0 + i);
-        for (int i = early; i < n && !*give_up; ++i) {
-            const int s = i % S::kStages;
-            if (!mbar_wait(empty + s, ((i / S::kStages) & 1) ^ 1)) {
-                if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
-                *give_up = 1;
-                break;
-            }
-            load_w(s, c0 + i);
-            load_x(s, c0 + i);
-        }
-    } else if (warp == 1 && lane == 0) {
-        // ---- the products
-        const uint32_t w_col = tmem_base + S::NX, x_col = w_col + 4;
-        bool ok = true;
-        for (int i = 0; i < c1 - c0 && ok && !*give_up; ++i) {
-            const int s = i % S::kStages;
-            ok = mbar_wait(full + s, (i / S::kStages) & 1);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride), scales = at + kWSmem + S::kXSmem;
-            scales_to_tmem(w_col, scale_desc(scales));
-#pragma unroll
-            for (int j = 0; j < S::kXAtoms; ++j) scales_to_tmem(x_col + 4 * j, scale_desc(scales + (1 + j) * kMx4AtomBytes));
-            const uint64_t w_desc = smem_desc(at), x_desc = smem_desc(at + kWSmem);
-#pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k)          // 32 bytes further along K: + 2 in the address field
-                mma_scaled(tmem_base, w_desc + 2 * k, x_desc + 2 * k, with_scale_byte(S::kInstr, k), w_col, x_col, (i | k) != 0);
-            umma_commit(empty + s);
-        }
-        if (!ok) {
-            if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
-            *give_up = 1;
-            __threadfence_block();
-        }
-        umma_commit(acc_full);
-    } else if (warp >= 2) {
-        pdl_wait();
-        const int quarter = warp & 3;
-        if constexpr (S::kConverts) {
-            // ---- rows of x to terms.  An item is a row's 128 columns of a chunk; the eight half warps take every eighth, a thread eight columns, and
-            // have kAhead of theirs under way.  All four warps go through every chunk, with an item of it or without, so that none is more than
-            // a round of the ring ahead of the products (a barrier's parity tells one round from the next, no more).
-            constexpr int kAhead = 4;
-            const int piece = threadIdx.x & 15, items = (c1 - c0) * a.M;
-            int item = (threadIdx.x - 64) >> 4;                      // this half warp's next one
-            Eight<RT> held[kAhead];
-            auto fetch = [&](int which, Eight<RT>& e) {
-                const int i = which / a.M, row = which - i * a.M;
-                if (which < items) e.load(static_cast<const RT*>(a.x) + (long long)row * a.K, (c0 + i) * BK + piece * 8, a.K, a.vector);
+                    for (int j = 0; j < S::kXAtoms; ++j)
+                        bulk_load(dst + kWSmem + S::kXSmem + (1 + j) * kMx4AtomBytes, a.x_scales + ((long long)j * a.chunks + c) * kMx4AtomBytes,
+                                  kMx4AtomBytes, full + s);
+                }
             };
+            pdl_wait();
+            for (int i = 0; i < early; ++i) load_x(i, c0 + i);
+            int it = early;
+            for (int tile = first_tile, i0 = early; tile < a.n_tiles && !a.skip_loads && !*give_up; tile += step, i0 = 0) {
+                for (int i = i0; i < n; ++i, ++it) {
+                    const int s = it % S::kStages;
+                    if (!mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1)) {
+                        give_up_at();
+                        break;
+                    }
+                    load_w(s, tile, c0 + i);
+                    load_x(s, c0 + i);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- the products: the whole warp walks, one thread of it issues
+        const bool issues = elect_one();
+        int it = 0, local = 0;
+        for (int tile = first_tile; tile < a.n_tiles && !__any_sync(0xffffffffu, *give_up); tile += step, ++local) {
+            const int buf = local & 1;
+            auto bring_scales = [&](int it) {
+                const uint32_t from = smem_addr(tiles + (size_t)(it % S::kStages) * S::kStageStride) + kWSmem + S::kXSmem;
+                const uint32_t to = tmem_base + 2 * S::NX + (it & 1) * S::kScaleCols;
 #pragma unroll
-            for (int h = 0; h < kAhead; ++h) fetch(item + 8 * h, held[h]);
-            for (int i = 0; i < c1 - c0; ++i) {
+                for (int j = 0; j < 1 + S::kXAtoms; ++j) scales_to_tmem(to + 4 * j, scale_desc(from + j * kMx4AtomBytes));
+            };
+            bool ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local >> 1) & 1) ^ 1));
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t tmem_d = tmem_base + buf * S::NX;
+            bool ahead = false;                // this stage has come, and its scales are on their way
+            for (int i = 0; i < n && ok; ++i, ++it) {
+                const int s = it % S::kStages;
+                if (!ahead) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full + s, (it / S::kStages) & 1));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (issues) bring_scales(it);
+                }
+                // the next stage's scales go first, if they are here: they are copied under this stage's products
+                ahead = i + 1 < n && __all_sync(0xffffffffu, mbar_here(full + (it + 1) % S::kStages, ((it + 1) / S::kStages) & 1));
+                if (ahead) {
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (issues) bring_scales(it + 1);
+                }
+                const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride);
+                const uint32_t w_col = tmem_base + 2 * S::NX + (it & 1) * S::kScaleCols;
+                const uint64_t w_desc = smem_desc(at), x_desc = smem_desc(at + kWSmem);
+                if (issues) {
+#pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; ++k)  // 32 bytes further along K: + 2 in the address field
+                        mma_scaled(tmem_d, w_desc + 2 * k, x_desc + 2 * k, with_scale_byte(S::kInstr, k), w_col, w_col + 4, (i | k) != 0);
+                    umma_commit(empty + s);
+                }
+                __syncwarp();
+            }
+            if (ok) {
+                if (issues) umma_commit(acc_full + buf);
+            } else if (lane == 0) {            // (the warps that wait for this accumulator give up by themselves)
+                give_up_at();
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 6) {
+        if constexpr (S::kConverts) {
+            // ---- rows of x to terms: chunk by chunk in turn among four warps, a half warp a row, a thread eight columns.  A warp is within a round of
+            // the ring, because the stage that it filled last was free (and there are as many stages as warps).
+            constexpr int kPasses = MR / 2;
+            const int half = lane >> 4, piece = lane & 15;
+            Eight<RT> held[kPasses];
+            auto fetch = [&](int i) {
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    const int row = 2 * p + half;
+                    if (row < a.M) held[p].load(static_cast<const RT*>(a.x) + (long long)row * a.K, (c0 + i) * BK + piece * 8, a.K, a.vector);
+                }
+            };
+            const int per = n, tiles_here = first_tile < a.n_tiles ? (a.n_tiles - first_tile + step - 1) / step : 0;
+            const long long total = (long long)per * tiles_here;
+            pdl_wait();
+            int i = warp - 6;                  // the chunk within its tile
+            while (per > 0 && i >= per) i -= per;
+            if (warp - 6 < total) fetch(i);
+            for (long long it = warp - 6; it < total; it += 4) {
                 if (__any_sync(0xffffffffu, *give_up)) break;        // all lanes together
-                const int s = i % S::kStages;
-                if (i >= S::kStages && !__all_sync(0xffffffffu, mbar_wait(empty + s, ((i / S::kStages) & 1) ^ 1))) {
-                    if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
-                    *give_up = 1;
+                const int s = (int)(it % S::kStages);
+                if (it >= S::kStages && !__all_sync(0xffffffffu, mbar_wait(empty + s, (uint32_t)((it / S::kStages) & 1) ^ 1))) {
+                    if (lane == 0) give_up_at();
                     break;
                 }
-                const bool there = item < (i + 1) * a.M;             // (at most one a chunk: no more than eight rows)
-                if (__any_sync(0xffffffffu, there)) {
-                    uint32_t top = there ? held[0].top() : 0;
+                unsigned char* dst = tiles + (size_t)s * S::kStageStride + kWSmem;
+#pragma unroll
+                for (int p = 0; p < kPasses; ++p) {
+                    const int row = 2 * p + half;
+                    if (2 * p >= a.M) break;                         // the same for all
+                    uint32_t top = row < a.M ? held[p].top() : 0;
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    if (there) {
-                        unsigned char* dst = tiles + (size_t)s * S::kStageStride + kWSmem;
-                        const int row = item - i * a.M;
+                    if (row < a.M) {
                         const uint32_t b = row_scale_byte(top);
-                        held[0].terms(b, [&](int term, uint2 bytes) {
+                        held[p].terms(b, [&](int term, uint2 bytes) {
                             const int column = term * MR + row;
                             *reinterpret_cast<uint2*>(dst + column * BK + (((piece >> 1) ^ (column & 7)) << 4) + (piece & 1) * 8) = bytes;
                             if ((piece & 3) == 0)
                                 dst[S::kXSmem + kMx4AtomBytes + (column & 31) * 16 + (column >> 5) * 4 + (piece >> 2)] = (uint8_t)term_scale_byte(b, term);
                         });
-#pragma unroll
-                        for (int h = 0; h + 1 < kAhead; ++h) held[h] = held[h + 1];
-                        fetch(item + 8 * kAhead, held[kAhead - 1]);
-                        item += 8;
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
                 if (lane == 0) mbar_arrive(full + s);
+                i += 4;
+                while (i >= per) i -= per;
+                if (it + 4 < total) fetch(i);
             }
             __syncwarp();
         }
-        // ---- this block's partial sums, row by row, to the rows' owners
-        const int r = quarter * 32 + lane;
-        float acc[MR];
-#pragma unroll
-        for (int j = 0; j < MR; ++j) acc[j] = 0.f;
-        if (c1 > c0) {
-            if (__all_sync(0xffffffffu, mbar_wait(acc_full, 0))) {      // all lanes together before tcgen05.ld
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    } else {
+        // ---- the sums: a thread has an output of the tile
+        pdl_wait();
+        const int r = (warp & 3) * 32 + lane;
+        bool dead = false;
+        int local = 0;
+        for (int tile = first_tile; tile < a.n_tiles; tile += step, ++local) {
+            const int buf = local & 1, out_n = tile * BW + r;
+            const float bias = a.bias && out_n < a.N ? to_f32<BiasT>(static_cast<const BiasT*>(a.bias)[out_n]) : 0.f;
+            if (!dead) {
+                const bool came = mbar_wait(acc_full + buf, (local >> 1) & 1);
+                dead = !__all_sync(0xffffffffu, came && !*give_up);              // all lanes together before tcgen05.ld
+                if (dead && lane == 0) give_up_at();
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t taddr = tmem_base + buf * S::NX + ((uint32_t)((warp & 3) * 32) << 16);
+            // calls put(row, sum) for the rows
+            auto rows = [&](auto put) {
 #pragma unroll
                 for (int j = 0; j < MR; j += 8) {
+                    if (j >= a.M) break;                             // the same for all
                     float v[S::kT][8];
+                    if (dead) {
 #pragma unroll
-                    for (int term = 0; term < S::kT; ++term) tmem_load_8(taddr + term * MR + j, v[term]);
-                    tmem_wait_load();
+                        for (int e = 0; e < 8; ++e) v[0][e] = __uint_as_float(0x7fffffffu);
 #pragma unroll
-                    for (int term = S::kT - 1; term >= 0; --term)        // the smallest first
+                        for (int term = 1; term < S::kT; ++term)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) acc[j + e] += v[term][e];
+                            for (int e = 0; e < 8; ++e) v[term][e] = 0.f;
+                    } else {
+#pragma unroll
+                        for (int term = 0; term < S::kT; ++term) tmem_load_8(taddr + term * MR + j, v[term]);
+                        tmem_wait_load();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float sum = v[S::kT - 1][e];                 // the smallest first
+#pragma unroll
+                        for (int term = S::kT - 2; term >= 0; --term) sum += v[term][e];
+                        if (j + e < a.M) put(j + e, sum);
+                    }
                 }
+            };
+            if (n_ranks == 1) {
+                rows([&](int row, float sum) {
+                    if (out_n < a.N) static_cast<OutT*>(a.out)[(long long)row * a.N + out_n] = from_f32<OutT>(sum + bias);
+                });
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + buf);
             } else {
-                if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
-                *give_up = 1;
-            }
-            if (*give_up) {
+                // this block's partial sums to the rows' owners: row j goes to block j % n_ranks, as its row j / n_ranks, sender `rank`
+                __syncwarp();
+                cluster_wait();                                      // every block has begun
+                int owner = 0, slot = rank;                          // slot = (j / n_ranks) * n_ranks + rank, kept without divisions
+                rows([&](int, float sum) {
+                    store_to_block(recv + slot * BW + r, (uint32_t)owner, sum);
+                    if (++owner == n_ranks) {
+                        owner = 0;
+                        slot += n_ranks;
+                    }
+                });
+                __syncwarp();
+                cluster_arrive();
+                cluster_wait();                                      // the partial sums are where they are added
+                for (int j = rank, own = 0; j < a.M; j += n_ranks, ++own) {
+                    float v[kMaxCluster];
 #pragma unroll
-                for (int j = 0; j < MR; ++j) acc[j] = __uint_as_float(0x7fffffffu);
-            }
-        }
-        __syncwarp();
-        cluster_wait();                             // every block has begun
-        // row j goes to block j % n_ranks, as that block's row j / n_ranks, sender `rank`
-        int owner = 0, slot = rank;                 // slot = (j / n_ranks) * n_ranks + rank, kept without divisions
+                    for (int q = 0; q < kMaxCluster; ++q) v[q] = q < n_ranks ? recv[(own * n_ranks + q) * BW + r] : 0.f;
+                    float sum = 0.f;                                 // in ascending order of K
 #pragma unroll
-        for (int j = 0; j < MR; ++j) {
-            if (j < a.M) store_to_block(recv + slot * BW + r, (uint32_t)owner, acc[j]);
-            if (++owner == n_ranks) {
-                owner = 0;
-                slot += n_ranks;
+                    for (int q = 0; q < kMaxCluster; ++q) sum += v[q];
+                    if (out_n < a.N) static_cast<OutT*>(a.out)[(long long)j * a.N + out_n] = from_f32<OutT>(sum + bias);
+                }
             }
         }
     }
-    __syncwarp();
-    if (warp < 2) cluster_wait();
-    cluster_arrive();
-    cluster_wait();                            // the partial sums are where they are added
-    if (warp >= 2) {
-        // ---- this block's rows, partial sums added in ascending order of K
-        const int r = (warp & 3) * 32 + lane;
-        const int n = tile * BW + r;
-        const float bias = a.bias && n < a.N ? to_f32<BiasT>(static_cast<const BiasT*>(a.bias)[n]) : 0.f;
-        for (int j = rank, own = 0; j < a.M; j += n_ranks, ++own) {
-            float v[kMaxCluster];
-#pragma unroll
-            for (int q = 0; q < kMaxCluster; ++q) v[q] = q < n_ranks ? recv[(own * n_ranks + q) * BW + r] : 0.f;
-            float sum = 0.f;
-#pragma unroll
-            for (int q = 0; q < kMaxCluster; ++q) sum += v[q];
-            if (n < a.N) static_cast<OutT*>(a.out)[(long long)j * a.N + n] = from_f32<OutT>(sum + bias);
-        }
+    if (n_ranks > 1 && (warp < 2 || warp >= 6)) {          // (the warps of the sums have been through both)
+        __syncwarp();
+        cluster_wait();
+        cluster_arrive();
+        cluster_wait();
     }
     if (*give_up) let_copies_land();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -329,15 +398,34 @@ __global__ void __launch_bounds__(256) mx4_terms_kernel(uint8_t* __restrict__ by
     });
 }
 
-// The blocks of a cluster: as many as the resident blocks leave for a tile, two a multiprocessor where they fit, and no
-// more than there are pieces of K.
-template <typename RT, int MR>
-int cluster_for(int n_tiles, int chunks, int n_sms) {
-    const int resident = n_sms * (Shape<RT, MR>::kSmemBytes <= 113 * 1024 ? 2 : 1);
-    int c = resident / n_tiles;
-    if (c > kMaxCluster) c = kMaxCluster;
-    if (c > chunks) c = chunks;
-    return c < 1 ? 1 : c;
+// The largest cluster of which n_tiles are resident together and have a piece of K a block; 1: a block alone.
+template <typename RT, int MR, typename Kernel>
+int cluster_for(Kernel kernel, int n_tiles, int chunks) {
+    using S = Shape<RT, MR>;
+    static const std::array<int, kMaxCluster + 1> resident = [&] {       // clusters of each size
+        std::array<int, kMaxCluster + 1> n = {};
+        for (int c = 2; c <= kMaxCluster; ++c) {
+            cudaLaunchConfig_t config = {};
+            config.gridDim = dim3((unsigned)(c * 512));
+            config.blockDim = dim3(S::kThreads);
+            config.dynamicSmemBytes = S::kSmemBytes;
+            cudaLaunchAttribute attribute[1];
+            attribute[0].id = cudaLaunchAttributeClusterDimension;
+            attribute[0].val.clusterDim.x = (unsigned)c;
+            attribute[0].val.clusterDim.y = 1;
+            attribute[0].val.clusterDim.z = 1;
+            config.attrs = attribute;
+            config.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n[c], kernel, &config) != cudaSuccess) {
+                cudaGetLastError();
+                n[c] = 0;
+            }
+        }
+        return n;
+    }();
+    for (int c = kMaxCluster; c >= 2; --c)
+        if (c <= chunks && resident[c] >= n_tiles) return c;
+    return 1;
 }
 
 template <typename RT, int MR, typename OutT, typename BiasT>
@@ -352,8 +440,10 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Args& args,
     int device = 0, n_sms = 0;
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
-    const int n_tiles = (args.N + BW - 1) / BW, c = cluster_for<RT, MR>(n_tiles, args.chunks, n_sms);
-    thn_launch_cluster(kernel, dim3((unsigned)(n_tiles * c)), dim3(kThreads), S::kSmemBytes, stream, dim3((unsigned)c, 1, 1), map_w, map_x, args);
+    const int c = cluster_for<RT, MR>(kernel, args.n_tiles, args.chunks);
+    const int slots = n_sms * (S::kSmemBytes <= 113 * 1024 ? 2 : 1);
+    const int grid = c > 1 ? args.n_tiles * c : args.n_tiles < slots ? args.n_tiles : slots;
+    thn_launch_cluster(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::kSmemBytes, stream, dim3((unsigned)c, 1, 1), map_w, map_x, args);
     return thn_launch_status("mx4_stream");
 }
 
@@ -436,6 +526,7 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     args.N = N;
     args.K = K;
     args.chunks = (int)(padded / BK);
+    args.n_tiles = (N + BW - 1) / BW;
     args.vector = ((uintptr_t)x & 15) == 0 && K % 8 == 0;
     args.err = err;
     args.skip_loads = skip_loads;
