@@ -44,7 +44,7 @@ struct Shape {
 struct Args {
     void* out;
     const void* bias;
-    int M, N, atoms;                // atoms: pieces of 128 columns of the sum
+    int bias_dtype, M, N, atoms;                // atoms: pieces of 128 columns of the sum
     int cuts, size, n_tiles;        // the rows of x in equal tiles
     int plane_atoms;                // rows of a term's plane / 128
     int* err;
@@ -134,7 +134,7 @@ struct Tile {
     int row0, here, columns, feature;
 };
 
-template <int MODE, typename OutT, typename BiasT>
+template <int MODE, typename OutT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pair_kernel(
     const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w_scales, const __grid_constant__ CUtensorMap map_x,
     const __grid_constant__ CUtensorMap map_x_scales, const Args a) {
@@ -295,7 +295,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
             const int buf = local % S::kBuffers;
             const int feature = t.feature + rank * 128 + quarter * 32 + lane;
             const bool there = feature < a.N;
-            const float bias = a.bias && there ? to_f32<BiasT>(static_cast<const BiasT*>(a.bias)[feature]) : 0.f;
+            const float bias = bias_of(a.bias, a.bias_dtype, feature, a.N);
             if (!dead) {
                 const bool came = mbar_wait(acc_full + buf, (local / S::kBuffers) & 1);
                 dead = !__all_sync(0xffffffffu, came && !*give_up);      // all lanes together before tcgen05.ld
@@ -367,9 +367,9 @@ bool map_planes(CUtensorMap* map, const void* base, long long width, long long r
                     {(cuuint64_t)width, (cuuint64_t)(width * rows), 0}, {128, (cuuint32_t)box_rows, (cuuint32_t)planes, 1}, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int MODE, typename OutT, typename BiasT>
+template <int MODE, typename OutT>
 int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) {
-    auto kernel = mx4_pair_kernel<MODE, OutT, BiasT>;
+    auto kernel = mx4_pair_kernel<MODE, OutT>;
     static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE>::kSmemBytes);
     if (configured != cudaSuccess) {
         thn_set_error("mx4_pair: cannot reserve %zu bytes of shared memory: %s", Shape<MODE>::kSmemBytes, cudaGetErrorString(configured));
@@ -384,7 +384,7 @@ int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) 
 }
 
 template <int MODE>
-int run(Args args, const void* codes, const void* scales, const void* x, const void* x_scales, int out_dtype, int bias_dtype, cudaStream_t stream) {
+int run(Args args, const void* codes, const void* scales, const void* x, const void* x_scales, int out_dtype, cudaStream_t stream) {
     using S = Shape<MODE>;
     const long long padded = (long long)args.atoms * kMx4Atom;
     args.cuts = (args.M + S::kCols - 1) / S::kCols;
@@ -406,10 +406,7 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
         thn_set_error("mx4_pair: cuTensorMapEncodeTiled failed for M=%d N=%d and %d pieces of K", args.M, args.N, args.atoms);
         return THN_BAD_ARGUMENT;
     }
-    if (out_dtype == THN_F32)
-        return bias_dtype == THN_F32 ? launch<MODE, float, float>(maps, args, stream) : launch<MODE, float, __nv_bfloat16>(maps, args, stream);
-    return bias_dtype == THN_F32 ? launch<MODE, __nv_bfloat16, float>(maps, args, stream)
-                                 : launch<MODE, __nv_bfloat16, __nv_bfloat16>(maps, args, stream);
+    return out_dtype == THN_F32 ? launch<MODE, float>(maps, args, stream) : launch<MODE, __nv_bfloat16>(maps, args, stream);
 }
 
 }  // namespace
@@ -439,6 +436,7 @@ THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_
     Args args = {};
     args.out = out;
     args.bias = bias;
+    args.bias_dtype = bias_dtype;
     args.M = M;
     args.N = N;
     args.atoms = (int)(mx4_padded(K) / kMx4Atom);
@@ -446,12 +444,12 @@ THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_
     args.skip_loads = skip_loads;
     THN_UNSUPPORTED_IF((long long)(N + 127) / 128 * args.atoms > 0x7fffffff || (long long)(M + 127) / 128 * 6 * args.atoms > 0x7fffffff,
                        "mx4_pair: M=%d N=%d K=%d: too many scales", M, N, K);
-    if (x_type == 2) return run<kQuantized>(args, codes, scales, x, x_scales, out_dtype, bias_dtype, stream);
+    if (x_type == 2) return run<kQuantized>(args, codes, scales, x, x_scales, out_dtype, stream);
     const int plane = (M + 127) / 128 * 128;
     uint8_t* bytes = static_cast<uint8_t*>(terms);
     uint8_t* term_scales = bytes + (long long)plane * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>) * mx4_padded(K);
     const int status = mx4_terms(bytes, term_scales, x, x_type, M, K, plane, stream);
     if (status != THN_OK) return status;
-    if (x_type == THN_F32) return run<kRows6>(args, codes, scales, bytes, term_scales, out_dtype, bias_dtype, stream);
-    return run<kRows2>(args, codes, scales, bytes, term_scales, out_dtype, bias_dtype, stream);
+    if (x_type == THN_F32) return run<kRows6>(args, codes, scales, bytes, term_scales, out_dtype, stream);
+    return run<kRows2>(args, codes, scales, bytes, term_scales, out_dtype, stream);
 }

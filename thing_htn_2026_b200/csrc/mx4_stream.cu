@@ -26,10 +26,11 @@ constexpr int kMaxStages = 12;
 constexpr int kMaxCluster = 8;
 constexpr int kConverted = 8;                          // rows that the kernel itself brings to terms
 
-// RT: the rows' type (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for
-template <typename RT, int MR>
+// RT: the rows' type (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for; PAIRS: how many pairs of rows the
+// kernel itself brings to terms (0: they come prepared, or in 4 bits)
+template <typename RT, int MR, int PAIRS>
 struct Shape {
-    static constexpr bool kQuantized = sizeof(RT) == 1, kConverts = !kQuantized && MR <= kConverted;
+    static constexpr bool kQuantized = sizeof(RT) == 1, kConverts = PAIRS > 0;
     static constexpr int kT = kQuantized ? 1 : kTerms<RT>;
     static constexpr int NX = MR * kT < 16 ? 16 : MR * kT;           // columns of the product
     static constexpr int kThreads = 192 + (kConverts ? 128 : 0);     // warp 0: TMA, warp 1: products and tensor memory, 2-5: sums, 6-9: rows to terms
@@ -57,7 +58,7 @@ struct Args {
     const uint8_t* x_scales;      // 4 bits, and terms that were prepared
     const uint8_t* w_scales;
     const void* bias;
-    int M, N, K, chunks, n_tiles, vector;      // vector: x's rows are whole aligned 16-byte pieces
+    int bias_dtype, M, N, K, chunks, n_tiles, vector;      // vector: x's rows are whole aligned 16-byte pieces
     int* err;
     int skip_loads;               // the test of the bounded waits: nothing is loaded
 };
@@ -81,10 +82,10 @@ __device__ __forceinline__ void store_to_block(float* mine, uint32_t rank, float
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
 }
 
-template <typename RT, int MR, typename OutT, typename BiasT>
-__global__ void __launch_bounds__(Shape<RT, MR>::kThreads) mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w,
+template <typename RT, int MR, int PAIRS, typename OutT>
+__global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                              const __grid_constant__ CUtensorMap map_x, const Args a) {
-    using S = Shape<RT, MR>;
+    using S = Shape<RT, MR, PAIRS>;
     pdl_launch_dependents();
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -220,55 +221,55 @@ __global__ void __launch_bounds__(Shape<RT, MR>::kThreads) mx4_stream_kernel(con
         }
     } else if (warp >= 6) {
         if constexpr (S::kConverts) {
-            // ---- rows of x to terms: chunk by chunk in turn among four warps, a half warp a row, a thread eight columns.  A warp is within a round of
-            // the ring, because the stage that it filled last was free (and there are as many stages as warps).
-            constexpr int kPasses = MR / 2;
+            // ---- rows of x to terms: chunk by chunk in turn among four warps, a half warp a row, a thread eight columns, the rows of a warp's next
+            // two chunks under way.  A warp is within a round of the ring, because the stage that it filled last was free (and there are as many
+            // stages as warps).  Rows behind the last one are zeros in columns that nobody reads.
             const int half = lane >> 4, piece = lane & 15;
-            Eight<RT> held[kPasses];
-            auto fetch = [&](int i) {
+            Eight<RT> held[2][PAIRS];
+            const int total = n * (first_tile < a.n_tiles ? (a.n_tiles - first_tile + step - 1) / step : 0);
+            auto fetch = [&](int it, Eight<RT> (&e)[PAIRS]) {
+                if (it >= total) return;
+                const int c = (c0 + it % n) * BK + piece * 8;
 #pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
+                for (int p = 0; p < PAIRS; ++p) {
                     const int row = 2 * p + half;
-                    if (row < a.M) held[p].load(static_cast<const RT*>(a.x) + (long long)row * a.K, (c0 + i) * BK + piece * 8, a.K, a.vector);
+                    e[p].load(static_cast<const RT*>(a.x) + (long long)min(row, a.M - 1) * a.K, c, row < a.M ? a.K : 0, a.vector);
                 }
             };
-            const int per = n, tiles_here = first_tile < a.n_tiles ? (a.n_tiles - first_tile + step - 1) / step : 0;
-            const long long total = (long long)per * tiles_here;
-            pdl_wait();
-            int i = warp - 6;                  // the chunk within its tile
-            while (per > 0 && i >= per) i -= per;
-            if (warp - 6 < total) fetch(i);
-            for (long long it = warp - 6; it < total; it += 4) {
-                if (__any_sync(0xffffffffu, *give_up)) break;        // all lanes together
-                const int s = (int)(it % S::kStages);
-                if (it >= S::kStages && !__all_sync(0xffffffffu, mbar_wait(empty + s, (uint32_t)((it / S::kStages) & 1) ^ 1))) {
+            auto convert = [&](int it, const Eight<RT> (&e)[PAIRS]) {
+                if (__any_sync(0xffffffffu, *give_up)) return false;           // all lanes together
+                const int s = it % S::kStages;
+                if (it >= S::kStages && !__all_sync(0xffffffffu, mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1))) {
                     if (lane == 0) give_up_at();
-                    break;
+                    return false;
                 }
                 unsigned char* dst = tiles + (size_t)s * S::kStageStride + kWSmem;
 #pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
-                    const int row = 2 * p + half;
-                    if (2 * p >= a.M) break;                         // the same for all
-                    uint32_t top = row < a.M ? held[p].top() : 0;
+                for (int p = 0; p < PAIRS; ++p) {
+                    uint32_t top = e[p].top();
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    if (row < a.M) {
-                        const uint32_t b = row_scale_byte(top);
-                        held[p].terms(b, [&](int term, uint2 bytes) {
-                            const int column = term * MR + row;
-                            *reinterpret_cast<uint2*>(dst + column * BK + (((piece >> 1) ^ (column & 7)) << 4) + (piece & 1) * 8) = bytes;
-                            if ((piece & 3) == 0)
-                                dst[S::kXSmem + kMx4AtomBytes + (column & 31) * 16 + (column >> 5) * 4 + (piece >> 2)] = (uint8_t)term_scale_byte(b, term);
-                        });
-                    }
+                    const uint32_t b = row_scale_byte(top);
+                    e[p].terms(b, [&](int term, uint2 bytes) {
+                        const int column = term * MR + 2 * p + half;
+                        *reinterpret_cast<uint2*>(dst + column * BK + (((piece >> 1) ^ (column & 7)) << 4) + (piece & 1) * 8) = bytes;
+                        if ((piece & 3) == 0)
+                            dst[S::kXSmem + kMx4AtomBytes + (column & 31) * 16 + (column >> 5) * 4 + (piece >> 2)] = (uint8_t)term_scale_byte(b, term);
+                    });
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + s);
-                i += 4;
-                while (i >= per) i -= per;
-                if (it + 4 < total) fetch(i);
+                return true;
+            };
+            pdl_wait();
+            fetch(warp - 6, held[0]);
+            fetch(warp - 2, held[1]);
+            for (int it = warp - 6; it < total; it += 8) {
+                if (!convert(it, held[0])) break;
+                fetch(it + 8, held[0]);
+                if (it + 4 >= total || !convert(it + 4, held[1])) break;
+                fetch(it + 12, held[1]);
             }
             __syncwarp();
         }
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(Shape<RT, MR>::kThreads) mx4_stream_kernel(con
         int local = 0;
         for (int tile = first_tile; tile < a.n_tiles; tile += step, ++local) {
             const int buf = local & 1, out_n = tile * BW + r;
-            const float bias = a.bias && out_n < a.N ? to_f32<BiasT>(static_cast<const BiasT*>(a.bias)[out_n]) : 0.f;
+            const float bias = bias_of(a.bias, a.bias_dtype, out_n, a.N);
             if (!dead) {
                 const bool came = mbar_wait(acc_full + buf, (local >> 1) & 1);
                 dead = !__all_sync(0xffffffffu, came && !*give_up);              // all lanes together before tcgen05.ld
@@ -399,9 +400,8 @@ __global__ void __launch_bounds__(256) mx4_terms_kernel(uint8_t* __restrict__ by
 }
 
 // The largest cluster of which n_tiles are resident together and have a piece of K a block; 1: a block alone.
-template <typename RT, int MR, typename Kernel>
+template <typename S, typename Kernel>
 int cluster_for(Kernel kernel, int n_tiles, int chunks) {
-    using S = Shape<RT, MR>;
     static const std::array<int, kMaxCluster + 1> resident = [&] {       // clusters of each size
         std::array<int, kMaxCluster + 1> n = {};
         for (int c = 2; c <= kMaxCluster; ++c) {
@@ -428,10 +428,10 @@ int cluster_for(Kernel kernel, int n_tiles, int chunks) {
     return 1;
 }
 
-template <typename RT, int MR, typename OutT, typename BiasT>
+template <typename RT, int MR, int PAIRS, typename OutT>
 int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Args& args, cudaStream_t stream) {
-    using S = Shape<RT, MR>;
-    auto kernel = mx4_stream_kernel<RT, MR, OutT, BiasT>;
+    using S = Shape<RT, MR, PAIRS>;
+    auto kernel = mx4_stream_kernel<RT, MR, PAIRS, OutT>;
     static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmemBytes);
     if (configured != cudaSuccess) {
         thn_set_error("mx4_stream: cannot reserve %zu bytes of shared memory: %s", S::kSmemBytes, cudaGetErrorString(configured));
@@ -440,7 +440,7 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Args& args,
     int device = 0, n_sms = 0;
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
-    const int c = cluster_for<RT, MR>(kernel, args.n_tiles, args.chunks);
+    const int c = cluster_for<S>(kernel, args.n_tiles, args.chunks);
     const int slots = n_sms * (S::kSmemBytes <= 113 * 1024 ? 2 : 1);
     const int grid = c > 1 ? args.n_tiles * c : args.n_tiles < slots ? args.n_tiles : slots;
     thn_launch_cluster(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::kSmemBytes, stream, dim3((unsigned)c, 1, 1), map_w, map_x, args);
@@ -448,9 +448,9 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Args& args,
 }
 
 // terms: for the rows' terms, kT * MR rows of `padded` bytes, then their scales (null where the kernel brings them itself)
-template <typename RT, int MR>
-int launch_rows(Args args, const void* codes, long long padded, void* terms, int out_dtype, int bias_dtype, cudaStream_t stream) {
-    using S = Shape<RT, MR>;
+template <typename RT, int MR, int PAIRS = 0>
+int launch_rows(Args args, const void* codes, long long padded, void* terms, int out_dtype, cudaStream_t stream) {
+    using S = Shape<RT, MR, PAIRS>;
     CUtensorMap map_w, map_x;
     bool made = map_unpacked(&map_w, codes, args.N, padded, BW);
     if constexpr (S::kQuantized) made = made && map_unpacked(&map_x, args.x, args.M, padded, S::NX);
@@ -466,11 +466,7 @@ int launch_rows(Args args, const void* codes, long long padded, void* terms, int
         thn_set_error("mx4_stream: cuTensorMapEncodeTiled failed for M=%d N=%d K=%d", args.M, args.N, args.K);
         return THN_BAD_ARGUMENT;
     }
-    if (out_dtype == THN_F32)
-        return bias_dtype == THN_F32 ? launch<RT, MR, float, float>(map_w, map_x, args, stream)
-                                     : launch<RT, MR, float, __nv_bfloat16>(map_w, map_x, args, stream);
-    return bias_dtype == THN_F32 ? launch<RT, MR, __nv_bfloat16, float>(map_w, map_x, args, stream)
-                                 : launch<RT, MR, __nv_bfloat16, __nv_bfloat16>(map_w, map_x, args, stream);
+    return out_dtype == THN_F32 ? launch<RT, MR, PAIRS, float>(map_w, map_x, args, stream) : launch<RT, MR, PAIRS, __nv_bfloat16>(map_w, map_x, args, stream);
 }
 
 // the rows that a block has room for
@@ -522,6 +518,7 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     args.x_scales = (const uint8_t*)x_scales;
     args.w_scales = (const uint8_t*)scales;
     args.bias = bias;
+    args.bias_dtype = bias_dtype;
     args.M = M;
     args.N = N;
     args.K = K;
@@ -530,15 +527,19 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     args.vector = ((uintptr_t)x & 15) == 0 && K % 8 == 0;
     args.err = err;
     args.skip_loads = skip_loads;
-#define GO(RT, MR) return launch_rows<RT, MR>(args, codes, padded, terms, out_dtype, bias_dtype, stream)
+#define GO(...) return launch_rows<__VA_ARGS__>(args, codes, padded, terms, out_dtype, stream)
     const int room = room_for(M);
     if (x_type == THN_F32) {
-        if (room == 8) GO(float, 8);
+        if (M <= 2) GO(float, 8, 1);
+        if (M <= 4) GO(float, 8, 2);
+        if (room == 8) GO(float, 8, 4);
         if (room == 16) GO(float, 16);
         GO(float, 32);
     }
     if (x_type == THN_BF16) {
-        if (room == 8) GO(__nv_bfloat16, 8);
+        if (M <= 2) GO(__nv_bfloat16, 8, 1);
+        if (M <= 4) GO(__nv_bfloat16, 8, 2);
+        if (room == 8) GO(__nv_bfloat16, 8, 4);
         if (room == 16) GO(__nv_bfloat16, 16);
         if (room == 32) GO(__nv_bfloat16, 32);
         GO(__nv_bfloat16, 64);

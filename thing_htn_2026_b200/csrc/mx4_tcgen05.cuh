@@ -125,6 +125,12 @@ __device__ __forceinline__ void tmem_load_8(uint32_t taddr, float* r) {
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// The bias of output n of N (null: none), whose type is a number of ThnDtype.
+__device__ __forceinline__ float bias_of(const void* bias, int dtype, int n, int N) {
+    if (bias == nullptr || n >= N) return 0.f;
+    return dtype == THN_F32 ? static_cast<const float*>(bias)[n] : __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[n]);
+}
+
 // ---- rows as they are, as sums of 8-bit floats.
 //
 // A block of 32 entries with its largest magnitude in [2^e, 2^(e+1)) is brought to [2^7, 2^8) by the scale 2^(e-7); its entries
