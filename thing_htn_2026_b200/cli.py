@@ -8,6 +8,7 @@ new tokens; prompts are seeded uniform-random ids) from tests/local_check.py:61-
     python -m thing_htn_2026_b200 generate --random-config tiny-b --seed 1 --prompt-lens 1,23 --max-new-tokens 12
     python -m thing_htn_2026_b200 random-model --random-config qwen3-4b --seed 0 --out DIR
     python -m thing_htn_2026_b200 bench --random-config qwen3-4b --shapes 8x512x64
+    python -m thing_htn_2026_b200 bench --random-config qwen3-8b --shapes 8x512x64 --weights mx4 --activations mx4
     python -m thing_htn_2026_b200 replay --model DIR --dtype float32 --out DIR --max-tokens N < steps.jsonl
 
 A model is either a folder (``--model``) or a named configuration with random weights
@@ -80,8 +81,9 @@ def _engine(args):
     if bool(args.model) == bool(args.random_config):
         raise SystemExit("give exactly one of --model DIR and --random-config NAME")
     if args.model:
-        return Engine(args.model, dtype=args.dtype, device=args.device)
-    return Engine.from_config(_named_config(args), seed=args.seed, dtype=args.dtype, device=args.device)
+        return Engine(args.model, dtype=args.dtype, device=args.device, weights=args.weights, activations=args.activations)
+    return Engine.from_config(_named_config(args), seed=args.seed, dtype=args.dtype, device=args.device, weights=args.weights,
+                              activations=args.activations)
 
 
 def _jobs(args, vocab: int):
@@ -166,6 +168,8 @@ def _model_options(p) -> None:
     p.add_argument("--device", default="cuda:0")
     p.add_argument("--dtype", default="bfloat16", type=_dtype_name, choices=["bfloat16", "float32"],
                    help="bfloat16 (bf16) or float32 (fp32)")
+    p.add_argument("--weights", choices=["mx4"], help="hold the layers' weights in microscaled 4-bit floating point")
+    p.add_argument("--activations", choices=["mx4"], help="with --weights mx4: bring what they multiply to 4 bits too")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--temperature", type=float, default=0.0, help="0 = greedy")
 

@@ -412,15 +412,20 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
 }  // namespace
 
 // The bytes of `terms` that M rows of a type need.
-THN_API long long thn_mx4_pair_scratch_bytes(int x_type, int M, int K) {
+static long long terms_needed(int x_type, int M, int K) {
     if (x_type == 2) return 0;
     const long long atoms = (long long)((M + 127) / 128) * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
     return atoms * 128 * padded + atoms * (padded / kMx4Atom) * kMx4AtomBytes;
 }
 
+THN_API int thn_mx4_pair_scratch(int x_type, int M, int K, long long* bytes) {
+    *bytes = terms_needed(x_type, M, K);
+    return THN_OK;
+}
+
 // out [M, N] of out_dtype = x [M, K] @ w [N, K]^T (+ bias [N] of bias_dtype, or null).
 //   x          [M, K] of x_type; 2: codes [M, padded / 2] with x_scales (mx4.cuh)
-//   codes, scales: W;  terms: scratch of thn_mx4_pair_scratch_bytes
+//   codes, scales: W;  terms: scratch of thn_mx4_pair_scratch
 // Scales and terms 16-byte, 4-bit codes 32-byte aligned.  err: device error word (THN_ERR_WAIT_TIMEOUT if a wait gave up).
 // skip_loads: 0; otherwise no operand is loaded, so that the waits run out (for the test of the waits only).
 THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_scales, int x_type, const void* codes, const void* scales,
@@ -431,8 +436,8 @@ THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_
     THN_UNSUPPORTED_IF(M < 1 || M > (1 << 24) || N < 1 || N > (1 << 24) || K < 1 || K > (1 << 24), "mx4_pair: M=%d N=%d K=%d not supported", M, N, K);
     THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 &&
                   (((uintptr_t)scales | (uintptr_t)x_scales | (uintptr_t)terms) & 15) == 0, "mx4_pair: codes must be 32-byte, scales and terms 16-byte aligned");
-    THN_CHECK_ARG(terms_bytes >= thn_mx4_pair_scratch_bytes(x_type, M, K), "mx4_pair: %lld bytes of scratch, %lld needed", terms_bytes,
-                  thn_mx4_pair_scratch_bytes(x_type, M, K));
+    THN_CHECK_ARG(terms_bytes >= terms_needed(x_type, M, K), "mx4_pair: %lld bytes of scratch, %lld needed", terms_bytes,
+                  terms_needed(x_type, M, K));
     Args args = {};
     args.out = out;
     args.bias = bias;

@@ -4,8 +4,8 @@
 //    narrow one.  W comes by TMA, which spreads its 4-bit codes over 8-bit containers as it copies, so no thread touches a weight;
 //    its scales come as 512 bytes for 128 rows and 128 columns, in the order of tensor memory, and go there by tcgen05.cp.
 //  * Rows in bfloat16 or float32 become two or six terms of 8-bit floats (mx4_tcgen05.cuh), a column of the narrow operand each;
-//    their sums are added at the end.  Up to kConverted rows this happens in the kernel, a half warp for a row's 128
-//    columns, beside the copies of W; more rows are prepared by a kernel of their own (mx4_terms_kernel), since every block would
+//    their sums are added at the end.  Up to converted_rows this happens in the kernel, a warp for 128 columns of
+//    them, beside the copies of W; more rows are prepared by a kernel of their own (mx4_terms_kernel), since every block would
 //    do it again, and come by TMA.  Rows in 4 bits are brought as W is.
 //  * Few tiles of 128 outputs: each is cut along K among the blocks of a cluster, whose partial sums meet in distributed shared
 //    memory and are added in ascending order: no scratch memory, no counters, the same result every time.  More tiles: a block
@@ -24,7 +24,9 @@ constexpr int BW = 128, BK = 128, UMMA_K = 32;
 constexpr uint32_t kWSmem = BW * BK, kWBytes = kWSmem / 2;     // in shared memory; as the barrier counts
 constexpr int kMaxStages = 12;
 constexpr int kMaxCluster = 8;
-constexpr int kConverted = 8;                          // rows that the kernel itself brings to terms
+// Rows that the kernel itself brings to terms, of a type.  (Float32 rows have six terms to compute: eight of them by 19,456 x 2,560 took 26 us so,
+// and 20 us prepared.)
+constexpr int converted_rows(int x_type) { return x_type == THN_F32 ? 4 : 8; }
 
 // RT: the rows' type (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for; PAIRS: how many pairs of rows the
 // kernel itself brings to terms (0: they come prepared, or in 4 bits)
@@ -490,15 +492,20 @@ int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K
 THN_API int thn_mx4_stream_rows(int x_type) { return x_type == THN_F32 ? 32 : 64; }
 
 // The bytes of `terms` that M rows of a type need.
-THN_API long long thn_mx4_stream_scratch_bytes(int x_type, int M, int K) {
-    if (x_type == 2 || M <= kConverted) return 0;
-    const long long rows = (long long)room_for(M) * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
+static long long terms_needed(int x_type, int M, int K) {
+    if (x_type == 2 || M <= converted_rows(x_type)) return 0;
+    const long long rows = (long long)(M <= 16 ? 16 : room_for(M)) * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
     return rows * padded + (rows + 127) / 128 * (padded / kMx4Atom) * kMx4AtomBytes;
+}
+
+THN_API int thn_mx4_stream_scratch(int x_type, int M, int K, long long* bytes) {
+    *bytes = terms_needed(x_type, M, K);
+    return THN_OK;
 }
 
 // out [M, N] of out_dtype = x [M, K] @ w [N, K]^T (+ bias [N] of bias_dtype, or null).
 //   x          [M, K] of x_type; 2: codes [M, padded / 2] with x_scales (mx4.cuh)
-//   codes, scales: W;  terms: scratch of thn_mx4_stream_scratch_bytes
+//   codes, scales: W;  terms: scratch of thn_mx4_stream_scratch
 // Scales and terms 16-byte, 4-bit codes 32-byte aligned.  err: device error word (THN_ERR_WAIT_TIMEOUT if a wait gave up).
 // skip_loads: 0; otherwise no operand is loaded, so that the waits run out (for the test of the waits only).
 THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* x_scales, int x_type, const void* codes, const void* scales,
@@ -509,8 +516,8 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     THN_UNSUPPORTED_IF(M < 1 || M > thn_mx4_stream_rows(x_type) || N < 1 || K < 1 || K > (1 << 24), "mx4_stream: M=%d N=%d K=%d not supported", M, N, K);
     THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 &&
                   (((uintptr_t)scales | (uintptr_t)x_scales | (uintptr_t)terms) & 15) == 0, "mx4_stream: codes must be 32-byte, scales and terms 16-byte aligned");
-    THN_CHECK_ARG(terms_bytes >= thn_mx4_stream_scratch_bytes(x_type, M, K), "mx4_stream: %lld bytes of scratch, %lld needed", terms_bytes,
-                  thn_mx4_stream_scratch_bytes(x_type, M, K));
+    THN_CHECK_ARG(terms_bytes >= terms_needed(x_type, M, K), "mx4_stream: %lld bytes of scratch, %lld needed", terms_bytes,
+                  terms_needed(x_type, M, K));
     const long long padded = mx4_padded(K);
     Args args = {};
     args.out = out;
@@ -532,8 +539,7 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     if (x_type == THN_F32) {
         if (M <= 2) GO(float, 8, 1);
         if (M <= 4) GO(float, 8, 2);
-        if (room == 8) GO(float, 8, 4);
-        if (room == 16) GO(float, 16);
+        if (room <= 16) GO(float, 16);
         GO(float, 32);
     }
     if (x_type == THN_BF16) {

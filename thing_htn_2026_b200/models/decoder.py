@@ -61,6 +61,19 @@ class DecoderModel:
                                            matrix_std, gain_std)
         return cls(config, tensors, dtype, device)
 
+    def quantize(self, weights: Optional[str], activations: Optional[str] = None) -> None:
+        """``weights`` "mx4": the weights of the layers' products are held in microscaled 4-bit floating point from here on
+        (:class:`ops.Mx4`); the embedding, the head, norms, routers, gates, convolutions and routed experts stay as they
+        are.  ``activations`` "mx4": what these products multiply is brought to 4 bits too, a row at a time, at every step.  None:
+        nothing is changed."""
+        if weights is None and activations is None:
+            return
+        if weights != "mx4" or activations not in (None, "mx4"):
+            raise ValueError(f"weights {weights!r} with activations {activations!r}: weights are 'mx4' or None, activations 'mx4' "
+                             f"(with such weights) or None")
+        if not sum(layer.quantize_products(activations == "mx4") for layer in self.layers):
+            raise ValueError("no layer of this model has products whose weights can be held in 4 bits")
+
     # ------------------------------------------------------------------ cache and positions
 
     def cache_needs(self) -> List[CacheNeed]:

@@ -152,11 +152,11 @@ _SIGNATURES = {
     "thn_mx4_quantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_arrange": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p],
-    "thn_mx4_pair_scratch_bytes": [c_int, c_int, c_int],
+    "thn_mx4_pair_scratch": [c_int, c_int, c_int, c_void_p],
     "thn_mx4_pair": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                      c_int, c_void_p, c_void_p],
     "thn_mx4_stream_rows": [c_int],
-    "thn_mx4_stream_scratch_bytes": [c_int, c_int, c_int],
+    "thn_mx4_stream_scratch": [c_int, c_int, c_int, c_void_p],
     "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                        c_int, c_void_p, c_void_p],
     "thn_gemm_f32": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -913,7 +913,8 @@ def _stream_takes(m: int, n: int, k: int, fused: bool = False) -> bool:
 def linear_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """silu(x gate^T) * (x up^T) for ``w_gate_up = cat(gate, up)``: one kernel where the
     weight-streaming product takes the shape, else the product followed by the activation."""
-    if x.dtype == torch.bfloat16 and _stream_takes(x.shape[0], w_gate_up.shape[0] // 2, x.shape[1], fused=True):
+    if not isinstance(w_gate_up, Mx4) and x.dtype == torch.bfloat16 \
+            and _stream_takes(x.shape[0], w_gate_up.shape[0] // 2, x.shape[1], fused=True):
         return linear_stream(x, w_gate_up, swiglu=True, err=err)
     return swiglu(linear(x, w_gate_up, err=err))
 
@@ -939,7 +940,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     engine/engine.py:341-350).  ``out_dtype=torch.float32`` keeps the accumulator's
     precision (used for logits).  ``bias`` (of the activation type, ``[N]``) is added to every row:
     in the vendor product's epilogue (float32, before the one rounding), or by a kernel of its own
-    after the FFMA product."""
+    after the FFMA product.  ``weight`` may be an :class:`Mx4` (:func:`linear_mx4`)."""
+    if isinstance(weight, Mx4):
+        return linear_mx4(quantize_mx4(x) if weight.quantizes_rows else x, weight, out_dtype or x.dtype, err, bias)
     if bias is not None:
         _need(bias, "linear bias", x.dtype)
         if bias.shape[0] != weight.shape[0]:
@@ -1002,12 +1005,13 @@ class Mx4:
     """A matrix ``[rows, columns]`` in microscaled 4-bit floating point: every 32 neighbouring entries of a row share a
     scale, a power of two held in a byte (``2^(byte - 127)``; 255: the block is not a number), and an entry is one of 0, 1/2, 1, 3/2,
     2, 3, 4, 6 with a sign, held in four bits.  :func:`quantize_mx4` makes one from numbers, :func:`mx4_from_parts` from stored codes
-    and scales.  ``data`` holds the codes and behind them the scales, laid out for the tensor cores (``csrc/mx4.cuh``)."""
+    and scales.  ``data`` holds the codes and behind them the scales, laid out for the tensor cores (``csrc/mx4.cuh``).
+    ``quantizes_rows``: as a weight of :func:`linear`, the rows that it multiplies are brought to 4 bits first."""
 
-    __slots__ = ("data", "rows", "columns", "code_bytes")
+    __slots__ = ("data", "rows", "columns", "code_bytes", "quantizes_rows")
 
-    def __init__(self, data: torch.Tensor, rows: int, columns: int):
-        self.data, self.rows, self.columns = data, rows, columns
+    def __init__(self, data: torch.Tensor, rows: int, columns: int, quantizes_rows: bool = False):
+        self.data, self.rows, self.columns, self.quantizes_rows = data, rows, columns, quantizes_rows
         self.code_bytes = rows * (-(-columns // 128) * 64)
 
     @classmethod
@@ -1093,6 +1097,18 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
+_mx4_terms_needs: Dict[Tuple[str, int, int, int], int] = {}
+
+
+def _mx4_terms_need(entry: str, kind: int, m: int, k: int) -> int:
+    key = (entry, kind, m, k)
+    if key not in _mx4_terms_needs:
+        size = c_longlong(0)
+        getattr(lib(), entry)(kind, m, k, ctypes.byref(size))
+        _mx4_terms_needs[key] = size.value
+    return _mx4_terms_needs[key]
+
+
 def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [M, K] @ weight[N, K]^T`` (+ ``bias [N]``) with a weight in 4 bits: float32 sums, one rounding to ``out_dtype`` (bfloat16 or
@@ -1129,10 +1145,7 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
         return out
     codes, scales = weight._pointers()
     few = m <= (32 if kind == 0 else 64)
-    if few:
-        size = 0 if kind == 2 or m <= 8 else lib().thn_mx4_stream_scratch_bytes(kind, m, k)
-    else:
-        size = 0 if kind == 2 else lib().thn_mx4_pair_scratch_bytes(kind, m, k)
+    size = 0 if kind == 2 else _mx4_terms_need("thn_mx4_stream_scratch" if few else "thn_mx4_pair_scratch", kind, m, k)
     terms = data.new_empty(size, dtype=torch.uint8) if size else None
     _call("thn_mx4_stream" if few else "thn_mx4_pair", out.data_ptr(), DTYPE_CODE[out_dtype], at, x_scales, kind, codes, scales, _ptr(bias), bias_code,
           _ptr(terms), size, m, n, k, 0, _ptr(err), _stream())

@@ -59,6 +59,8 @@ from .runtime import HostBatch, Runtime, StepContext
 
 @register_part("mixer", "attention")
 class Attention:
+    PRODUCTS = ("w_qkv", "w_o")
+
     @classmethod
     def tensor_specs(cls, spec: PartSpec) -> List[TensorSpec]:
         p = spec.params

@@ -94,6 +94,21 @@ class Block:
         mixer = getattr(self, "mixer", None)
         return mixer.cache_need() if mixer is not None else None
 
+    def quantize_products(self, quantize_rows: bool = False) -> int:
+        """Bring the weights of the members' products (their ``PRODUCTS``: names of weights that only :func:`ops.linear`
+        and :func:`ops.linear_swiglu` read) to 4 bits; ``quantize_rows``: the rows that they multiply too, at every step.
+        Returns how many there are."""
+        count = 0
+        for part in [self] + self.parts():
+            for name in getattr(part, "PRODUCTS", ()):
+                weight = getattr(part, name)
+                if isinstance(weight, torch.Tensor):
+                    quantized = ops.quantize_mx4(weight.contiguous())
+                    quantized.quantizes_rows = bool(quantize_rows)
+                    setattr(part, name, quantized)
+                    count += 1
+        return count
+
     def step_inputs(self, batch: HostBatch, out: Dict[str, List[int]]) -> None:
         """Integer inputs that members want computed on the host for this step, by name."""
         for part in self.parts():
@@ -160,6 +175,7 @@ class BranchNormBlock(Block):
 @register_part("block", "parallel")
 class ParallelBlock(Block):
     MEMBERS = {"norm": "norm", "mixer": "mixer", "ffn": "ffn", "side": "side"}
+    PRODUCTS = ("w_in",)
 
     @classmethod
     def tensor_specs(cls, spec: PartSpec) -> List[TensorSpec]:
@@ -199,6 +215,12 @@ class ParallelBlock(Block):
             if "beside" not in runtime.shared:
                 runtime.shared["beside"] = ops.Beside(runtime.device)
             self.beside = runtime.shared["beside"]
+
+    def quantize_products(self, quantize_rows: bool = False) -> int:
+        if self.w_in is not None:              # the members' slices of it are not read
+            self.mixer.take_rows(None, None)
+            self.ffn.take_rows(None, None)
+        return super().quantize_products(quantize_rows)
 
     def _sublayers(self, n: torch.Tensor, ctx: StepContext, entry: ScheduleEntry):
         if self.w_in is None:

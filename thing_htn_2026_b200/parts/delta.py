@@ -38,6 +38,8 @@ CONVOLVED = ("q", "k", "v")
 
 @register_part("mixer", "gated_delta")
 class GatedDelta:
+    PRODUCTS = ("w_in", "w_o")
+
     @staticmethod
     def _shape(spec: PartSpec) -> ops.DeltaShape:
         p = spec.params

@@ -61,6 +61,8 @@ from .runtime import Runtime
 
 @register_part("ffn", "swiglu")
 class SwiGLU:
+    PRODUCTS = ("w_gate_up", "w_down")
+
     @classmethod
     def tensor_specs(cls, spec: PartSpec) -> List[TensorSpec]:
         hidden, inter = int(spec.params["hidden_size"]), int(spec.params["intermediate_size"])
@@ -79,6 +81,8 @@ class SwiGLU:
 
 @register_part("ffn", "clamped_glu")
 class ClampedGLU:
+    PRODUCTS = ("w_gate_up", "w_down")
+
     @classmethod
     def tensor_specs(cls, spec: PartSpec) -> List[TensorSpec]:
         return SwiGLU.tensor_specs(spec)
@@ -159,6 +163,8 @@ class RoutedExperts:
 
 @register_part("ffn", "polynorm")
 class PolyNormFFN:
+    PRODUCTS = ("w_up", "w_down")
+
     @classmethod
     def tensor_specs(cls, spec: PartSpec) -> List[TensorSpec]:
         hidden, inter = int(spec.params["hidden_size"]), int(spec.params["intermediate_size"])
@@ -179,6 +185,8 @@ class PolyNormFFN:
 
 @register_part("ffn", "squared_relu")
 class SquaredReluFFN:
+    PRODUCTS = ("w_up", "w_down")
+
     @classmethod
     def tensor_specs(cls, spec: PartSpec) -> List[TensorSpec]:
         hidden, inter = int(spec.params["hidden_size"]), int(spec.params["intermediate_size"])

@@ -46,6 +46,7 @@ class PhasedMixer:
     """Base of the mixers in three phases.  ``state_base``: the index of this mixer's first state
     tensor in its cache entry (a pair moves the second mixer's behind the first's)."""
 
+    PRODUCTS = ("w_in", "w_out")
     inner_width: int = 0
     state_base: int = 0
 
@@ -74,6 +75,7 @@ class PhasedMixer:
 @register_part("mixer", "mixer_pair")
 class MixerPair:
     MEMBERS = ("left", "right")
+    PRODUCTS = ("w_in", "w_out")
 
     @classmethod
     def tensor_specs(cls, spec: PartSpec) -> List[TensorSpec]:

@@ -49,6 +49,8 @@ from .runtime import HostBatch, Runtime, StepContext
 
 @register_part("mixer", "latent_attention")
 class LatentAttention:
+    PRODUCTS = ("w_in", "w_uq", "w_up", "w_o")
+
     @staticmethod
     def _sizes(spec: PartSpec):
         p = spec.params

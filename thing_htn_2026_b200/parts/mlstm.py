@@ -36,6 +36,8 @@ PROJECTIONS = ("q", "k", "v", "g")     # the order of the fused product's column
 
 @register_part("mixer", "mlstm")
 class MatrixMemory:
+    PRODUCTS = ("w_in", "w_o")
+
     @staticmethod
     def _sizes(spec: PartSpec):
         p = spec.params

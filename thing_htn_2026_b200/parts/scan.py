@@ -33,6 +33,8 @@ from .runtime import Runtime, StepContext
 
 @register_part("mixer", "selective_scan")
 class SelectiveScan:
+    PRODUCTS = ("w_in", "w_o")
+
     @staticmethod
     def _sizes(spec: PartSpec):
         p = spec.params

@@ -33,6 +33,8 @@ from .runtime import Runtime, StepContext
 
 @register_part("mixer", "state_space")
 class StateSpaceMixer:
+    PRODUCTS = ("w_in", "w_o")
+
     @staticmethod
     def _sizes(spec: PartSpec):
         p = spec.params

@@ -36,6 +36,8 @@ BLENDS = WIDE + ("w",)
 
 @register_part("mixer", "time_mixing")
 class TimeMixing:
+    PRODUCTS = ("w_o",)
+
     @staticmethod
     def _sizes(spec: PartSpec):
         p = spec.params
