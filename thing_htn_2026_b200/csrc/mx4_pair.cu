@@ -21,7 +21,7 @@ namespace {
 enum Mode { kQuantized, kRows2, kRows6 };
 
 constexpr int kFeatures = 256;                             // of a pair
-constexpr int kEpilogueWarps = 16, kThreads = 64 + 32 * kEpilogueWarps;      // warp 0: TMA, warp 1: products and tensor memory
+constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;      // warp 0: TMA, warp 1: products and tensor memory
 
 template <int MODE>
 struct Shape {
@@ -187,103 +187,117 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
         return t;
     };
 
-    if (warp == 0 && lane == 0) {
-        // ---- TMA producer
+    if (warp == 0) {
+        // ---- the copies: a whole warp walks, one thread of it issues
+        const bool issues = elect_one();
+        const uint32_t leader_full = leader_addr(full);
         int it = 0;
-        for (int i = pair; i < a.n_tiles && !*give_up; i += n_pairs) {
+        for (int i = pair; i < a.n_tiles && !__any_sync(0xffffffffu, *give_up); i += n_pairs) {
             const Tile t = tile_of(i);
             const int b_row = t.row0 + rank * (t.columns / 2), a_row = t.feature + rank * 128;
             // (a last tile of fewer columns brings what a whole one does)
             constexpr uint32_t kBytes = (MODE == kQuantized ? S::kASmem : S::kASmem / 2) + S::kT * S::kBSmem + S::kScaleBytes;
             for (int kb = 0; kb < n_k && !a.skip_loads; ++kb, ++it) {
                 const int s = it % S::kStages;
-                if (!mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1)) {
-                    if (a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+                if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1))) {
+                    if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
                     *give_up = 1;
                     break;
                 }
                 unsigned char* dst = tiles + (size_t)s * S::kStageStride;
                 unsigned char* scales = dst + S::kASmem + S::kT * S::kBSmem;
-                const uint32_t bar = leader_addr(full + s);
+                const uint32_t bar = leader_full + s * (uint32_t)sizeof(uint64_t);
+                if (issues) {
                 if (rank == 0) mbar_expect_tx(full + s, 2 * kBytes);
                 load_box(dst, &map_w, bar, kb * 128, a_row);           // (bytes of codes, or entries)
                 load_box(dst + S::kASmem, &map_x, bar, kb * 128, b_row, 0);
                 load_box(scales, &map_w_scales, bar, 0, kb * S::kSteps, a_row >> 7, 0);
                 load_box(scales + S::kSteps * kMx4AtomBytes, &map_x_scales, bar, 0, kb * S::kSteps, t.row0 >> 7, 0);
+                }
+                __syncwarp();
             }
         }
     } else if (warp == 1 && rank == 0) {
-        // ---- the leading block issues the pair's products: a whole warp walks, one thread of it issues
+        // ---- the leading block issues the pair's products: a whole warp walks, one thread of it issues.  A stage's scales go to tensor memory ahead of
+        // the products of the stage before it, so that they are copied under those; two sets of columns take them in turn.
         const bool issues = elect_one();
-        int it = 0, local = 0;
-        for (int i = pair; i < a.n_tiles && !__any_sync(0xffffffffu, *give_up); i += n_pairs, ++local) {
+        auto bring_scales = [&](int s, uint32_t set) {           // W's, then x's, [term][piece of K][128 rows]
+            const uint32_t from = smem_addr(tiles + (size_t)s * S::kStageStride) + S::kASmem + S::kT * S::kBSmem;
+            const uint32_t to = tmem_base + S::kScaleCol + set * S::kScaleCols;
+#pragma unroll
+            for (int p = 0; p < S::kSteps; ++p) pair_scales(to + 4 * p, scale_desc(from + p * kMx4AtomBytes));
+#pragma unroll
+            for (int term = 0; term < S::kT; ++term)
+#pragma unroll
+                for (int j = 0; j < S::kAtoms; ++j)
+#pragma unroll
+                    for (int p = 0; p < S::kSteps; ++p)
+                        pair_scales(to + 4 * (S::kSteps + (term * S::kSteps + p) * S::kAtoms + j),
+                                    scale_desc(from + (S::kSteps + (term * S::kAtoms + j) * S::kSteps + p) * kMx4AtomBytes));
+        };
+        const int total = n_k * ((a.n_tiles - pair + n_pairs - 1) / n_pairs);
+        bool ok = true, brought = false;                         // whether this stage has come, and its scales are on their way
+        int it = 0, s = 0, local = 0;
+        uint32_t phase = 0;                                      // of the stage s
+        for (int i = pair; i < a.n_tiles && ok; i += n_pairs, ++local) {
             const Tile t = tile_of(i);
             const uint32_t instr = MODE == kQuantized ? scaled_instr(1, 1, kFeatures, t.columns) : scaled_instr(kE2M1, kE4M3, kFeatures, t.columns);
             const uint32_t first = (t.row0 & 127) >> 5;          // the tile's first column of scales
             const int buf = local % S::kBuffers;
-            // scales of a stage to its half of their columns: W's, then x's, [term][piece of K][128 rows]
-            auto bring_scales = [&](int it) {
-                const uint32_t from = smem_addr(tiles + (size_t)(it % S::kStages) * S::kStageStride) + S::kASmem + S::kT * S::kBSmem;
-                const uint32_t to = tmem_base + S::kScaleCol + (it & 1) * S::kScaleCols;
-#pragma unroll
-                for (int p = 0; p < S::kSteps; ++p) pair_scales(to + 4 * p, scale_desc(from + p * kMx4AtomBytes));
-#pragma unroll
-                for (int term = 0; term < S::kT; ++term)
-#pragma unroll
-                    for (int j = 0; j < S::kAtoms; ++j)
-#pragma unroll
-                        for (int p = 0; p < S::kSteps; ++p)
-                            pair_scales(to + 4 * (S::kSteps + (term * S::kSteps + p) * S::kAtoms + j),
-                                        scale_desc(from + (S::kSteps + (term * S::kAtoms + j) * S::kSteps + p) * kMx4AtomBytes));
-            };
-            bool ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1));
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1) && !*give_up);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + buf * S::kCols;
-            bool ahead = false;                                  // this stage has come, and its scales are on their way
             for (int kb = 0; kb < n_k && ok; ++kb, ++it) {
-                const int s = it % S::kStages;
-                if (!ahead) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(full + s, (it / S::kStages) & 1));
+                const int next = s + 1 == S::kStages ? 0 : s + 1;
+                const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
+                if (!brought) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full + s, phase));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (issues) bring_scales(it);
+                    if (issues) bring_scales(s, it & 1);
                 }
-                // the next stage's scales go first, if they are here: they are copied under this stage's products
-                ahead = kb + 1 < n_k && __all_sync(0xffffffffu, mbar_here(full + (it + 1) % S::kStages, ((it + 1) / S::kStages) & 1));
-                if (ahead) {
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (issues) bring_scales(it + 1);
+                // The next stage's scales ahead of this one's products: with rows in 4 bits, where issuing takes as long as the products, once they
+                // have come (8,192 rows of 4,096 by 24,576 outputs 323 us, 322 with the test and its second way); with fewer stages if they have.
+                brought = it + 1 < total;
+                if (brought && MODE == kQuantized) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full + next, next_phase));
+                    if (!ok) break;
+                } else if (brought) {
+                    brought = __all_sync(0xffffffffu, mbar_here(full + next, next_phase));
                 }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride);
                 const uint32_t w_col = tmem_base + S::kScaleCol + (it & 1) * S::kScaleCols, x_col = w_col + 4 * S::kSteps + first;
                 const uint64_t a_desc = smem_desc(at);
                 if (issues) {
+                    if (brought) bring_scales(next, (it + 1) & 1);
 #pragma unroll
-                for (int term = 0; term < S::kT; ++term) {
-                    const uint64_t b_desc = smem_desc(at + S::kASmem + term * S::kBSmem);
+                    for (int term = 0; term < S::kT; ++term) {
+                        const uint64_t b_desc = smem_desc(at + S::kASmem + term * S::kBSmem);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {          // 32 bytes further along K: + 2 in the address field
-                        if constexpr (MODE == kQuantized) {        // 64 entries, two of a piece's four scales
-                            if (k >= 2 && kb * 2 + 1 >= a.atoms) break;
-                            pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, (k & 1) * 2), w_col + 4 * (k >> 1),
-                                           x_col + (k >> 1) * S::kAtoms * 4, (kb | k) != 0);
-                        } else {                                   // 32 entries, one scale
-                            pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, k), w_col, x_col + term * S::kAtoms * 4,
-                                           (kb | k | term) != 0);
+                        for (int k = 0; k < 4; ++k) {      // 32 bytes further along K: + 2 in the address field
+                            if constexpr (MODE == kQuantized) {    // 64 entries, two of a piece's four scales
+                                if (k >= 2 && kb * 2 + 1 >= a.atoms) break;
+                                pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, (k & 1) * 2), w_col + 4 * (k >> 1),
+                                               x_col + (k >> 1) * S::kAtoms * 4, (kb | k) != 0);
+                            } else {                               // 32 entries, one scale
+                                pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, k), w_col,
+                                               x_col + term * S::kAtoms * 4, (kb | k | term) != 0);
+                            }
                         }
                     }
-                }
-                pair_commit(empty + s);                    // the stage is free in both blocks when these products are done
+                    pair_commit(empty + s);                // the stage is free in both blocks when these products are done
                 }
                 __syncwarp();
+                s = next;
+                phase = next_phase;
             }
-            if (ok) {
-                if (issues) pair_commit(acc_full + buf);
-            } else {                                       // (the warps that wait for this accumulator, in both blocks, give up by themselves)
-                if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
-                *give_up = 1;
-            }
+            if (ok && issues) pair_commit(acc_full + buf);
             __syncwarp();
+        }
+        if (!ok) {                                         // (the warps that wait for an accumulator, in both blocks, give up by themselves)
+            if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);
+            *give_up = 1;
         }
     } else if (warp >= 2) {
         // ---- epilogue: a warp reads tensor-memory lanes 32 * (warp % 4) .. + 31 (= features), every fourth chunk of 32 columns (= rows)

@@ -145,82 +145,87 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     if (n_ranks > 1) cluster_arrive();         // this block has begun: the others may reach into it
 
     if (warp == 0) {
-        // ---- the copies
-        if (elect_one()) {
-            auto load_x = [&](int s, int c) {
-                if constexpr (!S::kConverts) {
-                    unsigned char* dst = tiles + (size_t)s * S::kStageStride;
-                    tma_load_2d(dst + kWSmem, &map_x, full + s, c * BK, 0);
+        // ---- the copies: the whole warp walks, one thread of it issues
+        const bool issues = elect_one();
+        auto load_x = [&](int s, int c) {
+            if constexpr (!S::kConverts) {
+                unsigned char* dst = tiles + (size_t)s * S::kStageStride;
+                tma_load_2d(dst + kWSmem, &map_x, full + s, c * BK, 0);
 #pragma unroll
-                    for (int j = 0; j < S::kXAtoms; ++j)
-                        bulk_load(dst + kWSmem + S::kXSmem + (1 + j) * kMx4AtomBytes, a.x_scales + ((long long)j * a.chunks + c) * kMx4AtomBytes,
-                                  kMx4AtomBytes, full + s);
-                }
-            };
-            pdl_wait();
+                for (int j = 0; j < S::kXAtoms; ++j)
+                    bulk_load(dst + kWSmem + S::kXSmem + (1 + j) * kMx4AtomBytes, a.x_scales + ((long long)j * a.chunks + c) * kMx4AtomBytes,
+                              kMx4AtomBytes, full + s);
+            }
+        };
+        pdl_wait();
+        if (issues)
             for (int i = 0; i < early; ++i) load_x(i, c0 + i);
-            int it = early;
-            for (int tile = first_tile, i0 = early; tile < a.n_tiles && !a.skip_loads && !*give_up; tile += step, i0 = 0) {
-                for (int i = i0; i < n; ++i, ++it) {
-                    const int s = it % S::kStages;
-                    if (!mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1)) {
-                        give_up_at();
-                        break;
-                    }
+        __syncwarp();
+        int it = early;
+        bool ok = !a.skip_loads;
+        for (int tile = first_tile, i0 = early; tile < a.n_tiles && ok; tile += step, i0 = 0) {
+            for (int i = i0; i < n; ++i, ++it) {
+                const int s = it % S::kStages;
+                ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1) && !*give_up);
+                if (!ok) break;
+                if (issues) {
                     load_w(s, tile, c0 + i);
                     load_x(s, c0 + i);
                 }
+                __syncwarp();
             }
         }
+        if (!ok && !a.skip_loads && lane == 0) give_up_at();
         __syncwarp();
     } else if (warp == 1) {
-        // ---- the products: the whole warp walks, one thread of it issues
+        // ---- the products: the whole warp walks, one thread of it issues.  A stage's scales go to tensor memory ahead of the products of the stage
+        // before it, so that they are copied under those; two sets of columns take them in turn.
         const bool issues = elect_one();
-        int it = 0, local = 0;
-        for (int tile = first_tile; tile < a.n_tiles && !__any_sync(0xffffffffu, *give_up); tile += step, ++local) {
-            const int buf = local & 1;
-            auto bring_scales = [&](int it) {
-                const uint32_t from = smem_addr(tiles + (size_t)(it % S::kStages) * S::kStageStride) + kWSmem + S::kXSmem;
-                const uint32_t to = tmem_base + 2 * S::NX + (it & 1) * S::kScaleCols;
+        auto bring_scales = [&](int s, uint32_t set) {
+            const uint32_t from = smem_addr(tiles + (size_t)s * S::kStageStride) + kWSmem + S::kXSmem;
 #pragma unroll
-                for (int j = 0; j < 1 + S::kXAtoms; ++j) scales_to_tmem(to + 4 * j, scale_desc(from + j * kMx4AtomBytes));
-            };
-            bool ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local >> 1) & 1) ^ 1));
+            for (int j = 0; j < 1 + S::kXAtoms; ++j)
+                scales_to_tmem(tmem_base + 2 * S::NX + set * S::kScaleCols + 4 * j, scale_desc(from + j * kMx4AtomBytes));
+        };
+        const int total = n * ((a.n_tiles - first_tile + step - 1) / step);
+        bool ok = true, brought = false;       // whether this stage has come, and its scales are on their way
+        int it = 0, s = 0, local = 0;
+        uint32_t phase = 0;                    // of the stage s
+        for (int tile = first_tile; tile < a.n_tiles && ok; tile += step, ++local) {
+            const int buf = local & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local >> 1) & 1) ^ 1) && !*give_up);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + buf * S::NX;
-            bool ahead = false;                // this stage has come, and its scales are on their way
             for (int i = 0; i < n && ok; ++i, ++it) {
-                const int s = it % S::kStages;
-                if (!ahead) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(full + s, (it / S::kStages) & 1));
+                const int next = s + 1 == S::kStages ? 0 : s + 1;
+                const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
+                if (!brought) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full + s, phase));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (issues) bring_scales(it);
+                    if (issues) bring_scales(s, it & 1);
                 }
-                // the next stage's scales go first, if they are here: they are copied under this stage's products
-                ahead = i + 1 < n && __all_sync(0xffffffffu, mbar_here(full + (it + 1) % S::kStages, ((it + 1) / S::kStages) & 1));
-                if (ahead) {
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (issues) bring_scales(it + 1);
-                }
+                brought = it + 1 < total && __all_sync(0xffffffffu, mbar_here(full + next, next_phase));
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride);
                 const uint32_t w_col = tmem_base + 2 * S::NX + (it & 1) * S::kScaleCols;
                 const uint64_t w_desc = smem_desc(at), x_desc = smem_desc(at + kWSmem);
                 if (issues) {
+                    if (brought) bring_scales(next, (it + 1) & 1);
 #pragma unroll
                     for (int k = 0; k < BK / UMMA_K; ++k)  // 32 bytes further along K: + 2 in the address field
                         mma_scaled(tmem_d, w_desc + 2 * k, x_desc + 2 * k, with_scale_byte(S::kInstr, k), w_col, w_col + 4, (i | k) != 0);
                     umma_commit(empty + s);
                 }
                 __syncwarp();
+                s = next;
+                phase = next_phase;
             }
-            if (ok) {
-                if (issues) umma_commit(acc_full + buf);
-            } else if (lane == 0) {            // (the warps that wait for this accumulator give up by themselves)
-                give_up_at();
-            }
+            if (ok && issues) umma_commit(acc_full + buf);
             __syncwarp();
         }
+        if (!ok && lane == 0) give_up_at();    // (the warps that wait for an accumulator give up by themselves)
+        __syncwarp();
     } else if (warp >= 6) {
         if constexpr (S::kConverts) {
             // ---- rows of x to terms: chunk by chunk in turn among four warps, a half warp a row, a thread eight columns, the rows of a warp's next
