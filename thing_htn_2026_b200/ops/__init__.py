@@ -1047,9 +1047,16 @@ class Mx4:
         return at, at + self.code_bytes
 
 
-def _on_current_device(t: torch.Tensor, what: str) -> None:
-    if t.get_device() != torch.cuda.current_device():
+# (The checks below are written out rather than called one by one: a product of a few rows takes the device 4 to 10 us, about what its call takes
+# the host.)
+
+
+def _mx4_stream_for(t: torch.Tensor, what: str) -> int:
+    """The current stream, which must be one of the tensor's device."""
+    device = t.get_device()
+    if device != torch._C._cuda_getDevice():
         raise KernelError(f"{what}: tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def quantize_mx4(x: torch.Tensor) -> Mx4:
@@ -1057,15 +1064,17 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
     ``2^(floor(log2 max|x|) - 2)``, at least 2^-127, and an entry becomes the nearest magnitude, of two equally near ones that with
     the even code; what lies above 6 scales becomes 6.  A block that holds an infinity or a NaN is not a number as a whole."""
     _need(x, "quantize_mx4 x")
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise KernelError(f"quantize_mx4: a matrix with columns, please, not {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise KernelError(f"quantize_mx4: a matrix with columns, please, not {tuple(shape)}")
     code = _code(x, "quantize_mx4 x")
-    _on_current_device(x, "quantize_mx4 x")
-    rows, columns = x.shape
-    out = Mx4.empty(x, rows, columns)
-    codes, scales = out._pointers()
-    _call("thn_mx4_quantize", codes, scales, x.data_ptr(), rows, columns, code, _stream())
-    return out
+    stream = _mx4_stream_for(x, "quantize_mx4 x")
+    rows, columns = shape
+    atoms = (columns + 127) // 128
+    data = x.new_empty(((rows * 64 + (rows + 127) // 128 * 512) * atoms,), dtype=torch.uint8)
+    at = data.data_ptr()
+    _call("thn_mx4_quantize", at, at + rows * atoms * 64, x.data_ptr(), rows, columns, code, stream)
+    return Mx4(data, rows, columns)
 
 
 def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> Mx4:
@@ -1074,26 +1083,28 @@ def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> M
     _need(codes, "mx4_from_parts codes", torch.uint8)
     _need(scales, "mx4_from_parts scales", torch.uint8)
     columns = int(columns)
-    rows = codes.shape[0]
-    if columns < 1 or codes.dim() != 2 or tuple(codes.shape) != (rows, -(-columns // 2)) or tuple(scales.shape) != (rows, -(-columns // 32)):
+    rows = codes.shape[0] if codes.dim() else 0
+    if columns < 1 or tuple(codes.shape) != (rows, -(-columns // 2)) or tuple(scales.shape) != (rows, -(-columns // 32)):
         raise KernelError(f"mx4_from_parts: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} for {columns} columns")
     if scales.device != codes.device:
         raise KernelError(f"mx4_from_parts: codes on {codes.device}, scales on {scales.device}")
-    _on_current_device(codes, "mx4_from_parts codes")
+    stream = _mx4_stream_for(codes, "mx4_from_parts codes")
     out = Mx4.empty(codes, rows, columns)
     to_codes, to_scales = out._pointers()
-    _call("thn_mx4_arrange", to_codes, to_scales, codes.data_ptr(), scales.data_ptr(), rows, columns, _stream())
+    _call("thn_mx4_arrange", to_codes, to_scales, codes.data_ptr(), scales.data_ptr(), rows, columns, stream)
     return out
 
 
 def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The numbers ``[rows, columns]`` that ``q`` stands for, in float32 or bfloat16; both hold them exactly."""
-    if dtype not in DTYPE_CODE:
+    code = DTYPE_CODE.get(dtype)
+    if code is None:
         raise KernelError(f"dequantize_mx4: dtype {dtype} is not supported (float32 or bfloat16)")
-    _on_current_device(q.data, "dequantize_mx4 q")
-    out = q.data.new_empty(q.shape, dtype=dtype)
-    codes, scales = q._pointers()
-    _call("thn_mx4_dequantize", out.data_ptr(), codes, scales, q.rows, q.columns, DTYPE_CODE[dtype], _stream())
+    data = q.data
+    stream = _mx4_stream_for(data, "dequantize_mx4 q")
+    out = data.new_empty((q.rows, q.columns), dtype=dtype)
+    at = data.data_ptr()
+    _call("thn_mx4_dequantize", out.data_ptr(), at, at + q.code_bytes, q.rows, q.columns, code, stream)
     return out
 
 
@@ -1115,40 +1126,51 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     float32).  ``x`` is a tensor in bfloat16 or float32, which is multiplied as it is and whose type is the default
     ``out_dtype``, or an :class:`Mx4` (default: bfloat16).  A row of ``x`` that holds an infinity or a NaN comes out as NaN, and so does the
     column of a weight row that does.  ``err``: the step's device error word for the kernel's bounded waits."""
-    if isinstance(x, Mx4):
-        kind, data, (at, x_scales) = 2, x.data, x._pointers()
-        m, k = x.rows, x.columns
+    if x.__class__ is Mx4:
+        kind, data, m, k = 2, x.data, x.rows, x.columns
+        at = data.data_ptr()
+        x_scales = at + x.code_bytes
+        if out_dtype is None:
+            out_dtype = torch.bfloat16
     else:
         _need(x, "linear_mx4 x")
-        if x.dim() != 2:
-            raise KernelError(f"linear_mx4: x has {x.dim()} dimensions, not 2")
-        kind, data, at, x_scales = _code(x, "linear_mx4 x"), x, x.data_ptr(), None
-        m, k = x.shape
-    n = weight.rows
+        kind = _code(x, "linear_mx4 x")
+        shape = x.shape
+        if len(shape) != 2:
+            raise KernelError(f"linear_mx4: x has {len(shape)} dimensions, not 2")
+        data, at, x_scales, (m, k) = x, x.data_ptr(), None, shape
+        if out_dtype is None:
+            out_dtype = x.dtype
+    stream = _mx4_stream_for(data, "linear_mx4 x")
+    held, n = weight.data, weight.rows
     if k != weight.columns:
         raise KernelError(f"linear_mx4: shapes x {(m, k)}, weight {weight.shape}")
-    if data.get_device() != weight.data.get_device():
+    if held.get_device() != data.get_device():
         raise KernelError(f"linear_mx4: x on {data.device}, weight on {weight.device}")
-    _on_current_device(data, "linear_mx4 x")
-    if out_dtype is None:
-        out_dtype = torch.bfloat16 if kind == 2 else x.dtype
-    if out_dtype not in DTYPE_CODE:
+    out_code = DTYPE_CODE.get(out_dtype)
+    if out_code is None:
         raise KernelError(f"linear_mx4: out_dtype {out_dtype} is not supported (float32 or bfloat16)")
-    bias_code = 0
+    bias_at, bias_code = None, 0
     if bias is not None:
         _need(bias, "linear_mx4 bias")
         if tuple(bias.shape) != (n,) or bias.get_device() != data.get_device():
             raise KernelError(f"linear_mx4: a bias {tuple(bias.shape)} on {bias.device} for {n} outputs on {data.device}")
-        bias_code = _code(bias, "linear_mx4 bias")
+        bias_at, bias_code = bias.data_ptr(), _code(bias, "linear_mx4 bias")
+    if err is not None:
+        _need(err, "linear_mx4 err", torch.int32)
     out = data.new_empty((m, n), dtype=out_dtype)
     if m == 0 or n == 0:
         return out
-    codes, scales = weight._pointers()
+    codes = held.data_ptr()
     few = m <= (32 if kind == 0 else 64)
-    size = 0 if kind == 2 else _mx4_terms_need("thn_mx4_stream_scratch" if few else "thn_mx4_pair_scratch", kind, m, k)
-    terms = data.new_empty(size, dtype=torch.uint8) if size else None
-    _call("thn_mx4_stream" if few else "thn_mx4_pair", out.data_ptr(), DTYPE_CODE[out_dtype], at, x_scales, kind, codes, scales, _ptr(bias), bias_code,
-          _ptr(terms), size, m, n, k, 0, _ptr(err), _stream())
+    terms_at, size = None, 0
+    if kind != 2:
+        size = _mx4_terms_need("thn_mx4_stream_scratch" if few else "thn_mx4_pair_scratch", kind, m, k)
+        if size:
+            terms = data.new_empty((size,), dtype=torch.uint8)
+            terms_at = terms.data_ptr()
+    _call("thn_mx4_stream" if few else "thn_mx4_pair", out.data_ptr(), out_code, at, x_scales, kind, codes, codes + weight.code_bytes, bias_at, bias_code,
+          terms_at, size, m, n, k, 0, None if err is None else err.data_ptr(), stream)
     return out
 
 
