@@ -296,7 +296,7 @@ def test_a_wait_that_runs_out_is_reported(m, entry, quantized):
     out = torch.zeros((m, 300), dtype=torch.float32, device="cuda")
     err = ops.new_error_word("cuda")
     data, scales, kind = (q.codes, q.scales, 2) if quantized else (x, None, 1)
-    room = torch.empty(ops._mx4_terms_need(entry + "_scratch", kind, m, 640) or 16, dtype=torch.uint8, device="cuda")
+    room = torch.empty(ops._mx4_terms_need(entry + "_scratch", kind, m, 300, 640) or 16, dtype=torch.uint8, device="cuda")
     ops._call(entry, out.data_ptr(), 0, data.data_ptr(), ops._ptr(scales), kind, weight.codes.data_ptr(), weight.scales.data_ptr(), None, 0,
               room.data_ptr(), room.numel(), m, 300, 640, 1, err.data_ptr(), ops._stream())
     with pytest.raises(ops.KernelError, match="gave up"):

@@ -10,29 +10,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Eight neighbouring entries of a row as float32; what lies behind the last column is zero.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, long long c, long long columns, bool vector, float (&v)[8]) {
-    if (vector && c + 8 <= columns) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(row + c);
-            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        } else {
-            const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < columns ? to_f32<T>(row[c + i]) : 0.f;
-    }
-}
-
 // Two float32 to their codes, the first in the low half of the byte (nearest, ties to the even code, at most 6).
 __device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
     uint32_t r;
@@ -40,75 +17,184 @@ __device__ __forceinline__ uint32_t codes_of(float lo, float hi) {
     return r;
 }
 
-// A thread takes eight entries, four threads a block, sixteen the columns of four scale bytes.
+// Eight neighbouring entries of a row as they lie in memory; what lies behind the last column is zero.  vector: the row is whole aligned 16-byte
+// pieces.  top(): the largest magnitude as the bits of a float32; codes(b): the codes under the scale byte b.
+template <typename T>
+struct Piece;
+
+template <>
+struct Piece<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* row, int c, int columns, bool vector) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+            if (vector) {
+                const float4 q = c + h < columns ? *reinterpret_cast<const float4*>(row + c + h) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[h] = q.x; v[h + 1] = q.y; v[h + 2] = q.z; v[h + 3] = q.w;
+            } else {
+#pragma unroll
+                for (int i = h; i < h + 4; ++i) v[i] = c + i < columns ? row[c + i] : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        return m;
+    }
+    __device__ __forceinline__ uint32_t codes(uint32_t b) const {
+        const float factor = __uint_as_float((254 - min(b, 253u)) << 23);
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) word |= codes_of(v[2 * i] * factor, v[2 * i + 1] * factor) << (8 * i);
+        return word;
+    }
+};
+
+template <>
+struct Piece<__nv_bfloat16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const __nv_bfloat16* row, int c, int columns, bool vector) {
+        if (vector) {
+            const uint4 q = c < columns ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+            w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+        } else {
+            const uint16_t* bits = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[i] = (c + 2 * i < columns ? bits[c + 2 * i] : 0u) | (c + 2 * i + 1 < columns ? (uint32_t)bits[c + 2 * i + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        return max(m << 16, m & 0xffff0000u);
+    }
+    __device__ __forceinline__ uint32_t codes(uint32_t b) const {
+        const uint32_t factor = (254 - min(b, 253u)) << 7;
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t x;
+            asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(x) : "r"(w[i]), "r"(factor | factor << 16));      // exact, but for what is nothing beside 1/4
+            word |= codes_of(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) << (8 * i);
+        }
+        return word;
+    }
+};
+
+// Division of numbers below 2^31 by a divisor that the host knows: n / d = (hi(n m) + n) >> l with 2^(l-1) < d <= 2^l and
+// m = floor(2^32 (2^l - d) / d) + 1.
+struct Divisor {
+    uint32_t d, m, l;
+    explicit Divisor(uint32_t divisor) : d(divisor), l(0) {
+        while ((1ull << l) < d) ++l;
+        m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(n, m) + n) >> l; }
+};
+
+// Row and piece of a unit, and of those kThreads further on.
+struct Place {
+    uint32_t row, piece;
+    __device__ __forceinline__ Place(uint32_t unit, const Divisor& pieces) : row(pieces.of(unit)), piece(unit - row * pieces.d) {}
+    __device__ __forceinline__ void step(const Divisor& pieces) {
+        piece += kThreads;
+        if (pieces.d >= kThreads) {
+            if (piece >= pieces.d) {
+                piece -= pieces.d;
+                ++row;
+            }
+        } else {
+            const uint32_t more = pieces.of(piece);
+            row += more;
+            piece -= more * pieces.d;
+        }
+    }
+};
+
+// Pieces of eight entries: a thread takes kAhead of them, kThreads apart, and asks for all of them before it works on the first.  Bound by the
+// memory: 2,048 rows of 9,728 bfloat16 entries, which lie in the L2 cache or not.  Four threads have a block's entries, sixteen the columns of four
+// scale bytes.
+constexpr int kAhead = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                const T* __restrict__ x, long long rows, long long columns,
+                                                                const T* __restrict__ x, uint32_t units, Divisor pieces, long long columns,
                                                                 long long padded, bool vector) {
     pdl_launch_dependents();
     pdl_wait();
-    const long long pieces = padded / 8, unit = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const long long row = unit / pieces, piece = unit - row * pieces;
-    const bool there = row < rows;
-    float v[8];
-    if (there) {
-        load8(x + row * columns, piece * 8, columns, vector, v);
-    } else {
+    const uint32_t first = blockIdx.x * (uint32_t)(kThreads * kAhead) + threadIdx.x;
+    Piece<T> held[kAhead];
+    Place at(first, pieces);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    for (int a = 0; a < kAhead; ++a, at.step(pieces))
+        held[a].load(x + (long long)at.row * columns, (int)(at.piece * 8), first + a * kThreads < units ? (int)columns : 0, vector);
+    at = Place(first, pieces);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
+        uint32_t top = held[a].top();
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t field = top >> 23;
+        const uint32_t b = field == 255 ? 255 : field > 2 ? field - 2 : 0;
+        const uint32_t word = b == 255 ? 0 : held[a].codes(b);
+        // the sixteen threads' four scale bytes as one word
+        uint32_t four = b << (8 * ((threadIdx.x >> 2) & 3));
+        four |= __shfl_xor_sync(0xffffffffu, four, 4);
+        four |= __shfl_xor_sync(0xffffffffu, four, 8);
+        if (first + a * kThreads >= units) continue;
+        *reinterpret_cast<uint32_t*>(codes + (long long)at.row * (padded / 2) + at.piece * 4) = word;
+        if ((threadIdx.x & 15) == 0)
+            *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(at.row, at.piece / 16, padded / kMx4Atom)) = four;
     }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t field = top >> 23;
-    const uint32_t b = field == 255 ? 255 : field > 2 ? field - 2 : 0;
-    const float factor = __uint_as_float((254 - min(b, 253u)) << 23);
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) word |= codes_of(v[2 * i] * factor, v[2 * i + 1] * factor) << (8 * i);
-    if (b == 255) word = 0;
-    // the sixteen threads' four scale bytes as one word
-    uint32_t four = b << (8 * ((threadIdx.x >> 2) & 3));
-    four |= __shfl_xor_sync(0xffffffffu, four, 4);
-    four |= __shfl_xor_sync(0xffffffffu, four, 8);
-    if (!there) return;
-    *reinterpret_cast<uint32_t*>(codes + row * (padded / 2) + piece * 4) = word;
-    if ((threadIdx.x & 15) == 0)
-        *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, piece / 16, padded / kMx4Atom)) = four;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes,
-                                                                  const uint8_t* __restrict__ scales, long long rows,
+                                                                  const uint8_t* __restrict__ scales, uint32_t units, Divisor pieces,
                                                                   long long columns, long long padded, bool vector) {
     pdl_launch_dependents();
     pdl_wait();
-    const long long pieces = (columns + 7) / 8, unit = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const long long row = unit / pieces, c = (unit - row * pieces) * 8;
-    if (row >= rows) return;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + row * (padded / 2) + c / 2);
-    const float s = mx4_scale(scales[mx4_scale_at(row, c / kMx4Atom, padded / kMx4Atom) + (c % kMx4Atom) / kMx4Block]);
-    T* dst = out + row * columns + c;
-    float v[8];
+    const uint32_t first = blockIdx.x * (uint32_t)(kThreads * kAhead) + threadIdx.x;
+    uint32_t words[kAhead];
+    uint8_t bytes[kAhead];
+    Place at(first, pieces);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = mx4_value(word >> (4 * i)) * s;
-    if (vector && c + 8 <= columns) {
-        if constexpr (sizeof(T) == 2) {
-            uint4 packed;
-            __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&packed);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<uint4*>(dst) = packed;
-        } else {
-            *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
+        if (first + a * kThreads < units) {
+            words[a] = *reinterpret_cast<const uint32_t*>(codes + (long long)at.row * (padded / 2) + at.piece * 4);
+            bytes[a] = scales[mx4_scale_at(at.row, at.piece / 16, padded / kMx4Atom) + (at.piece % 16) / 4];
         }
-    } else {
+    }
+    at = Place(first, pieces);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < columns) dst[i] = from_f32<T>(v[i]);
+    for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
+        if (first + a * kThreads >= units) break;
+        const long long c = (long long)at.piece * 8;
+        const float s = mx4_scale(bytes[a]);
+        T* dst = out + (long long)at.row * columns + c;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mx4_value(words[a] >> (4 * i)) * s;
+        if (vector && c + 8 <= columns) {
+            if constexpr (sizeof(T) == 2) {
+                uint4 packed;
+                __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&packed);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                *reinterpret_cast<uint4*>(dst) = packed;
+            } else {
+                *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < columns) dst[i] = from_f32<T>(v[i]);
+        }
     }
 }
 
@@ -143,13 +229,48 @@ __global__ void __launch_bounds__(kThreads) mx4_arrange_kernel(uint8_t* __restri
 }
 
 int refuse_sizes(const char* what, long long rows, long long columns) {
-    THN_CHECK_ARG(rows >= 0 && columns >= 1 && columns <= (1 << 30), "%s: %lld rows of %lld entries", what, rows, columns);
-    THN_UNSUPPORTED_IF(rows * (mx4_padded(columns) / 8) > (long long)0x7fffffff * kThreads, "%s: %lld rows of %lld entries are too many",
-                       what, rows, columns);
+    THN_CHECK_ARG(rows >= 0 && columns >= 1 && columns <= (1 << 26), "%s: %lld rows of %lld entries", what, rows, columns);
+    THN_UNSUPPORTED_IF(rows > 0x7fffffff, "%s: %lld rows of %lld entries are too many", what, rows, columns);
     return THN_OK;
 }
 
 unsigned blocks_for(long long units) { return (unsigned)((units + kThreads - 1) / kThreads); }
+
+// Rows in steps of whole pieces of scales, so that a launch has fewer than 2^31 units: go(first row, rows).
+template <typename Go>
+int in_steps(long long rows, long long units_a_row, Go go) {
+    long long most = 0x7ffffff0 / units_a_row - kThreads * kAhead;
+    most = most < 128 ? 128 : most / 128 * 128;
+    for (long long row = 0; row < rows; row += most) {
+        const int status = go(row, rows - row < most ? rows - row : most);
+        if (status != THN_OK) return status;
+    }
+    return THN_OK;
+}
+
+template <typename T>
+int quantize(uint8_t* codes, uint8_t* scales, const T* x, long long rows, long long columns, cudaStream_t stream) {
+    const long long padded = mx4_padded(columns), pieces = padded / 8;
+    const bool vector = ((uintptr_t)x & 15) == 0 && columns % (16 / sizeof(T)) == 0;
+    return in_steps(rows, pieces, [&](long long row, long long n) {
+        thn_launch(mx4_quantize_kernel<T>, (unsigned)((n * pieces + kThreads * kAhead - 1) / (kThreads * kAhead)), kThreads, 0, stream, codes + row * (padded / 2),
+                   scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, x + row * columns, (uint32_t)(n * pieces), Divisor((uint32_t)pieces), columns,
+                   padded, vector);
+        return thn_launch_status("mx4_quantize");
+    });
+}
+
+template <typename T>
+int dequantize(T* out, const uint8_t* codes, const uint8_t* scales, long long rows, long long columns, cudaStream_t stream) {
+    const long long padded = mx4_padded(columns), pieces = (columns + 7) / 8;
+    const bool vector = ((uintptr_t)out & 15) == 0 && columns % (16 / sizeof(T)) == 0;
+    return in_steps(rows, pieces, [&](long long row, long long n) {
+        thn_launch(mx4_dequantize_kernel<T>, (unsigned)((n * pieces + kThreads * kAhead - 1) / (kThreads * kAhead)), kThreads, 0, stream, out + row * columns,
+                   codes + row * (padded / 2), scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, (uint32_t)(n * pieces), Divisor((uint32_t)pieces),
+                   columns, padded, vector);
+        return thn_launch_status("mx4_dequantize");
+    });
+}
 
 }  // namespace
 
@@ -159,16 +280,8 @@ THN_API int thn_mx4_quantize(void* codes, void* scales, const void* x, long long
     if (status != THN_OK) return status;
     THN_CHECK_ARG(dtype == THN_F32 || dtype == THN_BF16, "mx4_quantize: unknown dtype %d", dtype);
     if (rows == 0) return THN_OK;
-    const long long padded = mx4_padded(columns);
-    const unsigned blocks = blocks_for(rows * (padded / 8));
-    const bool vector = ((uintptr_t)x & 15) == 0 && columns % (dtype == THN_F32 ? 4 : 8) == 0;
-    if (dtype == THN_F32)
-        thn_launch(mx4_quantize_kernel<float>, blocks, kThreads, 0, stream, (uint8_t*)codes, (uint8_t*)scales, (const float*)x, rows, columns,
-                   padded, vector);
-    else
-        thn_launch(mx4_quantize_kernel<__nv_bfloat16>, blocks, kThreads, 0, stream, (uint8_t*)codes, (uint8_t*)scales,
-                   (const __nv_bfloat16*)x, rows, columns, padded, vector);
-    return thn_launch_status("mx4_quantize");
+    return dtype == THN_F32 ? quantize((uint8_t*)codes, (uint8_t*)scales, (const float*)x, rows, columns, stream)
+                            : quantize((uint8_t*)codes, (uint8_t*)scales, (const __nv_bfloat16*)x, rows, columns, stream);
 }
 
 // out [rows, columns] of dtype: what codes and scales stand for.
@@ -178,16 +291,8 @@ THN_API int thn_mx4_dequantize(void* out, const void* codes, const void* scales,
     if (status != THN_OK) return status;
     THN_CHECK_ARG(dtype == THN_F32 || dtype == THN_BF16, "mx4_dequantize: unknown dtype %d", dtype);
     if (rows == 0) return THN_OK;
-    const long long padded = mx4_padded(columns);
-    const unsigned blocks = blocks_for(rows * ((columns + 7) / 8));
-    const bool vector = ((uintptr_t)out & 15) == 0 && columns % (dtype == THN_F32 ? 4 : 8) == 0;
-    if (dtype == THN_F32)
-        thn_launch(mx4_dequantize_kernel<float>, blocks, kThreads, 0, stream, (float*)out, (const uint8_t*)codes, (const uint8_t*)scales,
-                   rows, columns, padded, vector);
-    else
-        thn_launch(mx4_dequantize_kernel<__nv_bfloat16>, blocks, kThreads, 0, stream, (__nv_bfloat16*)out, (const uint8_t*)codes,
-                   (const uint8_t*)scales, rows, columns, padded, vector);
-    return thn_launch_status("mx4_dequantize");
+    return dtype == THN_F32 ? dequantize((float*)out, (const uint8_t*)codes, (const uint8_t*)scales, rows, columns, stream)
+                            : dequantize((__nv_bfloat16*)out, (const uint8_t*)codes, (const uint8_t*)scales, rows, columns, stream);
 }
 
 // stored [rows, ceil(columns / 2)] and stored_scales [rows, ceil(columns / 32)], both row by row -> codes and scales.
@@ -197,6 +302,7 @@ THN_API int thn_mx4_arrange(void* codes, void* scales, const void* stored, const
     if (status != THN_OK) return status;
     if (rows == 0) return THN_OK;
     const long long padded = mx4_padded(columns);
+    THN_UNSUPPORTED_IF(rows * (padded / kMx4Atom) > (long long)0x7fffffff * kThreads, "mx4_arrange: %lld rows of %lld entries are too many", rows, columns);
     thn_launch(mx4_arrange_kernel, blocks_for(rows * (padded / kMx4Atom)), kThreads, 0, stream, (uint8_t*)codes, (uint8_t*)scales,
                (const uint8_t*)stored, (const uint8_t*)stored_scales, rows, columns, padded);
     return thn_launch_status("mx4_arrange");

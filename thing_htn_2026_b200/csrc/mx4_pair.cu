@@ -432,7 +432,8 @@ static long long terms_needed(int x_type, int M, int K) {
     return atoms * 128 * padded + atoms * (padded / kMx4Atom) * kMx4AtomBytes;
 }
 
-THN_API int thn_mx4_pair_scratch(int x_type, int M, int K, long long* bytes) {
+THN_API int thn_mx4_pair_scratch(int x_type, int M, int N, int K, long long* bytes) {
+    (void)N;
     *bytes = terms_needed(x_type, M, K);
     return THN_OK;
 }

@@ -4,7 +4,7 @@
 //    narrow one.  W comes by TMA, which spreads its 4-bit codes over 8-bit containers as it copies, so no thread touches a weight;
 //    its scales come as 512 bytes for 128 rows and 128 columns, in the order of tensor memory, and go there by tcgen05.cp.
 //  * Rows in bfloat16 or float32 become two or six terms of 8-bit floats (mx4_tcgen05.cuh), a column of the narrow operand each;
-//    their sums are added at the end.  Up to converted_rows this happens in the kernel, a warp for 128 columns of
+//    their sums are added at the end.  Up to kConverted rows this happens in the kernel, a warp for 128 columns of
 //    them, beside the copies of W; more rows are prepared by a kernel of their own (mx4_terms_kernel), since every block would
 //    do it again, and come by TMA.  Rows in 4 bits are brought as W is.
 //  * Few tiles of 128 outputs: each is cut along K among the blocks of a cluster, whose partial sums meet in distributed shared
@@ -24,9 +24,13 @@ constexpr int BW = 128, BK = 128, UMMA_K = 32;
 constexpr uint32_t kWSmem = BW * BK, kWBytes = kWSmem / 2;     // in shared memory; as the barrier counts
 constexpr int kMaxStages = 12;
 constexpr int kMaxCluster = 8;
-// Rows that the kernel itself brings to terms, of a type.  (Float32 rows have six terms to compute: eight of them by 19,456 x 2,560 took 26 us so,
-// and 20 us prepared.)
-constexpr int converted_rows(int x_type) { return x_type == THN_F32 ? 4 : 8; }
+// Rows that the kernel itself brings to terms.  Five to eight float32 rows, with six terms to compute, only by a weight of few pieces (four pieces of
+// K a block): by 19,456 x 2,560 eight of them took 26 us so and 13.7 us prepared, five by 1,333 x 1,000 4.6 us either way, a launch more.
+constexpr int kConverted = 8;
+constexpr long long kFewPieces = 4 * 296;
+inline bool converts(int x_type, int M, int N, int K) {
+    return M <= 4 || (M <= kConverted && (x_type != THN_F32 || (N + 127LL) / 128 * ((K + 127) / 128) <= kFewPieces));
+}
 
 // RT: the rows' type (float, __nv_bfloat16, or uint8_t: 4 bits); MR: rows the block has room for; PAIRS: how many pairs of rows the
 // kernel itself brings to terms (0: they come prepared, or in 4 bits)
@@ -497,14 +501,14 @@ int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K
 THN_API int thn_mx4_stream_rows(int x_type) { return x_type == THN_F32 ? 32 : 64; }
 
 // The bytes of `terms` that M rows of a type need.
-static long long terms_needed(int x_type, int M, int K) {
-    if (x_type == 2 || M <= converted_rows(x_type)) return 0;
+static long long terms_needed(int x_type, int M, int N, int K) {
+    if (x_type == 2 || converts(x_type, M, N, K)) return 0;
     const long long rows = (long long)(M <= 16 ? 16 : room_for(M)) * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
     return rows * padded + (rows + 127) / 128 * (padded / kMx4Atom) * kMx4AtomBytes;
 }
 
-THN_API int thn_mx4_stream_scratch(int x_type, int M, int K, long long* bytes) {
-    *bytes = terms_needed(x_type, M, K);
+THN_API int thn_mx4_stream_scratch(int x_type, int M, int N, int K, long long* bytes) {
+    *bytes = terms_needed(x_type, M, N, K);
     return THN_OK;
 }
 
@@ -521,8 +525,8 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     THN_UNSUPPORTED_IF(M < 1 || M > thn_mx4_stream_rows(x_type) || N < 1 || K < 1 || K > (1 << 24), "mx4_stream: M=%d N=%d K=%d not supported", M, N, K);
     THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 &&
                   (((uintptr_t)scales | (uintptr_t)x_scales | (uintptr_t)terms) & 15) == 0, "mx4_stream: codes must be 32-byte, scales and terms 16-byte aligned");
-    THN_CHECK_ARG(terms_bytes >= terms_needed(x_type, M, K), "mx4_stream: %lld bytes of scratch, %lld needed", terms_bytes,
-                  terms_needed(x_type, M, K));
+    THN_CHECK_ARG(terms_bytes >= terms_needed(x_type, M, N, K), "mx4_stream: %lld bytes of scratch, %lld needed", terms_bytes,
+                  terms_needed(x_type, M, N, K));
     const long long padded = mx4_padded(K);
     Args args = {};
     args.out = out;
@@ -544,6 +548,7 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
     if (x_type == THN_F32) {
         if (M <= 2) GO(float, 8, 1);
         if (M <= 4) GO(float, 8, 2);
+        if (converts(x_type, M, N, K)) GO(float, 8, 4);
         if (room <= 16) GO(float, 16);
         GO(float, 32);
     }

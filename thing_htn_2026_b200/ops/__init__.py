@@ -152,11 +152,11 @@ _SIGNATURES = {
     "thn_mx4_quantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_arrange": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p],
-    "thn_mx4_pair_scratch": [c_int, c_int, c_int, c_void_p],
+    "thn_mx4_pair_scratch": [c_int, c_int, c_int, c_int, c_void_p],
     "thn_mx4_pair": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                      c_int, c_void_p, c_void_p],
     "thn_mx4_stream_rows": [c_int],
-    "thn_mx4_stream_scratch": [c_int, c_int, c_int, c_void_p],
+    "thn_mx4_stream_scratch": [c_int, c_int, c_int, c_int, c_void_p],
     "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                        c_int, c_void_p, c_void_p],
     "thn_gemm_f32": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -1108,14 +1108,14 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
-_mx4_terms_needs: Dict[Tuple[str, int, int, int], int] = {}
+_mx4_terms_needs: Dict[Tuple[str, int, int, int, int], int] = {}
 
 
-def _mx4_terms_need(entry: str, kind: int, m: int, k: int) -> int:
-    key = (entry, kind, m, k)
+def _mx4_terms_need(entry: str, kind: int, m: int, n: int, k: int) -> int:
+    key = (entry, kind, m, n, k)
     if key not in _mx4_terms_needs:
         size = c_longlong(0)
-        getattr(lib(), entry)(kind, m, k, ctypes.byref(size))
+        getattr(lib(), entry)(kind, m, n, k, ctypes.byref(size))
         _mx4_terms_needs[key] = size.value
     return _mx4_terms_needs[key]
 
@@ -1165,7 +1165,7 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     few = m <= (32 if kind == 0 else 64)
     terms_at, size = None, 0
     if kind != 2:
-        size = _mx4_terms_need("thn_mx4_stream_scratch" if few else "thn_mx4_pair_scratch", kind, m, k)
+        size = _mx4_terms_need("thn_mx4_stream_scratch" if few else "thn_mx4_pair_scratch", kind, m, n, k)
         if size:
             terms = data.new_empty((size,), dtype=torch.uint8)
             terms_at = terms.data_ptr()
