@@ -45,16 +45,22 @@ struct Shape {
     static constexpr uint32_t kStageBytes = kWSmem + kXSmem + (1 + kXAtoms) * kMx4AtomBytes;
     static constexpr uint32_t kStageStride = (kStageBytes + 1023) / 1024 * 1024;
     static constexpr int kRecvFloats = (MR + kMaxCluster) * BW;      // [own row][sending block][output]
-    static constexpr size_t kFixed = kRecvFloats * 4 + 1024 /* alignment */ + 512 /* barriers */;
-    static constexpr size_t kBudget = 4 * kStageStride + kFixed <= 113 * 1024 ? 113 * 1024 : 226 * 1024;
-    static constexpr int kFit = (int)((kBudget - kFixed) / kStageStride);
-    static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
-    static_assert(kStages >= 4, "four warps bring rows to terms in turn: a warp must be within a round of the ring");
-    static constexpr size_t kSmemBytes = kStages * kStageStride + kFixed;
+    static constexpr size_t kFixed = 1024 /* alignment */ + 512 /* barriers */;
     static constexpr int kScaleCols = 4 + 4 * kXAtoms;               // of a stage; two stages' in turn, behind the two accumulators
     static constexpr int kUsedCols = 2 * NX + 2 * kScaleCols;
     static constexpr int kTmemCols = kUsedCols <= 64 ? 64 : kUsedCols <= 128 ? 128 : kUsedCols <= 256 ? 256 : 512;
     static_assert(kUsedCols <= 512, "tensor memory");
+    // (four warps bring rows to terms in turn: as many stages as warps keep each of them within a round of the ring)
+    static constexpr int kMinStages = kConverts ? 4 : 3;
+    // bytes of a block of a cluster or alone, and the stages that fit a multiprocessor's or half of its shared memory
+    static constexpr size_t recv_bytes(bool cluster) { return cluster ? kRecvFloats * 4 : 0; }
+    // (blocks that share a multiprocessor have tensor memory for both: the blocks of two clusters that wait for each other's would wait for good)
+    static constexpr int stages_for(int blocks, bool cluster) {
+        if (blocks == 2 && kTmemCols > 256) return 0;
+        const int n = (int)(((blocks == 2 ? 113 : 226) * 1024 - kFixed - recv_bytes(cluster)) / kStageStride);
+        return n < kMaxStages ? n : kMaxStages;
+    }
+    static_assert(stages_for(1, true) >= 4, "shared memory");
     static constexpr uint32_t kInstr = scaled_instr(kE2M1, kQuantized ? kE2M1 : kE4M3, BW, NX);
 };
 
@@ -64,7 +70,7 @@ struct Args {
     const uint8_t* x_scales;      // 4 bits, and terms that were prepared
     const uint8_t* w_scales;
     const void* bias;
-    int bias_dtype, M, N, K, chunks, n_tiles, vector;      // vector: x's rows are whole aligned 16-byte pieces
+    int bias_dtype, M, N, K, chunks, n_tiles, stages, vector;      // vector: x's rows are whole aligned 16-byte pieces
     int* err;
     int skip_loads;               // the test of the bounded waits: nothing is loaded
 };
@@ -95,13 +101,15 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     pdl_launch_dependents();
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* recv = reinterpret_cast<float*>(tiles + (size_t)S::kStages * S::kStageStride);
-    uint64_t* full = reinterpret_cast<uint64_t*>(recv + S::kRecvFloats);
-    uint64_t* empty = full + S::kStages;
-    uint64_t* acc_full = empty + S::kStages;   // [2] accumulator ready to be summed
+    const int stages = a.stages;
+    uint64_t* full = reinterpret_cast<uint64_t*>(tiles + (size_t)stages * S::kStageStride);
+    uint64_t* empty = full + kMaxStages;
+    uint64_t* acc_full = empty + kMaxStages;   // [2] accumulator ready to be summed
     uint64_t* acc_empty = acc_full + 2;        // [2] accumulator read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* give_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* recv = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(full) + 512);      // (a cluster's blocks)
+    static_assert((2 * kMaxStages + 4) * 8 + 8 <= 512, "barriers");
 
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank(), n_ranks = (int)cluster_size();
@@ -120,11 +128,11 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
         tma_load_2d(dst, &map_w, full + s, c * BK, tile * BW);
         bulk_load(dst + kWSmem + S::kXSmem, a.w_scales + ((long long)tile * a.chunks + c) * kMx4AtomBytes, kMx4AtomBytes, full + s);
     };
-    const int early = a.skip_loads ? 0 : min(S::kStages, n);
+    const int early = a.skip_loads ? 0 : min(stages, n);
     if (warp == 0 && elect_one()) {
         // W of the first stages, before anything else: nobody but this thread need know of the barriers yet
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
-        for (int s = 0; s < S::kStages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(full + s, S::kConverts ? 2 : 1);     // the copies, and the warp that brings x
             mbar_init(empty + s, 1);
         }
@@ -165,18 +173,22 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
         if (issues)
             for (int i = 0; i < early; ++i) load_x(i, c0 + i);
         __syncwarp();
-        int it = early;
+        int s = early == stages ? 0 : early;
+        uint32_t phase = early == stages ? 0 : 1;            // of the stage's last use; 1: never used
         bool ok = !a.skip_loads;
         for (int tile = first_tile, i0 = early; tile < a.n_tiles && ok; tile += step, i0 = 0) {
-            for (int i = i0; i < n; ++i, ++it) {
-                const int s = it % S::kStages;
-                ok = __all_sync(0xffffffffu, mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1) && !*give_up);
+            for (int i = i0; i < n; ++i) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty + s, phase) && !*give_up);
                 if (!ok) break;
                 if (issues) {
                     load_w(s, tile, c0 + i);
                     load_x(s, c0 + i);
                 }
                 __syncwarp();
+                if (++s == stages) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
         }
         if (!ok && !a.skip_loads && lane == 0) give_up_at();
@@ -201,7 +213,7 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + buf * S::NX;
             for (int i = 0; i < n && ok; ++i, ++it) {
-                const int next = s + 1 == S::kStages ? 0 : s + 1;
+                const int next = s + 1 == stages ? 0 : s + 1;
                 const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
                 if (!brought) {
                     ok = __all_sync(0xffffffffu, mbar_wait(full + s, phase));
@@ -249,8 +261,8 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
             };
             auto convert = [&](int it, const Eight<RT> (&e)[PAIRS]) {
                 if (__any_sync(0xffffffffu, *give_up)) return false;           // all lanes together
-                const int s = it % S::kStages;
-                if (it >= S::kStages && !__all_sync(0xffffffffu, mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1))) {
+                const int round = it / stages, s = it - round * stages;
+                if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(empty + s, (round & 1) ^ 1))) {
                     if (lane == 0) give_up_at();
                     return false;
                 }
@@ -410,51 +422,79 @@ __global__ void __launch_bounds__(256) mx4_terms_kernel(uint8_t* __restrict__ by
     });
 }
 
-// The largest cluster of which n_tiles are resident together and have a piece of K a block; 1: a block alone.
+// Clusters of `c` blocks that are resident together, `blocks` a multiprocessor.
 template <typename S, typename Kernel>
-int cluster_for(Kernel kernel, int n_tiles, int chunks) {
-    static const std::array<int, kMaxCluster + 1> resident = [&] {       // clusters of each size
-        std::array<int, kMaxCluster + 1> n = {};
-        for (int c = 2; c <= kMaxCluster; ++c) {
-            cudaLaunchConfig_t config = {};
-            config.gridDim = dim3((unsigned)(c * 512));
-            config.blockDim = dim3(S::kThreads);
-            config.dynamicSmemBytes = S::kSmemBytes;
-            cudaLaunchAttribute attribute[1];
-            attribute[0].id = cudaLaunchAttributeClusterDimension;
-            attribute[0].val.clusterDim.x = (unsigned)c;
-            attribute[0].val.clusterDim.y = 1;
-            attribute[0].val.clusterDim.z = 1;
-            config.attrs = attribute;
-            config.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n[c], kernel, &config) != cudaSuccess) {
-                cudaGetLastError();
-                n[c] = 0;
-            }
-        }
+int resident_clusters(Kernel kernel, int c, int blocks) {
+    static std::array<int, 2 * (kMaxCluster + 1)> held = [] {
+        std::array<int, 2 * (kMaxCluster + 1)> n;
+        n.fill(-1);
         return n;
     }();
-    for (int c = kMaxCluster; c >= 2; --c)
-        if (c <= chunks && resident[c] >= n_tiles) return c;
-    return 1;
+    int& n = held[(blocks - 1) * (kMaxCluster + 1) + c];
+    if (n < 0) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3((unsigned)(c * 512));
+        config.blockDim = dim3(S::kThreads);
+        config.dynamicSmemBytes = S::stages_for(blocks, true) * S::kStageStride + S::kFixed + S::recv_bytes(true);
+        cudaLaunchAttribute attribute[1];
+        attribute[0].id = cudaLaunchAttributeClusterDimension;
+        attribute[0].val.clusterDim.x = (unsigned)c;
+        attribute[0].val.clusterDim.y = 1;
+        attribute[0].val.clusterDim.z = 1;
+        config.attrs = attribute;
+        config.numAttrs = 1;
+        int found = 0;
+        if (cudaOccupancyMaxActiveClusters(&found, kernel, &config) != cudaSuccess) {
+            cudaGetLastError();
+            found = 0;
+        }
+        n = found;
+    }
+    return n;
+}
+
+// How a weight is cut: blocks of a cluster, and blocks a multiprocessor.
+struct Cut {
+    int cluster, blocks;
+};
+
+// Few tiles: the largest cluster of which all are resident together and that has a piece of K a block, two blocks a multiprocessor where a half of
+// its shared memory holds four stages, else one.  More tiles: blocks alone, two a multiprocessor where there are more tiles than those and four
+// stages fit (34,816 x 5,120 is 272 tiles: 1.84 rounds of single blocks, of which the second leaves the memory idle in part).
+template <typename S, typename Kernel>
+Cut cut_for(Kernel kernel, int n_tiles, int chunks, int n_sms) {
+    if (n_tiles <= n_sms) {
+        const int most = chunks < kMaxCluster ? chunks : kMaxCluster;
+        if (S::stages_for(2, true) >= 4)
+            for (int c = most; c >= 2; --c)
+                if (n_tiles * c <= 2 * n_sms && resident_clusters<S>(kernel, c, 2) >= n_tiles) return {c, 2};
+        for (int c = most; c >= 2; --c)
+            if (n_tiles * c <= n_sms && resident_clusters<S>(kernel, c, 1) >= n_tiles) return {c, 1};
+        if (S::stages_for(2, true) >= S::kMinStages)
+            for (int c = most; c >= 2; --c)
+                if (n_tiles * c <= 2 * n_sms && resident_clusters<S>(kernel, c, 2) >= n_tiles) return {c, 2};
+    }
+    return {1, n_tiles > n_sms && S::stages_for(2, false) >= 4 ? 2 : 1};
 }
 
 template <typename RT, int MR, int PAIRS, typename OutT>
-int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const Args& args, cudaStream_t stream) {
+int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, Args args, cudaStream_t stream) {
     using S = Shape<RT, MR, PAIRS>;
     auto kernel = mx4_stream_kernel<RT, MR, PAIRS, OutT>;
-    static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmemBytes);
+    static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
     if (configured != cudaSuccess) {
-        thn_set_error("mx4_stream: cannot reserve %zu bytes of shared memory: %s", S::kSmemBytes, cudaGetErrorString(configured));
+        thn_set_error("mx4_stream: cannot reserve %d bytes of shared memory: %s", 226 * 1024, cudaGetErrorString(configured));
         return (int)configured;
     }
     int device = 0, n_sms = 0;
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
-    const int c = cluster_for<S>(kernel, args.n_tiles, args.chunks);
-    const int slots = n_sms * (S::kSmemBytes <= 113 * 1024 ? 2 : 1);
-    const int grid = c > 1 ? args.n_tiles * c : args.n_tiles < slots ? args.n_tiles : slots;
-    thn_launch_cluster(kernel, dim3((unsigned)grid), dim3(S::kThreads), S::kSmemBytes, stream, dim3((unsigned)c, 1, 1), map_w, map_x, args);
+    const Cut cut = cut_for<S>(kernel, args.n_tiles, args.chunks, n_sms);
+    args.stages = S::stages_for(cut.blocks, cut.cluster > 1);
+    const size_t smem = args.stages * S::kStageStride + S::kFixed + S::recv_bytes(cut.cluster > 1);
+    const int slots = n_sms * cut.blocks;
+    const int grid = cut.cluster > 1 ? args.n_tiles * cut.cluster : args.n_tiles < slots ? args.n_tiles : slots;
+    thn_launch_cluster(kernel, dim3((unsigned)grid), dim3(S::kThreads), smem, stream, dim3((unsigned)cut.cluster, 1, 1), map_w, map_x, args);
     return thn_launch_status("mx4_stream");
 }
 
