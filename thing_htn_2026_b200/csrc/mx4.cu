@@ -85,36 +85,6 @@ struct Piece<__nv_bfloat16> {
     }
 };
 
-// Division of numbers below 2^31 by a divisor that the host knows: n / d = (hi(n m) + n) >> l with 2^(l-1) < d <= 2^l and
-// m = floor(2^32 (2^l - d) / d) + 1.
-struct Divisor {
-    uint32_t d, m, l;
-    explicit Divisor(uint32_t divisor) : d(divisor), l(0) {
-        while ((1ull << l) < d) ++l;
-        m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
-    }
-    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(n, m) + n) >> l; }
-};
-
-// Row and piece of a unit, and of those kThreads further on.
-struct Place {
-    uint32_t row, piece;
-    __device__ __forceinline__ Place(uint32_t unit, const Divisor& pieces) : row(pieces.of(unit)), piece(unit - row * pieces.d) {}
-    __device__ __forceinline__ void step(const Divisor& pieces) {
-        piece += kThreads;
-        if (pieces.d >= kThreads) {
-            if (piece >= pieces.d) {
-                piece -= pieces.d;
-                ++row;
-            }
-        } else {
-            const uint32_t more = pieces.of(piece);
-            row += more;
-            piece -= more * pieces.d;
-        }
-    }
-};
-
 // Pieces of eight entries: a thread takes kAhead of them, kThreads apart, and asks for all of them before it works on the first.  Bound by the
 // memory: 2,048 rows of 9,728 bfloat16 entries, which lie in the L2 cache or not.  Four threads have a block's entries, sixteen the columns of four
 // scale bytes.
@@ -122,17 +92,17 @@ constexpr int kAhead = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                const T* __restrict__ x, uint32_t units, Divisor pieces, long long columns,
+                                                                const T* __restrict__ x, uint32_t units, Mx4Divisor pieces, long long columns,
                                                                 long long padded, bool vector) {
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t first = blockIdx.x * (uint32_t)(kThreads * kAhead) + threadIdx.x;
     Piece<T> held[kAhead];
-    Place at(first, pieces);
+    Mx4Place<kThreads> at(first, pieces);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a, at.step(pieces))
         held[a].load(x + (long long)at.row * columns, (int)(at.piece * 8), first + a * kThreads < units ? (int)columns : 0, vector);
-    at = Place(first, pieces);
+    at = Mx4Place<kThreads>(first, pieces);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
         uint32_t top = held[a].top();
@@ -154,14 +124,14 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(uint8_t* __restr
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes,
-                                                                  const uint8_t* __restrict__ scales, uint32_t units, Divisor pieces,
+                                                                  const uint8_t* __restrict__ scales, uint32_t units, Mx4Divisor pieces,
                                                                   long long columns, long long padded, bool vector) {
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t first = blockIdx.x * (uint32_t)(kThreads * kAhead) + threadIdx.x;
     uint32_t words[kAhead];
     uint8_t bytes[kAhead];
-    Place at(first, pieces);
+    Mx4Place<kThreads> at(first, pieces);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
         if (first + a * kThreads < units) {
@@ -169,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict_
             bytes[a] = scales[mx4_scale_at(at.row, at.piece / 16, padded / kMx4Atom) + (at.piece % 16) / 4];
         }
     }
-    at = Place(first, pieces);
+    at = Mx4Place<kThreads>(first, pieces);
 #pragma unroll
     for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
         if (first + a * kThreads >= units) break;
@@ -254,7 +224,7 @@ int quantize(uint8_t* codes, uint8_t* scales, const T* x, long long rows, long l
     const bool vector = ((uintptr_t)x & 15) == 0 && columns % (16 / sizeof(T)) == 0;
     return in_steps(rows, pieces, [&](long long row, long long n) {
         thn_launch(mx4_quantize_kernel<T>, (unsigned)((n * pieces + kThreads * kAhead - 1) / (kThreads * kAhead)), kThreads, 0, stream, codes + row * (padded / 2),
-                   scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, x + row * columns, (uint32_t)(n * pieces), Divisor((uint32_t)pieces), columns,
+                   scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, x + row * columns, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces), columns,
                    padded, vector);
         return thn_launch_status("mx4_quantize");
     });
@@ -266,7 +236,7 @@ int dequantize(T* out, const uint8_t* codes, const uint8_t* scales, long long ro
     const bool vector = ((uintptr_t)out & 15) == 0 && columns % (16 / sizeof(T)) == 0;
     return in_steps(rows, pieces, [&](long long row, long long n) {
         thn_launch(mx4_dequantize_kernel<T>, (unsigned)((n * pieces + kThreads * kAhead - 1) / (kThreads * kAhead)), kThreads, 0, stream, out + row * columns,
-                   codes + row * (padded / 2), scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, (uint32_t)(n * pieces), Divisor((uint32_t)pieces),
+                   codes + row * (padded / 2), scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces),
                    columns, padded, vector);
         return thn_launch_status("mx4_dequantize");
     });

@@ -35,3 +35,34 @@ __device__ __forceinline__ float mx4_scale(uint32_t b) {
 __device__ __forceinline__ float mx4_value(uint32_t code) {
     return __uint_as_float((code & 7) << 22 | (code & 8) << 28) * 8.507059173023462e37f;      // 2^126
 }
+
+// Division of numbers below 2^31 by a divisor that the host knows: n / d = (hi(n m) + n) >> l with 2^(l-1) < d <= 2^l and
+// m = floor(2^32 (2^l - d) / d) + 1.
+struct Mx4Divisor {
+    uint32_t d, m, l;
+    explicit Mx4Divisor(uint32_t divisor) : d(divisor), l(0) {
+        while ((1ull << l) < d) ++l;
+        m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(n, m) + n) >> l; }
+};
+
+// Row and piece of a unit of eight entries, and of those STEP further on.
+template <uint32_t STEP>
+struct Mx4Place {
+    uint32_t row, piece;
+    __device__ __forceinline__ Mx4Place(uint32_t unit, const Mx4Divisor& pieces) : row(pieces.of(unit)), piece(unit - row * pieces.d) {}
+    __device__ __forceinline__ void step(const Mx4Divisor& pieces) {
+        piece += STEP;
+        if (pieces.d >= STEP) {
+            if (piece >= pieces.d) {
+                piece -= pieces.d;
+                ++row;
+            }
+        } else {
+            const uint32_t more = pieces.of(piece);
+            row += more;
+            piece -= more * pieces.d;
+        }
+    }
+};

@@ -9,7 +9,7 @@
 //    prepared, 128 columns of the sum at a time, kind::mxf8f6f4; W's codes are spread over 8-bit containers by TMA as they are
 //    copied.  Two terms at twice the rate of bfloat16 cost what a bfloat16 product costs; W is a quarter of the bytes.
 //  * Scales: 512 bytes for 128 rows and 128 columns, by TMA like the operands, to tensor memory by tcgen05.cp just ahead of the
-//    products that use them.  A tile's rows of x begin at a multiple of 64, two columns of scales.
+//    products that use them.  A tile's rows of x begin at a multiple of 64 rows of its operand, two columns of scales.
 //
 // A row's result depends on its own entries and its place in a tile alone.  Every wait on an mbarrier is bounded: after
 // kWaitLimitNs the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, what is left to store becomes NaN, and tensor
@@ -46,7 +46,7 @@ struct Args {
     const void* bias;
     int bias_dtype, M, N, atoms;                // atoms: pieces of 128 columns of the sum
     int cuts, size, n_tiles;        // the rows of x in equal tiles
-    int plane_atoms;                // rows of a term's plane / 128
+    int pitch;                      // rows of x's operand from one tile to the next
     int* err;
     int skip_loads;                 // the test of the bounded waits: nothing is loaded
 };
@@ -129,9 +129,9 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// Rows [row0, row0 + here) of x by features from `feature` on; columns: the rows rounded up to 64.
+// Rows [row0, row0 + here) of x, which begin at row x_row of its operand, by features from `feature` on; columns: the rows rounded up to 32.
 struct Tile {
-    int row0, here, columns, feature;
+    int row0, here, columns, x_row, feature;
 };
 
 template <int MODE, typename OutT>
@@ -182,7 +182,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
         const int f = i / a.cuts, cut = i - f * a.cuts;
         t.row0 = cut * a.size;
         t.here = min(a.size, a.M - t.row0);
-        t.columns = (t.here + 63) / 64 * 64;
+        t.columns = (t.here + 31) / 32 * 32;
+        t.x_row = cut * a.pitch;
         t.feature = f * kFeatures;
         return t;
     };
@@ -194,7 +195,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
         int it = 0;
         for (int i = pair; i < a.n_tiles && !__any_sync(0xffffffffu, *give_up); i += n_pairs) {
             const Tile t = tile_of(i);
-            const int b_row = t.row0 + rank * (t.columns / 2), a_row = t.feature + rank * 128;
+            const int b_row = t.x_row + rank * (t.columns / 2), a_row = t.feature + rank * 128;
             // (a last tile of fewer columns brings what a whole one does)
             constexpr uint32_t kBytes = (MODE == kQuantized ? S::kASmem : S::kASmem / 2) + S::kT * S::kBSmem + S::kScaleBytes;
             for (int kb = 0; kb < n_k && !a.skip_loads; ++kb, ++it) {
@@ -212,7 +213,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                 load_box(dst, &map_w, bar, kb * 128, a_row);           // (bytes of codes, or entries)
                 load_box(dst + S::kASmem, &map_x, bar, kb * 128, b_row, 0);
                 load_box(scales, &map_w_scales, bar, 0, kb * S::kSteps, a_row >> 7, 0);
-                load_box(scales + S::kSteps * kMx4AtomBytes, &map_x_scales, bar, 0, kb * S::kSteps, t.row0 >> 7, 0);
+                load_box(scales + S::kSteps * kMx4AtomBytes, &map_x_scales, bar, 0, kb * S::kSteps, t.x_row >> 7, 0);
                 }
                 __syncwarp();
             }
@@ -242,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
         for (int i = pair; i < a.n_tiles && ok; i += n_pairs, ++local) {
             const Tile t = tile_of(i);
             const uint32_t instr = MODE == kQuantized ? scaled_instr(1, 1, kFeatures, t.columns) : scaled_instr(kE2M1, kE4M3, kFeatures, t.columns);
-            const uint32_t first = (t.row0 & 127) >> 5;          // the tile's first column of scales
+            const uint32_t first = (t.x_row & 127) >> 5;          // the tile's first column of scales
             const int buf = local % S::kBuffers;
             ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1) && !*give_up);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -381,6 +382,13 @@ bool map_planes(CUtensorMap* map, const void* base, long long width, long long r
                     {(cuuint64_t)width, (cuuint64_t)(width * rows), 0}, {128, (cuuint32_t)box_rows, (cuuint32_t)planes, 1}, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+int pair_count() {
+    int device = 0, n_sms = 0;
+    cudaGetDevice(&device);
+    if (cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) cudaGetLastError();
+    return n_sms >= 2 ? n_sms / 2 : 1;
+}
+
 template <int MODE, typename OutT>
 int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) {
     auto kernel = mx4_pair_kernel<MODE, OutT>;
@@ -389,10 +397,7 @@ int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) 
         thn_set_error("mx4_pair: cannot reserve %zu bytes of shared memory: %s", Shape<MODE>::kSmemBytes, cudaGetErrorString(configured));
         return (int)configured;
     }
-    int device = 0, n_sms = 0;
-    cudaGetDevice(&device);
-    cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
-    const int pairs = args.n_tiles < n_sms / 2 ? args.n_tiles : n_sms / 2;
+    const int most = pair_count(), pairs = args.n_tiles < most ? args.n_tiles : most;
     thn_launch(kernel, dim3((unsigned)(2 * pairs)), kThreads, Shape<MODE>::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], args);
     return thn_launch_status("mx4_pair");
 }
@@ -401,21 +406,18 @@ template <int MODE>
 int run(Args args, const void* codes, const void* scales, const void* x, const void* x_scales, int out_dtype, cudaStream_t stream) {
     using S = Shape<MODE>;
     const long long padded = (long long)args.atoms * kMx4Atom;
-    args.cuts = (args.M + S::kCols - 1) / S::kCols;
-    args.size = ((args.M + args.cuts - 1) / args.cuts + 63) / 64 * 64;
-    args.cuts = (args.M + args.size - 1) / args.size;
     const long long n_tiles = (long long)args.cuts * ((args.N + kFeatures - 1) / kFeatures);
     THN_UNSUPPORTED_IF(n_tiles > 0x3fffffff, "mx4_pair: M=%d N=%d are too many tiles", args.M, args.N);
     args.n_tiles = (int)n_tiles;
-    args.plane_atoms = (args.M + 127) / 128;
+    const long long x_rows = MODE == kQuantized ? args.M : (long long)args.cuts * args.pitch;
     CUtensorMap maps[4];
     bool made = map_scales(&maps[1], scales, args.atoms, (args.N + 127) / 128, 1, S::kSteps, 1) &&
-                map_scales(&maps[3], x_scales, args.atoms, args.plane_atoms, S::kT, S::kSteps, S::kAtoms);
+                map_scales(&maps[3], x_scales, args.atoms, (x_rows + 127) / 128, S::kT, S::kSteps, S::kAtoms);
     if (MODE == kQuantized)
-        made = made && map_bytes(&maps[0], codes, args.N, padded / 2, 128) && map_planes(&maps[2], x, padded / 2, args.M, 1, S::kCols / 2);
+        made = made && map_bytes(&maps[0], codes, args.N, padded / 2, 128) && map_planes(&maps[2], x, padded / 2, x_rows, 1, S::kCols / 2);
     else
         made = made && map_unpacked(&maps[0], codes, args.N, padded, 128) &&
-               map_planes(&maps[2], x, padded, (long long)args.plane_atoms * 128, S::kT, S::kCols / 2);
+               map_planes(&maps[2], x, padded, x_rows, S::kT, S::kCols / 2);
     if (!made) {
         thn_set_error("mx4_pair: cuTensorMapEncodeTiled failed for M=%d N=%d and %d pieces of K", args.M, args.N, args.atoms);
         return THN_BAD_ARGUMENT;
@@ -425,16 +427,40 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
 
 }  // namespace
 
-// The bytes of `terms` that M rows of a type need.
-static long long terms_needed(int x_type, int M, int K) {
+// How M rows are cut into tiles by N outputs: the size (a multiple of 32) with which the pairs' rounds take the least time, a stage of a tile counted
+// with 4 clocks a column (rows in 4 bits: 2), the products' time, but 500 at least, which its thread takes to issue them; the rows of x's operand from one tile to the
+// next.  Terms are written by a kernel of this library, which begins every tile at a whole piece of 128 rows of scales; rows in 4 bits lie as they
+// do, and their tiles begin at multiples of 64.  (2,048 rows by 2,560 outputs are 130 tiles of 160 rows, two rounds, or 110 of 192, two rounds.)
+struct RowCuts {
+    int cuts, size, pitch;
+};
+static RowCuts cuts_for(bool quantized, int M, int N, int pairs) {
+    const int most = Shape<kQuantized>::kCols, grain = quantized ? 64 : 32, clocks = quantized ? 2 : 4;
+    const long long features = (N + kFeatures - 1) / kFeatures;
+    RowCuts best = {};
+    long long least = 0;
+    for (int size = most; size >= grain; size -= grain) {
+        const long long cuts = (M + size - 1) / size, rounds = (cuts * features + pairs - 1) / pairs;
+        const int columns = cuts == 1 ? (M + 31) / 32 * 32 : size;
+        const long long time = rounds * (clocks * columns < 500 ? 500 : clocks * columns);
+        if (best.cuts == 0 || time < least) {
+            best = {(int)cuts, size, quantized ? size : (size + 127) / 128 * 128};
+            least = time;
+        }
+    }
+    return best;
+}
+
+// The bytes of `terms` that M rows of a type need by N outputs.
+static long long terms_needed(int x_type, int M, int N, int K) {
     if (x_type == 2) return 0;
-    const long long atoms = (long long)((M + 127) / 128) * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
-    return atoms * 128 * padded + atoms * (padded / kMx4Atom) * kMx4AtomBytes;
+    const RowCuts c = cuts_for(false, M, N, pair_count());
+    const long long rows = (long long)c.cuts * c.pitch * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
+    return rows * padded + rows / 128 * (padded / kMx4Atom) * kMx4AtomBytes;
 }
 
 THN_API int thn_mx4_pair_scratch(int x_type, int M, int N, int K, long long* bytes) {
-    (void)N;
-    *bytes = terms_needed(x_type, M, K);
+    *bytes = terms_needed(x_type, M, N, K);
     return THN_OK;
 }
 
@@ -451,8 +477,8 @@ THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_
     THN_UNSUPPORTED_IF(M < 1 || M > (1 << 24) || N < 1 || N > (1 << 24) || K < 1 || K > (1 << 24), "mx4_pair: M=%d N=%d K=%d not supported", M, N, K);
     THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 &&
                   (((uintptr_t)scales | (uintptr_t)x_scales | (uintptr_t)terms) & 15) == 0, "mx4_pair: codes must be 32-byte, scales and terms 16-byte aligned");
-    THN_CHECK_ARG(terms_bytes >= terms_needed(x_type, M, K), "mx4_pair: %lld bytes of scratch, %lld needed", terms_bytes,
-                  terms_needed(x_type, M, K));
+    THN_CHECK_ARG(terms_bytes >= terms_needed(x_type, M, N, K), "mx4_pair: %lld bytes of scratch, %lld needed", terms_bytes,
+                  terms_needed(x_type, M, N, K));
     Args args = {};
     args.out = out;
     args.bias = bias;
@@ -462,13 +488,17 @@ THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_
     args.atoms = (int)(mx4_padded(K) / kMx4Atom);
     args.err = err;
     args.skip_loads = skip_loads;
-    THN_UNSUPPORTED_IF((long long)(N + 127) / 128 * args.atoms > 0x7fffffff || (long long)(M + 127) / 128 * 6 * args.atoms > 0x7fffffff,
-                       "mx4_pair: M=%d N=%d K=%d: too many scales", M, N, K);
+    const RowCuts rows = cuts_for(x_type == 2, M, N, pair_count());
+    args.cuts = rows.cuts;
+    args.size = rows.size;
+    args.pitch = rows.pitch;
+    const long long plane = (long long)rows.cuts * rows.pitch;
+    THN_UNSUPPORTED_IF((long long)(N + 127) / 128 * args.atoms > 0x7fffffff || plane / 128 * 6 * args.atoms > 0x7fffffff || plane * 6 > 0x7fffffff,
+                       "mx4_pair: M=%d N=%d K=%d is too large", M, N, K);
     if (x_type == 2) return run<kQuantized>(args, codes, scales, x, x_scales, out_dtype, stream);
-    const int plane = (M + 127) / 128 * 128;
     uint8_t* bytes = static_cast<uint8_t*>(terms);
-    uint8_t* term_scales = bytes + (long long)plane * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>) * mx4_padded(K);
-    const int status = mx4_terms(bytes, term_scales, x, x_type, M, K, plane, stream);
+    uint8_t* term_scales = bytes + plane * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>) * mx4_padded(K);
+    const int status = mx4_terms(bytes, term_scales, x, x_type, M, K, (int)plane, rows.size, rows.pitch, stream);
     if (status != THN_OK) return status;
     if (x_type == THN_F32) return run<kRows6>(args, codes, scales, bytes, term_scales, out_dtype, stream);
     return run<kRows2>(args, codes, scales, bytes, term_scales, out_dtype, stream);

@@ -388,38 +388,45 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     }
 }
 
-// Rows as terms of 8-bit floats: term t of row r at [t * plane + r], its scales as mx4.cuh lays out those of such a matrix.
-// A thread takes eight columns.
+// Rows as terms of 8-bit floats (mx4_terms).  A thread takes eight columns of kAhead units and asks for all of them first.
+constexpr int kTermThreads = 256, kAhead = 4;
+
 template <typename RT>
-__global__ void __launch_bounds__(256) mx4_terms_kernel(uint8_t* __restrict__ bytes, uint8_t* __restrict__ scales, const RT* __restrict__ x, int M, int K,
-                                                        int padded, int plane, bool vector) {
+__global__ void __launch_bounds__(kTermThreads) mx4_terms_kernel(uint8_t* __restrict__ bytes, uint8_t* __restrict__ scales, const RT* __restrict__ x,
+                                                                 uint32_t units, Mx4Divisor pieces, Mx4Divisor size, int pitch, int K, int padded, int plane,
+                                                                 bool vector) {
     pdl_launch_dependents();
     pdl_wait();
-    const int pieces = padded / 8;
-    const long long unit = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int row = (int)(unit / pieces), piece = (int)(unit - (long long)row * pieces);
-    const bool there = row < M;
-    Eight<RT> e;
-    if (there) e.load(x + (long long)row * K, piece * 8, K, vector);
-    uint32_t top = there ? e.top() : 0;
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t b = row_scale_byte(top);
-    // the sixteen threads' four scale bytes of the first term as one word
-    uint32_t four = b << (8 * ((threadIdx.x >> 2) & 3));
-    four |= __shfl_xor_sync(0xffffffffu, four, 4);
-    four |= __shfl_xor_sync(0xffffffffu, four, 8);
-    if (!there) return;
-    e.terms(b, [&](int term, uint2 v) {
-        const long long at = (long long)term * plane + row;
-        *reinterpret_cast<uint2*>(bytes + at * padded + piece * 8) = v;
-        if ((threadIdx.x & 15) == 0) {
-            uint32_t w = 0;
+    const uint32_t first = blockIdx.x * (uint32_t)(kTermThreads * kAhead) + threadIdx.x;
+    Eight<RT> held[kAhead];
+    Mx4Place<kTermThreads> place(first, pieces);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w |= term_scale_byte(four >> (8 * i) & 255, term) << (8 * i);
-            *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(at, piece / 16, padded / kMx4Atom)) = w;
-        }
-    });
+    for (int a = 0; a < kAhead; ++a, place.step(pieces))
+        held[a].load(x + (long long)place.row * K, place.piece * 8, first + a * kTermThreads < units ? K : 0, vector);
+    place = Mx4Place<kTermThreads>(first, pieces);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a, place.step(pieces)) {
+        uint32_t top = held[a].top();
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t b = row_scale_byte(top);
+        // the sixteen threads' four scale bytes of the first term as one word
+        uint32_t four = b << (8 * ((threadIdx.x >> 2) & 3));
+        four |= __shfl_xor_sync(0xffffffffu, four, 4);
+        four |= __shfl_xor_sync(0xffffffffu, four, 8);
+        if (first + a * kTermThreads >= units) continue;
+        const uint32_t tile = size.of(place.row), row = tile * pitch + (place.row - tile * size.d);
+        held[a].terms(b, [&](int term, uint2 v) {
+            const long long at = (long long)term * plane + row;
+            *reinterpret_cast<uint2*>(bytes + at * padded + place.piece * 8) = v;
+            if ((threadIdx.x & 15) == 0) {
+                uint32_t w = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w |= term_scale_byte(four >> (8 * i) & 255, term) << (8 * i);
+                *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(at, place.piece / 16, padded / kMx4Atom)) = w;
+            }
+        });
+    }
 }
 
 // Clusters of `c` blocks that are resident together, `blocks` a multiprocessor.
@@ -508,7 +515,7 @@ int launch_rows(Args args, const void* codes, long long padded, void* terms, int
     else if constexpr (!S::kConverts) {
         uint8_t* bytes = static_cast<uint8_t*>(terms);
         uint8_t* scales = bytes + (long long)S::kT * MR * padded;
-        const int status = mx4_terms(bytes, scales, args.x, sizeof(RT) == 4 ? THN_F32 : THN_BF16, args.M, args.K, MR, stream);
+        const int status = mx4_terms(bytes, scales, args.x, sizeof(RT) == 4 ? THN_F32 : THN_BF16, args.M, args.K, MR, MR, MR, stream);
         if (status != THN_OK) return status;
         args.x_scales = scales;
         made = made && map_bytes(&map_x, bytes, S::kT * MR, padded, S::NX);
@@ -525,15 +532,18 @@ int room_for(int M) { return M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64; }
 
 }  // namespace
 
-int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K, int plane, cudaStream_t stream) {
-    const long long padded = mx4_padded(K), blocks = ((long long)M * (padded / 8) + 255) / 256;
-    THN_UNSUPPORTED_IF(blocks > 0x7fffffff, "mx4_terms: %d rows of %d entries are too many", M, K);
+int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K, int plane, int size, int pitch, cudaStream_t stream) {
+    const long long padded = mx4_padded(K), units = (long long)M * (padded / 8);
+    THN_UNSUPPORTED_IF(units > 0x7ffff000, "mx4_terms: %d rows of %d entries are too many", M, K);
+    const unsigned blocks = (unsigned)((units + kTermThreads * kAhead - 1) / (kTermThreads * kAhead));
     const bool vector = ((uintptr_t)x & 15) == 0 && K % 8 == 0;
+    const Mx4Divisor pieces((uint32_t)(padded / 8)), rows((uint32_t)size);
     if (x_type == THN_F32)
-        thn_launch(mx4_terms_kernel<float>, (unsigned)blocks, 256, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const float*)x, M, K, (int)padded, plane, vector);
+        thn_launch(mx4_terms_kernel<float>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const float*)x, (uint32_t)units, pieces, rows,
+                   pitch, K, (int)padded, plane, vector);
     else
-        thn_launch(mx4_terms_kernel<__nv_bfloat16>, (unsigned)blocks, 256, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const __nv_bfloat16*)x, M, K,
-                   (int)padded, plane, vector);
+        thn_launch(mx4_terms_kernel<__nv_bfloat16>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const __nv_bfloat16*)x,
+                   (uint32_t)units, pieces, rows, pitch, K, (int)padded, plane, vector);
     return thn_launch_status("mx4_terms");
 }
 

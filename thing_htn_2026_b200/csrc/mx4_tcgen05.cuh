@@ -5,9 +5,9 @@
 
 #include "mx4.cuh"
 
-// Rows x [M, K] of a type (THN_F32, THN_BF16) as terms of 8-bit floats, see below: term t of row r is row t * plane + r of a matrix of bytes
-// [terms * plane, padded], whose scales lie as mx4.cuh says (mx4_stream.cu).
-int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K, int plane, cudaStream_t stream);
+// Rows x [M, K] of a type (THN_F32, THN_BF16) as terms of 8-bit floats, see below: term t of row r is row t * plane + r / size * pitch + r % size of a
+// matrix of bytes [terms * plane, padded], whose scales lie as mx4.cuh says (mx4_stream.cu).
+int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K, int plane, int size, int pitch, cudaStream_t stream);
 
 namespace {
 
