@@ -257,15 +257,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (issues) bring_scales(s, it & 1);
                 }
-                // The next stage's scales ahead of this one's products: with rows in 4 bits, where issuing takes as long as the products, once they
-                // have come (8,192 rows of 4,096 by 24,576 outputs 323 us, 322 with the test and its second way); with fewer stages if they have.
-                brought = it + 1 < total;
-                if (brought && MODE == kQuantized) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(full + next, next_phase));
-                    if (!ok) break;
-                } else if (brought) {
-                    brought = __all_sync(0xffffffffu, mbar_here(full + next, next_phase));
-                }
+                brought = it + 1 < total && __all_sync(0xffffffffu, mbar_here(full + next, next_phase));
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = smem_addr(tiles + (size_t)s * S::kStageStride);
                 const uint32_t w_col = tmem_base + S::kScaleCol + (it & 1) * S::kScaleCols, x_col = w_col + 4 * S::kSteps + first;
