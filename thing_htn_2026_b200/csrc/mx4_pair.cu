@@ -62,8 +62,10 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
     return a;
 }
+// All threads of both blocks.  (Not the .aligned form, which counts warps: a warp whose lanes come one after the other would count twice.)
 __device__ __forceinline__ void pair_barrier() {
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 // A box to this block's shared memory, its bytes counted by the leading block's barrier.
 __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
@@ -139,7 +141,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w_scales, const __grid_constant__ CUtensorMap map_x,
     const __grid_constant__ CUtensorMap map_x_scales, const Args a) {
     using S = Shape<MODE>;
-    pdl_launch_dependents();
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(tiles + (size_t)S::kStages * S::kStageStride);
@@ -165,6 +166,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
         *give_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
     if (warp == 1) {   // the same warp of both blocks allocates
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -172,9 +174,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     pair_barrier();                            // both blocks' barriers stand
+    __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     constexpr uint32_t tmem_base = 0;          // all columns are this pair's
-    pdl_wait();
 
     // Neighbouring tiles share their rows of W: the tiles of rows run fastest.
     auto tile_of = [&](int i) {
@@ -346,10 +348,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     pair_barrier();                            // neither block leaves while the other may reach into it
+    __syncwarp();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512) : "memory");
     }
+    // neither block leaves before both have given their tensor memory back
+    __syncthreads();
+    pair_barrier();
 }
 
 // A tensor map of up to four dimensions, the strides in bytes from the second on.
@@ -390,7 +396,9 @@ int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) 
         return (int)configured;
     }
     const int most = pair_count(), pairs = args.n_tiles < most ? args.n_tiles : most;
-    thn_launch(kernel, dim3((unsigned)(2 * pairs)), kThreads, Shape<MODE>::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], args);
+    // In plain stream order, and no kernel is scheduled early behind it: a pair holds all tensor memory of two multiprocessors from its start to its end,
+    // and a long chain of such kernels and small ones, each scheduled under the one before, was seen to stop for good.
+    thn_launch_ordered(kernel, dim3((unsigned)(2 * pairs)), kThreads, Shape<MODE>::kSmemBytes, stream, maps[0], maps[1], maps[2], maps[3], args);
     return thn_launch_status("mx4_pair");
 }
 

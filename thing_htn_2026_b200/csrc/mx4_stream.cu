@@ -144,16 +144,10 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (int i = 0; i < early; ++i) load_w(i, first_tile, c0 + i);
     }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
-                     "r"(S::kTmemCols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     __syncwarp();
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    __syncwarp();
+    uint32_t tmem_base = 0;                    // of the warps of the products and the sums
     if (n_ranks > 1) cluster_arrive();         // this block has begun: the others may reach into it
 
     if (warp == 0) {
@@ -196,6 +190,16 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     } else if (warp == 1) {
         // ---- the products: the whole warp walks, one thread of it issues.  A stage's scales go to tensor memory ahead of the products of the stage
         // before it, so that they are copied under those; two sets of columns take them in turn.
+        // (Tensor memory is taken once the kernels before are done: one of them may still need it for blocks on this multiprocessor.)
+        pdl_wait();
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                     "r"(S::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        asm volatile("bar.sync 1, 160;" ::: "memory");         // the warps of the sums
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
         const bool issues = elect_one();
         auto bring_scales = [&](int s, uint32_t set) {
             const uint32_t from = smem_addr(tiles + (size_t)s * S::kStageStride) + kWSmem + S::kXSmem;
@@ -299,6 +303,10 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     } else {
         // ---- the sums: a thread has an output of the tile
         pdl_wait();
+        __syncwarp();
+        asm volatile("bar.sync 1, 160;" ::: "memory");         // tensor memory is there
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
         const int r = (warp & 3) * 32 + lane;
         bool dead = false;
         int local = 0;
@@ -382,6 +390,7 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     if (*give_up) let_copies_land();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    __syncwarp();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
