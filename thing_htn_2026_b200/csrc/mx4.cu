@@ -85,26 +85,24 @@ struct Piece<__nv_bfloat16> {
     }
 };
 
-// Pieces of eight entries: a thread takes kAhead of them, kThreads apart, and asks for all of them before it works on the first.  Bound by the
-// memory: 2,048 rows of 9,728 bfloat16 entries, which lie in the L2 cache or not.  Four threads have a block's entries, sixteen the columns of four
-// scale bytes.
-constexpr int kAhead = 4;
-
-template <typename T>
+// Pieces of eight entries: a thread takes AHEAD of them, kThreads apart, and asks for all of them before it works on the first.  Four threads have a
+// block's entries, sixteen the columns of four scale bytes.  Bound by the memory where there are many: 2,048 x 9,728 bfloat16 entries 12.5 us, 4.0
+// TB/s (one piece a thread: 19 us).
+template <int AHEAD, typename T>
 __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                 const T* __restrict__ x, uint32_t units, Mx4Divisor pieces, long long columns,
                                                                 long long padded, bool vector) {
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t first = blockIdx.x * (uint32_t)(kThreads * kAhead) + threadIdx.x;
-    Piece<T> held[kAhead];
+    const uint32_t first = blockIdx.x * (uint32_t)(kThreads * AHEAD) + threadIdx.x;
+    Piece<T> held[AHEAD];
     Mx4Place<kThreads> at(first, pieces);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a, at.step(pieces))
+    for (int a = 0; a < AHEAD; ++a, at.step(pieces))
         held[a].load(x + (long long)at.row * columns, (int)(at.piece * 8), first + a * kThreads < units ? (int)columns : 0, vector);
     at = Mx4Place<kThreads>(first, pieces);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
+    for (int a = 0; a < AHEAD; ++a, at.step(pieces)) {
         uint32_t top = held[a].top();
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -122,18 +120,18 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(uint8_t* __restr
     }
 }
 
-template <typename T>
+template <int AHEAD, typename T>
 __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes,
                                                                   const uint8_t* __restrict__ scales, uint32_t units, Mx4Divisor pieces,
                                                                   long long columns, long long padded, bool vector) {
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t first = blockIdx.x * (uint32_t)(kThreads * kAhead) + threadIdx.x;
-    uint32_t words[kAhead];
-    uint8_t bytes[kAhead];
+    const uint32_t first = blockIdx.x * (uint32_t)(kThreads * AHEAD) + threadIdx.x;
+    uint32_t words[AHEAD];
+    uint8_t bytes[AHEAD];
     Mx4Place<kThreads> at(first, pieces);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
+    for (int a = 0; a < AHEAD; ++a, at.step(pieces)) {
         if (first + a * kThreads < units) {
             words[a] = *reinterpret_cast<const uint32_t*>(codes + (long long)at.row * (padded / 2) + at.piece * 4);
             bytes[a] = scales[mx4_scale_at(at.row, at.piece / 16, padded / kMx4Atom) + (at.piece % 16) / 4];
@@ -141,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict_
     }
     at = Mx4Place<kThreads>(first, pieces);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a, at.step(pieces)) {
+    for (int a = 0; a < AHEAD; ++a, at.step(pieces)) {
         if (first + a * kThreads >= units) break;
         const long long c = (long long)at.piece * 8;
         const float s = mx4_scale(bytes[a]);
@@ -209,7 +207,7 @@ unsigned blocks_for(long long units) { return (unsigned)((units + kThreads - 1) 
 // Rows in steps of whole pieces of scales, so that a launch has fewer than 2^31 units: go(first row, rows).
 template <typename Go>
 int in_steps(long long rows, long long units_a_row, Go go) {
-    long long most = 0x7ffffff0 / units_a_row - kThreads * kAhead;
+    long long most = 0x7ffffff0 / units_a_row - kThreads * kMx4Ahead;
     most = most < 128 ? 128 : most / 128 * 128;
     for (long long row = 0; row < rows; row += most) {
         const int status = go(row, rows - row < most ? rows - row : most);
@@ -223,7 +221,9 @@ int quantize(uint8_t* codes, uint8_t* scales, const T* x, long long rows, long l
     const long long padded = mx4_padded(columns), pieces = padded / 8;
     const bool vector = ((uintptr_t)x & 15) == 0 && columns % (16 / sizeof(T)) == 0;
     return in_steps(rows, pieces, [&](long long row, long long n) {
-        thn_launch(mx4_quantize_kernel<T>, (unsigned)((n * pieces + kThreads * kAhead - 1) / (kThreads * kAhead)), kThreads, 0, stream, codes + row * (padded / 2),
+        const int ahead = mx4_ahead(n * pieces);
+        thn_launch(ahead == 1 ? mx4_quantize_kernel<1, T> : mx4_quantize_kernel<kMx4Ahead, T>,
+                   (unsigned)((n * pieces + kThreads * ahead - 1) / (kThreads * ahead)), kThreads, 0, stream, codes + row * (padded / 2),
                    scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, x + row * columns, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces), columns,
                    padded, vector);
         return thn_launch_status("mx4_quantize");
@@ -235,9 +235,11 @@ int dequantize(T* out, const uint8_t* codes, const uint8_t* scales, long long ro
     const long long padded = mx4_padded(columns), pieces = (columns + 7) / 8;
     const bool vector = ((uintptr_t)out & 15) == 0 && columns % (16 / sizeof(T)) == 0;
     return in_steps(rows, pieces, [&](long long row, long long n) {
-        thn_launch(mx4_dequantize_kernel<T>, (unsigned)((n * pieces + kThreads * kAhead - 1) / (kThreads * kAhead)), kThreads, 0, stream, out + row * columns,
-                   codes + row * (padded / 2), scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces),
-                   columns, padded, vector);
+        const int ahead = mx4_ahead(n * pieces);
+        thn_launch(ahead == 1 ? mx4_dequantize_kernel<1, T> : mx4_dequantize_kernel<kMx4Ahead, T>,
+                   (unsigned)((n * pieces + kThreads * ahead - 1) / (kThreads * ahead)), kThreads, 0, stream, out + row * columns,
+                   codes + row * (padded / 2), scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, (uint32_t)(n * pieces),
+                   Mx4Divisor((uint32_t)pieces), columns, padded, vector);
         return thn_launch_status("mx4_dequantize");
     });
 }

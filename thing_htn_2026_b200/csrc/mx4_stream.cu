@@ -400,24 +400,24 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     }
 }
 
-// Rows as terms of 8-bit floats (mx4_terms).  A thread takes eight columns of kAhead units and asks for all of them first.
-constexpr int kTermThreads = 256, kAhead = 4;
+// Rows as terms of 8-bit floats (mx4_terms).  A thread takes eight columns of AHEAD units and asks for all of them first.
+constexpr int kTermThreads = 256;
 
-template <typename RT>
+template <int AHEAD, typename RT>
 __global__ void __launch_bounds__(kTermThreads) mx4_terms_kernel(uint8_t* __restrict__ bytes, uint8_t* __restrict__ scales, const RT* __restrict__ x,
                                                                  uint32_t units, Mx4Divisor pieces, Mx4Divisor size, int pitch, int K, int padded, int plane,
                                                                  bool vector) {
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t first = blockIdx.x * (uint32_t)(kTermThreads * kAhead) + threadIdx.x;
-    Eight<RT> held[kAhead];
+    const uint32_t first = blockIdx.x * (uint32_t)(kTermThreads * AHEAD) + threadIdx.x;
+    Eight<RT> held[AHEAD];
     Mx4Place<kTermThreads> place(first, pieces);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a, place.step(pieces))
+    for (int a = 0; a < AHEAD; ++a, place.step(pieces))
         held[a].load(x + (long long)place.row * K, place.piece * 8, first + a * kTermThreads < units ? K : 0, vector);
     place = Mx4Place<kTermThreads>(first, pieces);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a, place.step(pieces)) {
+    for (int a = 0; a < AHEAD; ++a, place.step(pieces)) {
         uint32_t top = held[a].top();
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -547,14 +547,15 @@ int room_for(int M) { return M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64; }
 int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K, int plane, int size, int pitch, cudaStream_t stream) {
     const long long padded = mx4_padded(K), units = (long long)M * (padded / 8);
     THN_UNSUPPORTED_IF(units > 0x7ffff000, "mx4_terms: %d rows of %d entries are too many", M, K);
-    const unsigned blocks = (unsigned)((units + kTermThreads * kAhead - 1) / (kTermThreads * kAhead));
+    const int ahead = mx4_ahead(units);
+    const unsigned blocks = (unsigned)((units + kTermThreads * ahead - 1) / (kTermThreads * ahead));
     const bool vector = ((uintptr_t)x & 15) == 0 && K % 8 == 0;
     const Mx4Divisor pieces((uint32_t)(padded / 8)), rows((uint32_t)size);
     if (x_type == THN_F32)
-        thn_launch(mx4_terms_kernel<float>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const float*)x, (uint32_t)units, pieces, rows,
+        thn_launch(ahead == 1 ? mx4_terms_kernel<1, float> : mx4_terms_kernel<kMx4Ahead, float>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const float*)x, (uint32_t)units, pieces, rows,
                    pitch, K, (int)padded, plane, vector);
     else
-        thn_launch(mx4_terms_kernel<__nv_bfloat16>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const __nv_bfloat16*)x,
+        thn_launch(ahead == 1 ? mx4_terms_kernel<1, __nv_bfloat16> : mx4_terms_kernel<kMx4Ahead, __nv_bfloat16>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const __nv_bfloat16*)x,
                    (uint32_t)units, pieces, rows, pitch, K, (int)padded, plane, vector);
     return thn_launch_status("mx4_terms");
 }
