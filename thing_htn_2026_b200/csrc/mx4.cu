@@ -166,34 +166,39 @@ __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict_
     }
 }
 
-// Codes and scales as they are stored, row by row, into this library's layout: a thread per 128 columns of a row.
+// Codes and scales as they are stored, row by row, into this library's layout.  A thread has eight codes, sixteen the columns of four scale bytes; words:
+// the stored rows are whole aligned words.
 __global__ void __launch_bounds__(kThreads) mx4_arrange_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                const uint8_t* __restrict__ stored, const uint8_t* __restrict__ stored_scales,
-                                                               long long rows, long long columns, long long padded) {
+                                                               uint32_t units, Mx4Divisor pieces, int columns, int padded, bool words) {
     pdl_launch_dependents();
     pdl_wait();
-    const long long atoms = padded / kMx4Atom, unit = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const long long row = unit / atoms, atom = unit - row * atoms;
-    if (row >= rows) return;
-    const long long row_bytes = (columns + 1) / 2, blocks = (columns + kMx4Block - 1) / kMx4Block;
-    const uint8_t* src = stored + row * row_bytes;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(codes + row * (padded / 2) + atom * (kMx4Atom / 2));
-    for (int w = 0; w < kMx4Atom / 8; ++w) {
-        uint32_t word = 0;
+    const uint32_t unit = blockIdx.x * (uint32_t)kThreads + threadIdx.x, row = pieces.of(unit), piece = unit - row * pieces.d;
+    if (unit >= units) return;
+    const int row_bytes = (columns + 1) / 2, blocks = (columns + kMx4Block - 1) / kMx4Block;
+    const uint8_t* src = stored + (long long)row * row_bytes;
+    uint32_t word = 0;
+    if (words) {
+        if ((int)piece * 4 < row_bytes) word = *reinterpret_cast<const uint32_t*>(src + piece * 4);
+    } else {
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const long long at = atom * (kMx4Atom / 2) + w * 4 + i;
+            const int at = (int)piece * 4 + i;
             uint32_t byte = at < row_bytes ? src[at] : 0;
             if (2 * at + 1 >= columns) byte &= 15;
             word |= byte << (8 * i);
         }
-        dst[w] = word;
     }
-    uint32_t four = 0;
-    for (int i = 0; i < 4; ++i) {
-        const long long at = atom * 4 + i;
-        if (at < blocks) four |= (uint32_t)stored_scales[row * blocks + at] << (8 * i);
+    *reinterpret_cast<uint32_t*>(codes + (long long)row * (padded / 2) + piece * 4) = word;
+    if ((piece & 15) == 0) {
+        uint32_t four = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = (int)(piece >> 4) * 4 + i;
+            if (at < blocks) four |= (uint32_t)stored_scales[(long long)row * blocks + at] << (8 * i);
+        }
+        *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, piece >> 4, padded / kMx4Atom)) = four;
     }
-    *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, atom, atoms)) = four;
 }
 
 int refuse_sizes(const char* what, long long rows, long long columns) {
@@ -201,8 +206,6 @@ int refuse_sizes(const char* what, long long rows, long long columns) {
     THN_UNSUPPORTED_IF(rows > 0x7fffffff, "%s: %lld rows of %lld entries are too many", what, rows, columns);
     return THN_OK;
 }
-
-unsigned blocks_for(long long units) { return (unsigned)((units + kThreads - 1) / kThreads); }
 
 // Rows in steps of whole pieces of scales, so that a launch has fewer than 2^31 units: go(first row, rows).
 template <typename Go>
@@ -273,9 +276,12 @@ THN_API int thn_mx4_arrange(void* codes, void* scales, const void* stored, const
     const int status = refuse_sizes("mx4_arrange", rows, columns);
     if (status != THN_OK) return status;
     if (rows == 0) return THN_OK;
-    const long long padded = mx4_padded(columns);
-    THN_UNSUPPORTED_IF(rows * (padded / kMx4Atom) > (long long)0x7fffffff * kThreads, "mx4_arrange: %lld rows of %lld entries are too many", rows, columns);
-    thn_launch(mx4_arrange_kernel, blocks_for(rows * (padded / kMx4Atom)), kThreads, 0, stream, (uint8_t*)codes, (uint8_t*)scales,
-               (const uint8_t*)stored, (const uint8_t*)stored_scales, rows, columns, padded);
-    return thn_launch_status("mx4_arrange");
+    const long long padded = mx4_padded(columns), pieces = padded / 8, row_bytes = (columns + 1) / 2, blocks = (columns + kMx4Block - 1) / kMx4Block;
+    const bool words = columns % 8 == 0 && ((uintptr_t)stored & 3) == 0;
+    return in_steps(rows, pieces, [&](long long row, long long n) {
+        thn_launch(mx4_arrange_kernel, (unsigned)((n * pieces + kThreads - 1) / kThreads), kThreads, 0, stream, (uint8_t*)codes + row * (padded / 2),
+                   (uint8_t*)scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, (const uint8_t*)stored + row * row_bytes,
+                   (const uint8_t*)stored_scales + row * blocks, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces), (int)columns, (int)padded, words);
+        return thn_launch_status("mx4_arrange");
+    });
 }
