@@ -243,11 +243,55 @@ def test_refusals():
         ops.linear_mx4(x, weight, bias=torch.zeros(9, device="cuda"))
     with pytest.raises(ops.KernelError, match="CUDA"):
         ops.linear_mx4(x.cpu(), weight)
+    with pytest.raises(ops.KernelError, match="Mx4"):
+        ops.linear_mx4(x, torch.zeros((10, 64), dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ops.KernelError, match="err"):
+        ops.linear_mx4(x, weight, err=torch.zeros(1, device="cuda"))
+    with pytest.raises(ops.KernelError, match="Mx4"):
+        ops.dequantize_mx4(x)
     parts = torch.zeros((4, 32), dtype=torch.uint8, device="cuda")
     with pytest.raises(ops.KernelError, match="codes"):
         ops.mx4_from_parts(parts, torch.zeros((4, 3), dtype=torch.uint8, device="cuda"), 64)
     with pytest.raises(ops.KernelError, match="codes"):
         ops.mx4_from_parts(parts, torch.zeros((4, 2), dtype=torch.uint8, device="cuda"), 70)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 7, 20, 90])
+def test_rows_that_begin_anywhere(m, dtype):
+    """Rows and a bias whose first entry is not at a multiple of 16 bytes."""
+    n, k = 300, 512
+    weight, _ = weight_of(n, k, 7)
+    x, bias = rows_of(m, k, dtype, 8), rows_of(1, n, dtype, 9)[0]
+    shifted = torch.empty(m * k + 1, dtype=dtype, device="cuda")[1:].view(m, k).copy_(x)
+    moved = torch.empty(n + 1, dtype=dtype, device="cuda")[1:].copy_(bias)
+    assert shifted.data_ptr() % 16 and shifted.is_contiguous()
+    assert torch.equal(ops.linear_mx4(shifted, weight, bias=moved), ops.linear_mx4(x, weight, bias=bias))
+    a, b = ops.quantize_mx4(shifted), ops.quantize_mx4(x)
+    assert torch.equal(a.codes, b.codes) and np.array_equal(scale_bytes(a), scale_bytes(b))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 2560, 9728), (8, 6144, 2560), (40, 2560, 4096), (300, 1000, 1000)])
+@pytest.mark.parametrize("quantized", [False, True])
+def test_the_same_call_gives_the_same_bits(m, n, k, quantized):
+    weight, _ = weight_of(n, k, 1)
+    x = rows_of(m, k, torch.bfloat16, 2)
+    given = ops.quantize_mx4(x) if quantized else x
+    first = ops.linear_mx4(given, weight, out_dtype=torch.float32)
+    for _ in range(20):
+        assert torch.equal(ops.linear_mx4(given, weight, out_dtype=torch.float32), first)
+
+
+def test_a_matrix_from_its_bytes():
+    weight, _ = weight_of(130, 200, 3)
+    again = ops.Mx4(weight.data.clone(), 130, 200)
+    assert torch.equal(ops.dequantize_mx4(again), ops.dequantize_mx4(weight)) and again.nbytes == weight.nbytes
+    for data, rows in ((weight.data[:-1], 130), (weight.data, 257), (weight.data.view(2, -1), 130), (weight.data.view(torch.int8), 130),
+                       (weight.data.cpu(), 130)):
+        with pytest.raises(ops.KernelError, match="Mx4"):
+            ops.Mx4(data, rows, 200)
+    with pytest.raises(ops.KernelError, match="Mx4"):
+        ops.Mx4(torch.zeros(weight.nbytes + 1, dtype=torch.uint8, device="cuda")[1:], 130, 200)
 
 
 def test_another_stream_and_a_recorded_graph():

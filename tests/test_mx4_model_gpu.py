@@ -114,6 +114,14 @@ def test_generation_with_and_without_graphs_gives_the_same_tokens(activations):
 
 
 @pytest.mark.gpu
+def test_a_model_that_holds_4_bits_already_takes_the_choice_of_rows():
+    first = engine_of("tiny-a", "float32", weights="mx4")
+    held = [first.model.layers[0].mixer.w_qkv, first.model.layers[0].ffn.w_down]
+    second = Engine(None, dtype="float32", model=first.model, max_tokens=1024, max_batch=4, weights="mx4", activations="mx4")
+    assert second.model.layers[0].mixer.w_qkv is held[0] and all(w.quantizes_rows for w in held)
+
+
+@pytest.mark.gpu
 def test_from_the_command_line():
     done = subprocess.run([sys.executable, "-m", "thing_htn_2026_b200", "generate", "--random-config", "tiny-a", "--prompt-lens", "5,17",
                            "--max-new-tokens", "4", "--weights", "mx4", "--activations", "mx4"], cwd=ROOT, capture_output=True, text=True, timeout=600)
@@ -123,6 +131,17 @@ def test_from_the_command_line():
     from thing_htn_2026_b200 import cli
     steps = list(engine.generate(cli.make_prompts_of([5, 17], engine.model.vocab_size, 0), 4))
     assert [p["tokens"] for p in printed] == [[s[j] for s in steps] for j in range(2)]
+
+
+def test_tensors_on_the_cpu_are_refused():
+    with pytest.raises(ops.KernelError, match="CUDA only"):
+        ops.quantize_mx4(torch.zeros(2, 64))
+    with pytest.raises(ops.KernelError, match="CUDA only"):
+        ops.mx4_from_parts(torch.zeros((2, 32), dtype=torch.uint8), torch.zeros((2, 2), dtype=torch.uint8), 64)
+    with pytest.raises(ops.KernelError, match="CUDA only"):
+        ops.Mx4(torch.zeros(768, dtype=torch.uint8), 4, 64)
+    with pytest.raises(ops.KernelError, match="Mx4"):
+        ops.linear_mx4(torch.zeros(2, 64), torch.zeros(3, 64))
 
 
 def test_refused_choices():

@@ -1011,14 +1011,17 @@ class Mx4:
     __slots__ = ("data", "rows", "columns", "code_bytes", "quantizes_rows")
 
     def __init__(self, data: torch.Tensor, rows: int, columns: int, quantizes_rows: bool = False):
-        self.data, self.rows, self.columns, self.quantizes_rows = data, rows, columns, quantizes_rows
-        self.code_bytes = rows * (-(-columns // 128) * 64)
+        _need(data, "Mx4 data", torch.uint8)
+        rows, columns = int(rows), int(columns)
+        if rows < 0 or columns < 1 or data.dim() != 1 or data.shape[0] != _mx4_bytes(rows, columns) or data.data_ptr() % 32:
+            raise KernelError(f"Mx4: {tuple(data.shape)} bytes at a multiple of {data.data_ptr() & -data.data_ptr()} for {rows} rows of {columns} "
+                              f"columns: {_mx4_bytes(rows, columns)} bytes at a multiple of 32, please")
+        self._set(data, rows, columns, quantizes_rows)
 
-    @classmethod
-    def empty(cls, like: torch.Tensor, rows: int, columns: int) -> "Mx4":
-        """Room for a matrix on the device of ``like``."""
-        atoms = -(-columns // 128)
-        return cls(like.new_empty((rows * 64 + (-(-rows // 128)) * 512) * atoms, dtype=torch.uint8), rows, columns)
+    def _set(self, data: torch.Tensor, rows: int, columns: int, quantizes_rows: bool = False) -> "Mx4":
+        self.data, self.rows, self.columns, self.quantizes_rows = data, rows, columns, quantizes_rows
+        self.code_bytes = rows * ((columns + 127) // 128 * 64)
+        return self
 
     @property
     def codes(self) -> torch.Tensor:
@@ -1051,6 +1054,10 @@ class Mx4:
 # the host.)
 
 
+def _mx4_bytes(rows: int, columns: int) -> int:
+    return (rows * 64 + (rows + 127) // 128 * 512) * ((columns + 127) // 128)
+
+
 def _mx4_stream_for(t: torch.Tensor, what: str) -> int:
     """The current stream, which must be one of the tensor's device."""
     device = t.get_device()
@@ -1070,11 +1077,10 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
     code = _code(x, "quantize_mx4 x")
     stream = _mx4_stream_for(x, "quantize_mx4 x")
     rows, columns = shape
-    atoms = (columns + 127) // 128
-    data = x.new_empty(((rows * 64 + (rows + 127) // 128 * 512) * atoms,), dtype=torch.uint8)
-    at = data.data_ptr()
-    _call("thn_mx4_quantize", at, at + rows * atoms * 64, x.data_ptr(), rows, columns, code, stream)
-    return Mx4(data, rows, columns)
+    out = Mx4.__new__(Mx4)._set(x.new_empty((_mx4_bytes(rows, columns),), dtype=torch.uint8), rows, columns)
+    codes, scales = out._pointers()
+    _call("thn_mx4_quantize", codes, scales, x.data_ptr(), rows, columns, code, stream)
+    return out
 
 
 def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> Mx4:
@@ -1089,7 +1095,7 @@ def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> M
     if scales.device != codes.device:
         raise KernelError(f"mx4_from_parts: codes on {codes.device}, scales on {scales.device}")
     stream = _mx4_stream_for(codes, "mx4_from_parts codes")
-    out = Mx4.empty(codes, rows, columns)
+    out = Mx4.__new__(Mx4)._set(codes.new_empty((_mx4_bytes(rows, columns),)), rows, columns)
     to_codes, to_scales = out._pointers()
     _call("thn_mx4_arrange", to_codes, to_scales, codes.data_ptr(), scales.data_ptr(), rows, columns, stream)
     return out
@@ -1098,6 +1104,8 @@ def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> M
 def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The numbers ``[rows, columns]`` that ``q`` stands for, in float32 or bfloat16; both hold them exactly."""
     code = DTYPE_CODE.get(dtype)
+    if q.__class__ is not Mx4:
+        raise KernelError(f"dequantize_mx4: an Mx4, please, not {type(q).__name__}")
     if code is None:
         raise KernelError(f"dequantize_mx4: dtype {dtype} is not supported (float32 or bfloat16)")
     data = q.data
@@ -1125,7 +1133,10 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     """``x [M, K] @ weight[N, K]^T`` (+ ``bias [N]``) with a weight in 4 bits: float32 sums, one rounding to ``out_dtype`` (bfloat16 or
     float32).  ``x`` is a tensor in bfloat16 or float32, which is multiplied as it is and whose type is the default
     ``out_dtype``, or an :class:`Mx4` (default: bfloat16).  A row of ``x`` that holds an infinity or a NaN comes out as NaN, and so does the
-    column of a weight row that does.  ``err``: the step's device error word for the kernel's bounded waits."""
+    column of a weight row that does.  ``err``: the step's device error word for the kernel's bounded waits (what a wait that gave up
+    leaves is NaN in any case)."""
+    if weight.__class__ is not Mx4:
+        raise KernelError(f"linear_mx4: a weight in 4 bits (Mx4), please, not {type(weight).__name__}")
     if x.__class__ is Mx4:
         kind, data, m, k = 2, x.data, x.rows, x.columns
         at = data.data_ptr()

@@ -107,6 +107,9 @@ class Block:
                     quantized.quantizes_rows = bool(quantize_rows)
                     setattr(part, name, quantized)
                     count += 1
+                elif isinstance(weight, ops.Mx4):
+                    weight.quantizes_rows = bool(quantize_rows)
+                    count += 1
         return count
 
     def step_inputs(self, batch: HostBatch, out: Dict[str, List[int]]) -> None:
