@@ -330,6 +330,58 @@ def test_another_stream_and_a_recorded_graph():
             assert torch.equal(outs[i][0], want[i]) and torch.equal(outs[i][1], want[2 + i])
 
 
+@pytest.mark.parametrize("m", [1, 8, 40, 100])
+def test_a_weight_that_was_written_just_before(m):
+    """Quantised, brought back, or taken from its parts by the kernel ahead of the product that reads it, again and again in the same memory."""
+    n, k, count = 19000, 2560, 12
+    g = torch.Generator(device="cuda").manual_seed(1)
+    source = [torch.randn((n, k), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    parts = [(torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8),
+              torch.randint(118, 127, (n, k // 32), generator=g, device="cuda", dtype=torch.uint8)) for _ in range(2)]
+    x = rows_of(m, k, torch.bfloat16, 2)
+    makes = [lambda i: ops.quantize_mx4(source[i]), lambda i: ops.mx4_from_parts(*parts[i], k)]
+    for make in makes:
+        held = [make(i) for i in range(2)]
+        torch.cuda.synchronize()
+        want = [ops.linear_mx4(x, w) for w in held]
+        torch.cuda.synchronize()
+        got = [ops.linear_mx4(x, make(i % 2)) for i in range(count)]
+        got += [ops.linear_mx4(ops.quantize_mx4(x), make(i % 2)) for i in range(count)]
+        rows = ops.linear_mx4(ops.quantize_mx4(x), held[0]), ops.linear_mx4(ops.quantize_mx4(x), held[1])
+        for i in range(count):
+            assert torch.equal(got[i], want[i % 2]) and torch.equal(got[count + i], rows[i % 2])
+    held = [ops.quantize_mx4(s) for s in source]
+    back = [ops.dequantize_mx4(w, torch.bfloat16) for w in held]
+    torch.cuda.synchronize()
+    want = [ops.linear(x, w) for w in back]
+    torch.cuda.synchronize()
+    del back
+    got = [ops.linear(x, ops.dequantize_mx4(held[i % 2], torch.bfloat16)) for i in range(count)]
+    assert all(torch.equal(got[i], want[i % 2]) for i in range(count))
+
+
+def test_two_streams_at_once():
+    """The same weight multiplied on two streams whose calls overlap: few rows, many rows and quantised rows."""
+    weight, _ = weight_of(4000, 2048, 5)
+    inputs = [rows_of(m, 2048, dtype, m) for m, dtype in ((1, torch.bfloat16), (6, torch.float32), (30, torch.bfloat16), (260, torch.bfloat16),
+                                                         (100, torch.float32))]
+
+    def all_products():
+        return [ops.linear_mx4(x, weight) for x in inputs] + [ops.linear_mx4(ops.quantize_mx4(x), weight) for x in inputs]
+
+    want = all_products()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append(all_products())
+    torch.cuda.synchronize()
+    for products in got:
+        assert all(torch.equal(a, b) for a, b in zip(products, want))
+
+
 @pytest.mark.parametrize("m,entry", [(5, "thn_mx4_stream"), (60, "thn_mx4_stream"), (200, "thn_mx4_pair")])
 @pytest.mark.parametrize("quantized", [False, True])
 def test_a_wait_that_runs_out_is_reported(m, entry, quantized):

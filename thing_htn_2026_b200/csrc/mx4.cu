@@ -4,6 +4,10 @@
 // less, where the scale is already the smallest), and an entry's code is that of the nearest magnitude to |x| 2^(127 - b), of two
 // equally near ones the even code, and 6 above 6.  All of it is exact but that one rounding: the scale is a power of two.  A
 // block that holds an infinity or a NaN gets the scale byte 255 and codes of zero.
+//
+// What these kernels write may be the next product's weight, which a product reads while the kernels before it still run.  So
+// they let no later kernel be scheduled ahead of their end, and a kernel that begins after their end has all that they wrote; but
+// for rows that are quantised to be multiplied (early), which a product reads after its wait.
 #include "mx4.cuh"
 
 namespace {
@@ -91,8 +95,8 @@ struct Piece<__nv_bfloat16> {
 template <int AHEAD, typename T>
 __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                 const T* __restrict__ x, uint32_t units, Mx4Divisor pieces, long long columns,
-                                                                long long padded, bool vector) {
-    pdl_launch_dependents();
+                                                                long long padded, bool vector, bool early) {
+    if (early) pdl_launch_dependents();
     pdl_wait();
     const uint32_t first = blockIdx.x * (uint32_t)(kThreads * AHEAD) + threadIdx.x;
     Piece<T> held[AHEAD];
@@ -124,7 +128,6 @@ template <int AHEAD, typename T>
 __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict__ out, const uint8_t* __restrict__ codes,
                                                                   const uint8_t* __restrict__ scales, uint32_t units, Mx4Divisor pieces,
                                                                   long long columns, long long padded, bool vector) {
-    pdl_launch_dependents();
     pdl_wait();
     const uint32_t first = blockIdx.x * (uint32_t)(kThreads * AHEAD) + threadIdx.x;
     uint32_t words[AHEAD];
@@ -171,7 +174,6 @@ __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict_
 __global__ void __launch_bounds__(kThreads) mx4_arrange_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                const uint8_t* __restrict__ stored, const uint8_t* __restrict__ stored_scales,
                                                                uint32_t units, Mx4Divisor pieces, int columns, int padded, bool words) {
-    pdl_launch_dependents();
     pdl_wait();
     const uint32_t unit = blockIdx.x * (uint32_t)kThreads + threadIdx.x, row = pieces.of(unit), piece = unit - row * pieces.d;
     if (unit >= units) return;
@@ -220,7 +222,7 @@ int in_steps(long long rows, long long units_a_row, Go go) {
 }
 
 template <typename T>
-int quantize(uint8_t* codes, uint8_t* scales, const T* x, long long rows, long long columns, cudaStream_t stream) {
+int quantize(uint8_t* codes, uint8_t* scales, const T* x, long long rows, long long columns, bool early, cudaStream_t stream) {
     const long long padded = mx4_padded(columns), pieces = padded / 8;
     const bool vector = ((uintptr_t)x & 15) == 0 && columns % (16 / sizeof(T)) == 0;
     return in_steps(rows, pieces, [&](long long row, long long n) {
@@ -228,7 +230,7 @@ int quantize(uint8_t* codes, uint8_t* scales, const T* x, long long rows, long l
         thn_launch(ahead == 1 ? mx4_quantize_kernel<1, T> : mx4_quantize_kernel<kMx4Ahead, T>,
                    (unsigned)((n * pieces + kThreads * ahead - 1) / (kThreads * ahead)), kThreads, 0, stream, codes + row * (padded / 2),
                    scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, x + row * columns, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces), columns,
-                   padded, vector);
+                   padded, vector, early);
         return thn_launch_status("mx4_quantize");
     });
 }
@@ -249,14 +251,15 @@ int dequantize(T* out, const uint8_t* codes, const uint8_t* scales, long long ro
 
 }  // namespace
 
-// x [rows, columns] of dtype -> codes and scales (mx4.cuh).  codes and scales 16-byte aligned.
-THN_API int thn_mx4_quantize(void* codes, void* scales, const void* x, long long rows, long long columns, int dtype, cudaStream_t stream) {
+// x [rows, columns] of dtype -> codes and scales (mx4.cuh).  codes and scales 16-byte aligned.  early: what they become is never read as a weight.
+THN_API int thn_mx4_quantize(void* codes, void* scales, const void* x, long long rows, long long columns, int dtype, int early,
+                             cudaStream_t stream) {
     const int status = refuse_sizes("mx4_quantize", rows, columns);
     if (status != THN_OK) return status;
     THN_CHECK_ARG(dtype == THN_F32 || dtype == THN_BF16, "mx4_quantize: unknown dtype %d", dtype);
     if (rows == 0) return THN_OK;
-    return dtype == THN_F32 ? quantize((uint8_t*)codes, (uint8_t*)scales, (const float*)x, rows, columns, stream)
-                            : quantize((uint8_t*)codes, (uint8_t*)scales, (const __nv_bfloat16*)x, rows, columns, stream);
+    return dtype == THN_F32 ? quantize((uint8_t*)codes, (uint8_t*)scales, (const float*)x, rows, columns, early != 0, stream)
+                            : quantize((uint8_t*)codes, (uint8_t*)scales, (const __nv_bfloat16*)x, rows, columns, early != 0, stream);
 }
 
 // out [rows, columns] of dtype: what codes and scales stand for.

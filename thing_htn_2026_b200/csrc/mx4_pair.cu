@@ -211,11 +211,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                 unsigned char* scales = dst + S::kASmem + S::kT * S::kBSmem;
                 const uint32_t bar = leader_full + s * (uint32_t)sizeof(uint64_t);
                 if (issues) {
-                if (rank == 0) mbar_expect_tx(full + s, 2 * kBytes);
-                load_box(dst, &map_w, bar, kb * 128, a_row);           // (bytes of codes, or entries)
-                load_box(dst + S::kASmem, &map_x, bar, kb * 128, b_row, 0);
-                load_box(scales, &map_w_scales, bar, 0, kb * S::kSteps, a_row >> 7, 0);
-                load_box(scales + S::kSteps * kMx4AtomBytes, &map_x_scales, bar, 0, kb * S::kSteps, t.x_row >> 7, 0);
+                    if (rank == 0) mbar_expect_tx(full + s, 2 * kBytes);
+                    load_box(dst, &map_w, bar, kb * 128, a_row);           // (bytes of codes, or entries)
+                    load_box(dst + S::kASmem, &map_x, bar, kb * 128, b_row, 0);
+                    load_box(scales, &map_w_scales, bar, 0, kb * S::kSteps, a_row >> 7, 0);
+                    load_box(scales + S::kSteps * kMx4AtomBytes, &map_x_scales, bar, 0, kb * S::kSteps, t.x_row >> 7, 0);
                 }
                 __syncwarp();
             }
@@ -430,7 +430,8 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
 // How M rows are cut into tiles by N outputs: the size (a multiple of 32) with which the pairs' rounds take the least time, a stage of a tile counted
 // with 4 clocks a column (rows in 4 bits: 2), the products' time, but 500 at least, which its thread takes to issue them; the rows of x's operand from one tile to the
 // next.  Terms are written by a kernel of this library, which begins every tile at a whole piece of 128 rows of scales; rows in 4 bits lie as they
-// do, and their tiles begin at multiples of 64.  (2,048 rows by 2,560 outputs are 130 tiles of 160 rows, two rounds, or 110 of 192, two rounds.)
+// do, and their tiles begin at multiples of 64.  (2,048 rows by 2,560 outputs are 130 tiles of 160 rows and not 110 of 192: two rounds of 74 pairs
+// either way.)
 struct RowCuts {
     int cuts, size, pitch;
 };

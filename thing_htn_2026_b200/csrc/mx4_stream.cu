@@ -11,10 +11,12 @@
 //    memory and are added in ascending order: no scratch memory, no counters, the same result every time.  More tiles: a block
 //    alone walks several, and brings the next one's while the last one's sums are stored.
 //  * Two blocks a multiprocessor while the rows are few: the bytes in flight cover the memory's latency.
+//  * W of the first stages is asked for while the kernels before still run; those that write a weight in this form (mx4.cu) let nothing run ahead of
+//    their end.
 //
 // Every wait on an mbarrier is bounded: after kWaitLimitNs the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, the
 // block's partial sums become NaN, and tensor memory is given back.  No wait depends on another block.
-#include <array>
+#include <atomic>
 
 #include "mx4_tcgen05.cuh"
 
@@ -444,13 +446,9 @@ __global__ void __launch_bounds__(kTermThreads) mx4_terms_kernel(uint8_t* __rest
 // Clusters of `c` blocks that are resident together, `blocks` a multiprocessor.
 template <typename S, typename Kernel>
 int resident_clusters(Kernel kernel, int c, int blocks) {
-    static std::array<int, 2 * (kMaxCluster + 1)> held = [] {
-        std::array<int, 2 * (kMaxCluster + 1)> n;
-        n.fill(-1);
-        return n;
-    }();
-    int& n = held[(blocks - 1) * (kMaxCluster + 1) + c];
-    if (n < 0) {
+    static std::atomic<int> held[2][kMaxCluster + 1];      // one more than the number; 0: not asked for yet
+    std::atomic<int>& n = held[blocks - 1][c];
+    if (n == 0) {
         cudaLaunchConfig_t config = {};
         config.gridDim = dim3((unsigned)(c * 512));
         config.blockDim = dim3(S::kThreads);
@@ -467,9 +465,9 @@ int resident_clusters(Kernel kernel, int c, int blocks) {
             cudaGetLastError();
             found = 0;
         }
-        n = found;
+        n = found + 1;
     }
-    return n;
+    return n - 1;
 }
 
 // How a weight is cut: blocks of a cluster, and blocks a multiprocessor.

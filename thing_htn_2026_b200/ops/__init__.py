@@ -149,7 +149,7 @@ _SIGNATURES = {
                                    c_int, c_int, c_int, c_void_p],
     "thn_delta_decode": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p],
-    "thn_mx4_quantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
+    "thn_mx4_quantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_int, c_void_p],
     "thn_mx4_dequantize": [c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_void_p],
     "thn_mx4_arrange": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p],
     "thn_mx4_pair_scratch": [c_int, c_int, c_int, c_int, c_void_p],
@@ -942,7 +942,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     in the vendor product's epilogue (float32, before the one rounding), or by a kernel of its own
     after the FFMA product.  ``weight`` may be an :class:`Mx4` (:func:`linear_mx4`)."""
     if isinstance(weight, Mx4):
-        return linear_mx4(quantize_mx4(x) if weight.quantizes_rows else x, weight, out_dtype or x.dtype, err, bias)
+        return linear_mx4(_quantize_mx4(x, early=True) if weight.quantizes_rows else x, weight, out_dtype or x.dtype, err, bias)
     if bias is not None:
         _need(bias, "linear bias", x.dtype)
         if bias.shape[0] != weight.shape[0]:
@@ -1066,10 +1066,9 @@ def _mx4_stream_for(t: torch.Tensor, what: str) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-def quantize_mx4(x: torch.Tensor) -> Mx4:
-    """``x [rows, columns]`` (bfloat16 or float32) in microscaled 4-bit floating point.  A block's scale is
-    ``2^(floor(log2 max|x|) - 2)``, at least 2^-127, and an entry becomes the nearest magnitude, of two equally near ones that with
-    the even code; what lies above 6 scales becomes 6.  A block that holds an infinity or a NaN is not a number as a whole."""
+def _quantize_mx4(x: torch.Tensor, early: bool) -> Mx4:
+    """``early``: the kernel after this one may be scheduled while it runs; only for rows that are multiplied by a weight, since a product
+    reads its weight while the kernels before it are still at work."""
     _need(x, "quantize_mx4 x")
     shape = x.shape
     if len(shape) != 2 or shape[1] < 1:
@@ -1079,8 +1078,15 @@ def quantize_mx4(x: torch.Tensor) -> Mx4:
     rows, columns = shape
     out = Mx4.__new__(Mx4)._set(x.new_empty((_mx4_bytes(rows, columns),), dtype=torch.uint8), rows, columns)
     codes, scales = out._pointers()
-    _call("thn_mx4_quantize", codes, scales, x.data_ptr(), rows, columns, code, stream)
+    _call("thn_mx4_quantize", codes, scales, x.data_ptr(), rows, columns, code, int(early), stream)
     return out
+
+
+def quantize_mx4(x: torch.Tensor) -> Mx4:
+    """``x [rows, columns]`` (bfloat16 or float32) in microscaled 4-bit floating point.  A block's scale is
+    ``2^(floor(log2 max|x|) - 2)``, at least 2^-127, and an entry becomes the nearest magnitude, of two equally near ones that with
+    the even code; what lies above 6 scales becomes 6.  A block that holds an infinity or a NaN is not a number as a whole."""
+    return _quantize_mx4(x, early=False)
 
 
 def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> Mx4:
@@ -1102,7 +1108,8 @@ def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> M
 
 
 def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """The numbers ``[rows, columns]`` that ``q`` stands for, in float32 or bfloat16; both hold them exactly."""
+    """The numbers ``[rows, columns]`` that ``q`` stands for, in float32 or bfloat16.  Both hold them exactly, but for what stored scales of 2^126
+    and 2^127 bring past their largest number: an infinity."""
     code = DTYPE_CODE.get(dtype)
     if q.__class__ is not Mx4:
         raise KernelError(f"dequantize_mx4: an Mx4, please, not {type(q).__name__}")
@@ -1169,6 +1176,8 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
         bias_at, bias_code = bias.data_ptr(), _code(bias, "linear_mx4 bias")
     if err is not None:
         _need(err, "linear_mx4 err", torch.int32)
+        if err.get_device() != data.get_device():
+            raise KernelError(f"linear_mx4: an error word on {err.device} for x on {data.device}")
     out = data.new_empty((m, n), dtype=out_dtype)
     if m == 0 or n == 0:
         return out
