@@ -47,7 +47,7 @@ struct Mx4Divisor {
     __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(n, m) + n) >> l; }
 };
 
-// Row and piece of a unit of eight entries, and of those STEP further on.
+// Row and piece of a unit, so many neighbouring entries, and of those STEP further on.
 template <uint32_t STEP>
 struct Mx4Place {
     uint32_t row, piece;
@@ -66,8 +66,3 @@ struct Mx4Place {
         }
     }
 };
-
-// How many units of eight entries a thread takes: one where there are few, for the latency (nine rows of 9,728 to terms, ahead of their product by 2,560
-// outputs: 8.2 us together, 9.7 with four), four where there are enough for every multiprocessor's threads, for the loads under way.
-constexpr int kMx4Ahead = 4;
-inline int mx4_ahead(long long units) { return units < 148 * 1024 ? 1 : kMx4Ahead; }
