@@ -402,48 +402,42 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     }
 }
 
-// Rows as terms of 8-bit floats (mx4_terms).  A thread takes eight columns of AHEAD units and asks for all of them first.
-constexpr int kTermThreads = 256;
-// One unit a thread where there are few, for the latency (nine rows of 9,728 to terms, ahead of their product by 2,560 outputs: 8.2 us together, 9.7 with
-// four), four where there are enough for every multiprocessor's threads, for the loads under way.
-constexpr int kTermAhead = 4;
+// Rows as terms of 8-bit floats (mx4_terms).  A thread takes sixteen columns; two of them have a block's, eight the columns of four scale bytes.  2,048 rows of
+// 9,728 bfloat16 entries 15.3 us (eight columns a thread: 22.4; two units a thread: 15.7).
+constexpr int kTermThreads = 256, kTermEntries = 16;
 
-template <int AHEAD, typename RT>
+template <typename RT>
 __global__ void __launch_bounds__(kTermThreads) mx4_terms_kernel(uint8_t* __restrict__ bytes, uint8_t* __restrict__ scales, const RT* __restrict__ x,
                                                                  uint32_t units, Mx4Divisor pieces, Mx4Divisor size, int pitch, int K, int padded, int plane,
                                                                  bool vector) {
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t first = blockIdx.x * (uint32_t)(kTermThreads * AHEAD) + threadIdx.x;
-    Eight<RT> held[AHEAD];
-    Mx4Place<kTermThreads> place(first, pieces);
+    const uint32_t unit = blockIdx.x * (uint32_t)kTermThreads + threadIdx.x;
+    const uint32_t from = pieces.of(unit), piece = unit - from * pieces.d;
+    Eight<RT> held[2];
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a, place.step(pieces))
-        held[a].load(x + (long long)place.row * K, place.piece * 8, first + a * kTermThreads < units ? K : 0, vector);
-    place = Mx4Place<kTermThreads>(first, pieces);
+    for (int h = 0; h < 2; ++h) held[h].load(x + (long long)from * K, piece * kTermEntries + 8 * h, unit < units ? K : 0, vector);
+    uint32_t top = max(held[0].top(), held[1].top());
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const uint32_t b = row_scale_byte(top);
+    // the eight threads' four scale bytes of the first term as one word
+    uint32_t four = b << (8 * ((threadIdx.x >> 1) & 3));
+    four |= __shfl_xor_sync(0xffffffffu, four, 2);
+    four |= __shfl_xor_sync(0xffffffffu, four, 4);
+    if (unit >= units) return;
+    const uint32_t tile = size.of(from), row = tile * pitch + (from - tile * size.d);
+    uint2 low[kTerms<RT>];
+    held[0].terms(b, [&](int term, uint2 v) { low[term] = v; });
+    held[1].terms(b, [&](int term, uint2 v) {
+        const long long at = (long long)term * plane + row;
+        *reinterpret_cast<uint4*>(bytes + at * padded + piece * kTermEntries) = make_uint4(low[term].x, low[term].y, v.x, v.y);
+        if ((threadIdx.x & 7) == 0) {
+            uint32_t w = 0;
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a, place.step(pieces)) {
-        uint32_t top = held[a].top();
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t b = row_scale_byte(top);
-        // the sixteen threads' four scale bytes of the first term as one word
-        uint32_t four = b << (8 * ((threadIdx.x >> 2) & 3));
-        four |= __shfl_xor_sync(0xffffffffu, four, 4);
-        four |= __shfl_xor_sync(0xffffffffu, four, 8);
-        if (first + a * kTermThreads >= units) continue;
-        const uint32_t tile = size.of(place.row), row = tile * pitch + (place.row - tile * size.d);
-        held[a].terms(b, [&](int term, uint2 v) {
-            const long long at = (long long)term * plane + row;
-            *reinterpret_cast<uint2*>(bytes + at * padded + place.piece * 8) = v;
-            if ((threadIdx.x & 15) == 0) {
-                uint32_t w = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w |= term_scale_byte(four >> (8 * i) & 255, term) << (8 * i);
-                *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(at, place.piece / 16, padded / kMx4Atom)) = w;
-            }
-        });
-    }
+            for (int i = 0; i < 4; ++i) w |= term_scale_byte(four >> (8 * i) & 255, term) << (8 * i);
+            *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(at, piece / 8, padded / kMx4Atom)) = w;
+        }
+    });
 }
 
 // Clusters of `c` blocks that are resident together, `blocks` a multiprocessor.
@@ -546,18 +540,17 @@ int room_for(int M) { return M <= 8 ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64; }
 }  // namespace
 
 int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K, int plane, int size, int pitch, cudaStream_t stream) {
-    const long long padded = mx4_padded(K), units = (long long)M * (padded / 8);
+    const long long padded = mx4_padded(K), units = (long long)M * (padded / kTermEntries);
     THN_UNSUPPORTED_IF(units > 0x7ffff000, "mx4_terms: %d rows of %d entries are too many", M, K);
-    const int ahead = units < 148 * 1024 ? 1 : kTermAhead;
-    const unsigned blocks = (unsigned)((units + kTermThreads * ahead - 1) / (kTermThreads * ahead));
+    const unsigned blocks = (unsigned)((units + kTermThreads - 1) / kTermThreads);
     const bool vector = ((uintptr_t)x & 15) == 0 && K % 8 == 0;
-    const Mx4Divisor pieces((uint32_t)(padded / 8)), rows((uint32_t)size);
+    const Mx4Divisor pieces((uint32_t)(padded / kTermEntries)), rows((uint32_t)size);
     if (x_type == THN_F32)
-        thn_launch(ahead == 1 ? mx4_terms_kernel<1, float> : mx4_terms_kernel<kTermAhead, float>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes,
-                   (uint8_t*)scales, (const float*)x, (uint32_t)units, pieces, rows, pitch, K, (int)padded, plane, vector);
+        thn_launch(mx4_terms_kernel<float>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const float*)x, (uint32_t)units, pieces, rows,
+                   pitch, K, (int)padded, plane, vector);
     else
-        thn_launch(ahead == 1 ? mx4_terms_kernel<1, __nv_bfloat16> : mx4_terms_kernel<kTermAhead, __nv_bfloat16>, blocks, kTermThreads, 0, stream,
-                   (uint8_t*)bytes, (uint8_t*)scales, (const __nv_bfloat16*)x, (uint32_t)units, pieces, rows, pitch, K, (int)padded, plane, vector);
+        thn_launch(mx4_terms_kernel<__nv_bfloat16>, blocks, kTermThreads, 0, stream, (uint8_t*)bytes, (uint8_t*)scales, (const __nv_bfloat16*)x,
+                   (uint32_t)units, pieces, rows, pitch, K, (int)padded, plane, vector);
     return thn_launch_status("mx4_terms");
 }
 
