@@ -185,6 +185,20 @@ def test_product_of_many_pieces_of_k_a_block(m, n, k, dtype):
     check_product(m, n, k, dtype, dtype, quantized=True)
 
 
+@pytest.mark.parametrize("k", [1000, 4096, 12288])
+@pytest.mark.parametrize("m", [3, 8, 32, 33, 100, 300])
+def test_float32_rows_are_summed_as_in_float32(m, k):
+    """The error's root mean square is at most that of products added one after the other in float32: with both signs the partial sum
+    after i of K grows as sqrt(i / K) of the result, and each addition is off by 2^-24 / sqrt(3) of it in the mean, so sqrt(K / 6) 2^-24 of the
+    result's."""
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    x = torch.randn((m, k), generator=g, device="cuda")
+    weight, w = weight_of(1024, k, k)
+    y = x.double() @ w.t()
+    error = ops.linear_mx4(x, weight).double() - y
+    assert error.norm() <= (k / 6) ** 0.5 * 2.0 ** -24 * y.norm()
+
+
 @pytest.mark.parametrize("spread", [2.0 ** -60, 2.0 ** 60])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m", [3, 150])

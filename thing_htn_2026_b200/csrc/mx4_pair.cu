@@ -26,7 +26,11 @@ constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;      // w
 template <int MODE>
 struct Shape {
     static constexpr int kT = MODE == kQuantized ? 1 : MODE == kRows2 ? 2 : 6;
-    static constexpr int kCols = 192, kBuffers = 2;                          // columns of an accumulator; accumulators
+    static constexpr int kCols = 192;                                        // of an accumulator
+    // Accumulators of a tile, and tiles that are held at once.  The tensor core cuts a sum's last bits off at every step of 32 columns, and six terms in one
+    // accumulator would be six times as many cuts: 300 float32 rows, K = 4,096: 6.8e-6 off in relation to the result, 1.1e-6 for products
+    // added one after the other in float32.  So float32's first terms have an accumulator of their own.
+    static constexpr int kSums = MODE == kRows6 ? 2 : 1, kBuffers = 2 / kSums;
     static constexpr int kSteps = MODE == kQuantized ? 2 : 1;                // pieces of 128 columns of the sum that a stage holds
     static constexpr int kAtoms = (kCols + 64 + 127) / 128;                  // of scales that a tile's rows of x can touch
     static constexpr uint32_t kASmem = 128 * 128, kBSmem = kCols / 2 * 128;  // of one block, a term
@@ -35,7 +39,7 @@ struct Shape {
     static constexpr int kFit = (int)((226 * 1024 - 2048) / kStageStride);
     static constexpr int kStages = kFit < 8 ? kFit : 8;
     static constexpr size_t kSmemBytes = kStages * kStageStride + 1024 /* alignment */ + 512 /* barriers */;
-    static constexpr uint32_t kScaleCol = kCols * kBuffers;                  // W's scales, then x's
+    static constexpr uint32_t kScaleCol = kCols * kSums * kBuffers;          // W's scales, then x's
     static constexpr uint32_t kScaleCols = kSteps * 4 * (1 + kT * kAtoms);   // of a stage; two stages' in turn
     static_assert(kScaleCol + 2 * kScaleCols <= 512, "tensor memory");
     static_assert(kStages >= 2, "shared memory");
@@ -249,7 +253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
             const int buf = local % S::kBuffers;
             ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, ((local / S::kBuffers) & 1) ^ 1) && !*give_up);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t tmem_d = tmem_base + buf * S::kCols;
+            const uint32_t tmem_d = tmem_base + buf * S::kSums * S::kCols;
             for (int kb = 0; kb < n_k && ok; ++kb, ++it) {
                 const int next = s + 1 == S::kStages ? 0 : s + 1;
                 const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
@@ -276,8 +280,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                                 pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, (k & 1) * 2), w_col + 4 * (k >> 1),
                                                x_col + (k >> 1) * S::kAtoms * 4, (kb | k) != 0);
                             } else {                               // 32 entries, one scale
-                                pair_mma<MODE>(tmem_d, a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, k), w_col,
-                                               x_col + term * S::kAtoms * 4, (kb | k | term) != 0);
+                                const bool second = S::kSums == 2 && term > 0;
+                                pair_mma<MODE>(tmem_d + (second ? S::kCols : 0), a_desc + 2 * k, b_desc + 2 * k, with_scale_byte(instr, k), w_col,
+                                               x_col + term * S::kAtoms * 4, (kb | k | (second ? term - 1 : term)) != 0);
                             }
                         }
                     }
@@ -314,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                 }
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t taddr = tmem_base + buf * S::kCols + ((uint32_t)(quarter * 32) << 16);
+            const uint32_t taddr = tmem_base + buf * S::kSums * S::kCols + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
             for (int c = 32 * group; c < t.here; c += 32 * (kEpilogueWarps / 4)) {
                 float v[32];
@@ -323,6 +328,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7fffffffu);
                 } else {
                     tmem_load_32(taddr + c, v);
+                    if constexpr (S::kSums == 2) {
+                        float rest[32];
+                        tmem_load_32(taddr + S::kCols + c, rest);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] += rest[j];
+                    }
                 }
                 if (there) {
                     OutT* out = static_cast<OutT*>(a.out) + (long long)(t.row0 + c) * a.N + feature;
