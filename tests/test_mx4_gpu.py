@@ -185,6 +185,22 @@ def test_product_of_many_pieces_of_k_a_block(m, n, k, dtype):
     check_product(m, n, k, dtype, dtype, quantized=True)
 
 
+@pytest.mark.parametrize("quantized", [False, True])
+def test_rows_of_several_bands(quantized):
+    """More bytes of rows than are multiplied by all of the weight at once, with a last band and a last tile of another size."""
+    m, n, k = (4100, 520, 8200) if not quantized else (13000, 520, 8200)
+    x = rows_of(m, k, torch.bfloat16, 1)
+    weight, w = weight_of(n, k, 2)
+    given = ops.quantize_mx4(x) if quantized else x
+    got = ops.linear_mx4(given, weight, out_dtype=torch.float32)
+    few = torch.cat([torch.arange(0, m, 97), torch.arange(m - 70, m)]).cuda()
+    x64 = (ops.dequantize_mx4(given) if quantized else x)[few].double()
+    y = x64 @ w.t()
+    error = (got[few].double() - y).abs()
+    assert (error <= bound(x64, w, y, None if quantized else torch.bfloat16, torch.float32, None)).all()
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("k", [1000, 4096, 12288])
 @pytest.mark.parametrize("m", [3, 8, 32, 33, 100, 300])
 def test_float32_rows_are_summed_as_in_float32(m, k):

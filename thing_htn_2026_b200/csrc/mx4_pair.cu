@@ -50,6 +50,7 @@ struct Args {
     const void* bias;
     int bias_dtype, M, N, atoms;                // atoms: pieces of 128 columns of the sum
     int cuts, size, n_tiles;        // the rows of x in equal tiles
+    int band;                       // how many of them are multiplied by all of W before the next
     int pitch;                      // rows of x's operand from one tile to the next
     int* err;
     int skip_loads;                 // the test of the bounded waits: nothing is loaded
@@ -182,10 +183,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     constexpr uint32_t tmem_base = 0;          // all columns are this pair's
 
-    // Neighbouring tiles share their rows of W: the tiles of rows run fastest.
+    // Neighbouring tiles share their rows of W: the tiles of rows run fastest, within a band of them that stays in L2.
+    const int n_features = (a.N + kFeatures - 1) / kFeatures;
     auto tile_of = [&](int i) {
         Tile t;
-        const int f = i / a.cuts, cut = i - f * a.cuts;
+        const int first = i / (a.band * n_features) * a.band, here = min(a.band, a.cuts - first), j = i - first * n_features;
+        const int f = j / here, cut = first + j - f * here;
         t.row0 = cut * a.size;
         t.here = min(a.size, a.M - t.row0);
         t.columns = (t.here + 31) / 32 * 32;
@@ -413,6 +416,11 @@ int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) 
     return thn_launch_status("mx4_pair");
 }
 
+// The bytes of x's operand that are multiplied by all of W before the next ones: less than half of L2, beside W and the results on their way.  16,384
+// bfloat16 rows by 24,576 x 4,096 are 134 MB of terms: 2.6 ms in three bands, 3.4 in one, which every 256 rows of W bring from memory again; by 4,096 x
+// 12,288 1.28 and 1.64 ms; bands of 24 or 96 MB are level or slower.
+constexpr long long kBandBytes = 48 << 20;
+
 template <int MODE>
 int run(Args args, const void* codes, const void* scales, const void* x, const void* x_scales, int out_dtype, cudaStream_t stream) {
     using S = Shape<MODE>;
@@ -420,6 +428,9 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
     const long long n_tiles = (long long)args.cuts * ((args.N + kFeatures - 1) / kFeatures);
     THN_UNSUPPORTED_IF(n_tiles > 0x3fffffff, "mx4_pair: M=%d N=%d are too many tiles", args.M, args.N);
     args.n_tiles = (int)n_tiles;
+    const long long x_bytes = (long long)args.M * padded * S::kT / (MODE == kQuantized ? 2 : 1);
+    const long long bands = (x_bytes + kBandBytes - 1) / kBandBytes;
+    args.band = bands < args.cuts ? (int)((args.cuts + bands - 1) / bands) : 1;
     const long long x_rows = MODE == kQuantized ? args.M : (long long)args.cuts * args.pitch;
     CUtensorMap maps[4];
     bool made = map_scales(&maps[1], scales, args.atoms, (args.N + 127) / 128, 1, S::kSteps, 1) &&
