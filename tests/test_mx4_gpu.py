@@ -340,7 +340,7 @@ def test_another_stream_and_a_recorded_graph():
     for x in static:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            outs.append([ops.linear_mx4(x, weight), ops.linear_mx4(ops.quantize_mx4(x), weight)])
+            outs.append([ops.linear_mx4(x, weight), ops.linear_mx4(ops.quantize_mx4(x, to_multiply=True), weight)])
         graphs.append(graph)
     for _ in range(3):
         for x in static:

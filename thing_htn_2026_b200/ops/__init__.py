@@ -942,7 +942,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     in the vendor product's epilogue (float32, before the one rounding), or by a kernel of its own
     after the FFMA product.  ``weight`` may be an :class:`Mx4` (:func:`linear_mx4`)."""
     if isinstance(weight, Mx4):
-        return linear_mx4(_quantize_mx4(x, early=True) if weight.quantizes_rows else x, weight, out_dtype or x.dtype, err, bias)
+        return linear_mx4(quantize_mx4(x, to_multiply=True) if weight.quantizes_rows else x, weight, out_dtype or x.dtype, err, bias)
     if bias is not None:
         _need(bias, "linear bias", x.dtype)
         if bias.shape[0] != weight.shape[0]:
@@ -1045,10 +1045,6 @@ class Mx4:
     def nbytes(self) -> int:
         return self.data.numel()
 
-    def _pointers(self) -> Tuple[int, int]:
-        at = self.data.data_ptr()
-        return at, at + self.code_bytes
-
 
 # (The checks below are written out rather than called one by one: a product of a few rows takes the device 4 to 10 us, about what its call takes
 # the host.)
@@ -1066,9 +1062,12 @@ def _mx4_stream_for(t: torch.Tensor, what: str) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-def _quantize_mx4(x: torch.Tensor, early: bool) -> Mx4:
-    """``early``: the kernel after this one may be scheduled while it runs; only for rows that are multiplied by a weight, since a product
-    reads its weight while the kernels before it are still at work."""
+def quantize_mx4(x: torch.Tensor, to_multiply: bool = False) -> Mx4:
+    """``x [rows, columns]`` (bfloat16 or float32) in microscaled 4-bit floating point.  A block's scale is
+    ``2^(floor(log2 max|x|) - 2)``, at least 2^-127, and an entry becomes the nearest magnitude, of two equally near ones that with
+    the even code; what lies above 6 scales becomes 6.  A block that holds an infinity or a NaN is not a number as a whole.
+    ``to_multiply``: the result is multiplied by a weight and is never a weight itself (which a product reads while the kernels before it are still at
+    work); the kernel after this one may then be scheduled while it runs."""
     _need(x, "quantize_mx4 x")
     shape = x.shape
     if len(shape) != 2 or shape[1] < 1:
@@ -1076,17 +1075,11 @@ def _quantize_mx4(x: torch.Tensor, early: bool) -> Mx4:
     code = _code(x, "quantize_mx4 x")
     stream = _mx4_stream_for(x, "quantize_mx4 x")
     rows, columns = shape
-    out = Mx4.__new__(Mx4)._set(x.new_empty((_mx4_bytes(rows, columns),), dtype=torch.uint8), rows, columns)
-    codes, scales = out._pointers()
-    _call("thn_mx4_quantize", codes, scales, x.data_ptr(), rows, columns, code, int(early), stream)
+    data = x.new_empty((_mx4_bytes(rows, columns),), dtype=torch.uint8)
+    out = Mx4.__new__(Mx4)._set(data, rows, columns)
+    at = data.data_ptr()
+    _call("thn_mx4_quantize", at, at + out.code_bytes, x.data_ptr(), rows, columns, code, 1 if to_multiply else 0, stream)
     return out
-
-
-def quantize_mx4(x: torch.Tensor) -> Mx4:
-    """``x [rows, columns]`` (bfloat16 or float32) in microscaled 4-bit floating point.  A block's scale is
-    ``2^(floor(log2 max|x|) - 2)``, at least 2^-127, and an entry becomes the nearest magnitude, of two equally near ones that with
-    the even code; what lies above 6 scales becomes 6.  A block that holds an infinity or a NaN is not a number as a whole."""
-    return _quantize_mx4(x, early=False)
 
 
 def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> Mx4:
@@ -1102,8 +1095,8 @@ def mx4_from_parts(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> M
         raise KernelError(f"mx4_from_parts: codes on {codes.device}, scales on {scales.device}")
     stream = _mx4_stream_for(codes, "mx4_from_parts codes")
     out = Mx4.__new__(Mx4)._set(codes.new_empty((_mx4_bytes(rows, columns),)), rows, columns)
-    to_codes, to_scales = out._pointers()
-    _call("thn_mx4_arrange", to_codes, to_scales, codes.data_ptr(), scales.data_ptr(), rows, columns, stream)
+    at = out.data.data_ptr()
+    _call("thn_mx4_arrange", at, at + out.code_bytes, codes.data_ptr(), scales.data_ptr(), rows, columns, stream)
     return out
 
 
