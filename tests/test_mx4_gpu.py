@@ -273,6 +273,9 @@ def test_refusals():
         ops.linear_mx4(x, weight, bias=torch.zeros(9, device="cuda"))
     with pytest.raises(ops.KernelError, match="CUDA"):
         ops.linear_mx4(x.cpu(), weight)
+    narrow, _ = weight_of(3, 1, 0)
+    with pytest.raises(ops.KernelError, match="at most"):
+        ops.linear_mx4(torch.zeros(((1 << 24) + 1, 1), dtype=torch.bfloat16, device="cuda"), narrow)
     with pytest.raises(ops.KernelError, match="Mx4"):
         ops.linear_mx4(x, torch.zeros((10, 64), dtype=torch.bfloat16, device="cuda"))
     with pytest.raises(ops.KernelError, match="err"):

@@ -1116,6 +1116,7 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
+_MX4_MOST = 1 << 24       # rows, outputs or columns of a product
 _mx4_terms_needs: Dict[Tuple[str, int, int, int, int], int] = {}
 
 
@@ -1156,6 +1157,8 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     held, n = weight.data, weight.rows
     if k != weight.columns:
         raise KernelError(f"linear_mx4: shapes x {(m, k)}, weight {weight.shape}")
+    if m > _MX4_MOST or n > _MX4_MOST or k > _MX4_MOST:
+        raise KernelError(f"linear_mx4: {m} rows by {n} x {k}: {_MX4_MOST} at most, please, of each")
     if held.get_device() != data.get_device():
         raise KernelError(f"linear_mx4: x on {data.device}, weight on {weight.device}")
     out_code = DTYPE_CODE.get(out_dtype)
