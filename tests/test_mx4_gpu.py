@@ -315,6 +315,22 @@ def test_the_same_call_gives_the_same_bits(m, n, k, quantized):
         assert torch.equal(ops.linear_mx4(given, weight, out_dtype=torch.float32), first)
 
 
+@pytest.mark.parametrize("rows,columns", [(1, 1), (3, 32), (130, 96), (129, 4128), (5, 4100), (7, 2056), (300, 77)])
+def test_stored_parts_that_begin_anywhere(rows, columns):
+    """Stored codes and scales at odd addresses, beside the same at whole pieces; the unused half of a row's last byte is not taken."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    codes = torch.randint(0, 256, (rows, (columns + 1) // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.randint(0, 256, (rows, -(-columns // 32)), generator=g, device="cuda", dtype=torch.uint8)
+    moved = [torch.empty(t.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view(t.shape).copy_(t) for t in (codes, scales)]
+    want = torch.zeros((rows, -(-columns // 128) * 64), dtype=torch.uint8, device="cuda")
+    want[:, :codes.shape[1]] = codes
+    if columns % 2:
+        want[:, codes.shape[1] - 1] &= 15
+    for parts in ((codes, scales), moved):
+        q = ops.mx4_from_parts(*parts, columns)
+        assert torch.equal(q.codes, want) and np.array_equal(scale_bytes(q), scales.cpu().numpy())
+
+
 def test_a_matrix_from_its_bytes():
     weight, _ = weight_of(130, 200, 3)
     again = ops.Mx4(weight.data.clone(), 130, 200)

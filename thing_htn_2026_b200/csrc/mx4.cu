@@ -206,38 +206,34 @@ __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(T* __restrict_
     }
 }
 
-// Codes and scales as they are stored, row by row, into this library's layout.  A thread has eight codes, sixteen the columns of four scale bytes; words:
-// the stored rows are whole aligned words.
+// Codes and scales as they are stored, row by row, into this library's layout.  A thread has a block, four the columns of four scale bytes; wide: the
+// stored rows are whole aligned 16-byte pieces.  24,576 x 4,096: 18.6 us, 5.7 TB/s (eight codes a thread: 58).
 __global__ void __launch_bounds__(kThreads) mx4_arrange_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                const uint8_t* __restrict__ stored, const uint8_t* __restrict__ stored_scales,
-                                                               uint32_t units, Mx4Divisor pieces, int columns, int padded, bool words) {
+                                                               uint32_t units, Mx4Divisor pieces, int columns, int padded, bool wide) {
     pdl_wait();
     const uint32_t unit = blockIdx.x * (uint32_t)kThreads + threadIdx.x, row = pieces.of(unit), piece = unit - row * pieces.d;
+    const int row_bytes = (columns + 1) / 2, blocks = (columns + kMx4Block - 1) / kMx4Block, from = (int)piece * (kMx4Block / 2);
+    const uint8_t* src = stored + (long long)row * row_bytes + from;
+    const bool there = unit < units && (int)piece < blocks;
+    uint32_t word[4] = {0, 0, 0, 0};
+    if (there && wide) {
+        const uint4 q = *reinterpret_cast<const uint4*>(src);
+        word[0] = q.x; word[1] = q.y; word[2] = q.z; word[3] = q.w;
+    } else if (there) {
+#pragma unroll
+        for (int i = 0; i < kMx4Block / 2; ++i) {
+            uint32_t byte = from + i < row_bytes ? src[i] : 0;
+            if (2 * (from + i) + 1 >= columns) byte &= 15;
+            word[i / 4] |= byte << (8 * (i & 3));
+        }
+    }
+    uint32_t four = there ? (uint32_t)stored_scales[(long long)row * blocks + piece] << (8 * (piece & 3)) : 0;
+    four |= __shfl_xor_sync(0xffffffffu, four, 1);
+    four |= __shfl_xor_sync(0xffffffffu, four, 2);
     if (unit >= units) return;
-    const int row_bytes = (columns + 1) / 2, blocks = (columns + kMx4Block - 1) / kMx4Block;
-    const uint8_t* src = stored + (long long)row * row_bytes;
-    uint32_t word = 0;
-    if (words) {
-        if ((int)piece * 4 < row_bytes) word = *reinterpret_cast<const uint32_t*>(src + piece * 4);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = (int)piece * 4 + i;
-            uint32_t byte = at < row_bytes ? src[at] : 0;
-            if (2 * at + 1 >= columns) byte &= 15;
-            word |= byte << (8 * i);
-        }
-    }
-    *reinterpret_cast<uint32_t*>(codes + (long long)row * (padded / 2) + piece * 4) = word;
-    if ((piece & 15) == 0) {
-        uint32_t four = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = (int)(piece >> 4) * 4 + i;
-            if (at < blocks) four |= (uint32_t)stored_scales[(long long)row * blocks + at] << (8 * i);
-        }
-        *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, piece >> 4, padded / kMx4Atom)) = four;
-    }
+    *reinterpret_cast<uint4*>(codes + (long long)row * (padded / 2) + from) = make_uint4(word[0], word[1], word[2], word[3]);
+    if ((piece & 3) == 0) *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, piece >> 2, padded / kMx4Atom)) = four;
 }
 
 int refuse_sizes(const char* what, long long rows, long long columns) {
@@ -323,12 +319,12 @@ THN_API int thn_mx4_arrange(void* codes, void* scales, const void* stored, const
     const int status = refuse_sizes("mx4_arrange", rows, columns);
     if (status != THN_OK) return status;
     if (rows == 0) return THN_OK;
-    const long long padded = mx4_padded(columns), pieces = padded / 8, row_bytes = (columns + 1) / 2, blocks = (columns + kMx4Block - 1) / kMx4Block;
-    const bool words = columns % 8 == 0 && ((uintptr_t)stored & 3) == 0;
+    const long long padded = mx4_padded(columns), pieces = padded / kMx4Block, row_bytes = (columns + 1) / 2, blocks = (columns + kMx4Block - 1) / kMx4Block;
+    const bool wide = columns % kMx4Block == 0 && ((uintptr_t)stored & 15) == 0;
     return in_steps(rows, pieces, [&](long long row, long long n) {
         thn_launch(mx4_arrange_kernel, (unsigned)((n * pieces + kThreads - 1) / kThreads), kThreads, 0, stream, (uint8_t*)codes + row * (padded / 2),
                    (uint8_t*)scales + row / 128 * (padded / kMx4Atom) * kMx4AtomBytes, (const uint8_t*)stored + row * row_bytes,
-                   (const uint8_t*)stored_scales + row * blocks, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces), (int)columns, (int)padded, words);
+                   (const uint8_t*)stored_scales + row * blocks, (uint32_t)(n * pieces), Mx4Divisor((uint32_t)pieces), (int)columns, (int)padded, wide);
         return thn_launch_status("mx4_arrange");
     });
 }

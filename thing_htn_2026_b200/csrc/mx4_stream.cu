@@ -555,7 +555,7 @@ int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K
 }
 
 // How many rows of a type (THN_F32, THN_BF16, 2: 4 bits) thn_mx4_stream takes.
-THN_API int thn_mx4_stream_rows(int x_type) { return x_type == THN_F32 ? 32 : 64; }
+static int rows_taken(int x_type) { return x_type == THN_F32 ? 32 : 64; }
 
 // The bytes of `terms` that M rows of a type need.
 static long long terms_needed(int x_type, int M, int N, int K) {
@@ -579,7 +579,7 @@ THN_API int thn_mx4_stream(void* out, int out_dtype, const void* x, const void* 
                            cudaStream_t stream) {
     THN_CHECK_ARG(x_type >= 0 && x_type <= 2 && (out_dtype == THN_F32 || out_dtype == THN_BF16) && (bias_dtype == THN_F32 || bias_dtype == THN_BF16),
                   "mx4_stream: unknown type %d, %d or %d", x_type, out_dtype, bias_dtype);
-    THN_UNSUPPORTED_IF(M < 1 || M > thn_mx4_stream_rows(x_type) || N < 1 || K < 1 || K > (1 << 24), "mx4_stream: M=%d N=%d K=%d not supported", M, N, K);
+    THN_UNSUPPORTED_IF(M < 1 || M > rows_taken(x_type) || N < 1 || K < 1 || K > (1 << 24), "mx4_stream: M=%d N=%d K=%d not supported", M, N, K);
     THN_CHECK_ARG((((uintptr_t)codes | (uintptr_t)(x_type == 2 ? x : codes)) & 31) == 0 &&
                   (((uintptr_t)scales | (uintptr_t)x_scales | (uintptr_t)terms) & 15) == 0, "mx4_stream: codes must be 32-byte, scales and terms 16-byte aligned");
     THN_CHECK_ARG(terms_bytes >= terms_needed(x_type, M, N, K), "mx4_stream: %lld bytes of scratch, %lld needed", terms_bytes,

@@ -155,7 +155,6 @@ _SIGNATURES = {
     "thn_mx4_pair_scratch": [c_int, c_int, c_int, c_int, c_void_p],
     "thn_mx4_pair": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                      c_int, c_void_p, c_void_p],
-    "thn_mx4_stream_rows": [c_int],
     "thn_mx4_stream_scratch": [c_int, c_int, c_int, c_int, c_void_p],
     "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                        c_int, c_void_p, c_void_p],
@@ -1178,7 +1177,7 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     if m == 0 or n == 0:
         return out
     codes = held.data_ptr()
-    few = m <= (32 if kind == 0 else 64)
+    few = m <= (32 if kind == 0 else 64)          # the rows that thn_mx4_stream takes
     terms_at, size = None, 0
     if kind != 2:
         size = _mx4_terms_need("thn_mx4_stream_scratch" if few else "thn_mx4_pair_scratch", kind, m, n, k)
