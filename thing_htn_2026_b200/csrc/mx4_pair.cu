@@ -158,6 +158,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rank = (int)block_in_pair(), pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
     const int n_k = (a.atoms + S::kSteps - 1) / S::kSteps;
+    const uint32_t b_smem = a.size / 2 * 128;              // of x, one block, a term
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -206,7 +207,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
             const Tile t = tile_of(i);
             const int b_row = t.x_row + rank * (t.columns / 2), a_row = t.feature + rank * 128;
             // (a last tile of fewer columns brings what a whole one does)
-            constexpr uint32_t kBytes = (MODE == kQuantized ? S::kASmem : S::kASmem / 2) + S::kT * S::kBSmem + S::kScaleBytes;
+            const uint32_t bytes = (MODE == kQuantized ? S::kASmem : S::kASmem / 2) + S::kT * b_smem + S::kScaleBytes;
             for (int kb = 0; kb < n_k && !a.skip_loads; ++kb, ++it) {
                 const int s = it % S::kStages;
                 if (!__all_sync(0xffffffffu, mbar_wait(empty + s, ((it / S::kStages) & 1) ^ 1))) {
@@ -218,7 +219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                 unsigned char* scales = dst + S::kASmem + S::kT * S::kBSmem;
                 const uint32_t bar = leader_full + s * (uint32_t)sizeof(uint64_t);
                 if (issues) {
-                    if (rank == 0) mbar_expect_tx(full + s, 2 * kBytes);
+                    if (rank == 0) mbar_expect_tx(full + s, 2 * bytes);
                     load_box(dst, &map_w, bar, kb * 128, a_row);           // (bytes of codes, or entries)
                     load_box(dst + S::kASmem, &map_x, bar, kb * 128, b_row, 0);
                     load_box(scales, &map_w_scales, bar, 0, kb * S::kSteps, a_row >> 7, 0);
@@ -275,7 +276,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
                     if (brought) bring_scales(next, (it + 1) & 1);
 #pragma unroll
                     for (int term = 0; term < S::kT; ++term) {
-                        const uint64_t b_desc = smem_desc(at + S::kASmem + term * S::kBSmem);
+                        const uint64_t b_desc = smem_desc(at + S::kASmem + term * b_smem);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {      // 32 bytes further along K: + 2 in the address field
                             if constexpr (MODE == kQuantized) {    // 64 entries, two of a piece's four scales
@@ -436,10 +437,10 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
     bool made = map_scales(&maps[1], scales, args.atoms, (args.N + 127) / 128, 1, S::kSteps, 1) &&
                 map_scales(&maps[3], x_scales, args.atoms, (x_rows + 127) / 128, S::kT, S::kSteps, S::kAtoms);
     if (MODE == kQuantized)
-        made = made && map_bytes(&maps[0], codes, args.N, padded / 2, 128) && map_planes(&maps[2], x, padded / 2, x_rows, 1, S::kCols / 2);
+        made = made && map_bytes(&maps[0], codes, args.N, padded / 2, 128) && map_planes(&maps[2], x, padded / 2, x_rows, 1, args.size / 2);
     else
         made = made && map_unpacked(&maps[0], codes, args.N, padded, 128) &&
-               map_planes(&maps[2], x, padded, x_rows, S::kT, S::kCols / 2);
+               map_planes(&maps[2], x, padded, x_rows, S::kT, args.size / 2);
     if (!made) {
         thn_set_error("mx4_pair: cuTensorMapEncodeTiled failed for M=%d N=%d and %d pieces of K", args.M, args.N, args.atoms);
         return THN_BAD_ARGUMENT;
@@ -450,24 +451,26 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
 }  // namespace
 
 // How M rows are cut into tiles by N outputs: the size (a multiple of 32) with which the pairs' rounds take the least time, a stage of a tile counted
-// with 4 clocks a column (rows in 4 bits: 2), the products' time, but 500 at least, which its thread takes to issue them; the rows of x's operand from one tile to the
-// next.  Terms are written by a kernel of this library, which begins every tile at a whole piece of 128 rows of scales; rows in 4 bits lie as they
+// with its products' time, 2 clocks a column and term, or that of its bytes of shared memory at 64 a clock, whichever is longer; the rows of x's operand from one tile to
+// the next.  Terms are written by a kernel of this library, which begins every tile at a whole piece of 128 rows of scales; rows in 4 bits lie as they
 // do, and their tiles begin at multiples of 64.  (2,048 rows by 2,560 outputs are 130 tiles of 160 rows and not 110 of 192: two rounds of 74 pairs
 // either way.)
 struct RowCuts {
     int cuts, size, pitch;
 };
-static RowCuts cuts_for(bool quantized, int M, int N, int pairs) {
-    const int most = Shape<kQuantized>::kCols, grain = quantized ? 64 : 32, clocks = quantized ? 2 : 4;
+static RowCuts cuts_for(int x_type, int M, int N, int pairs) {
+    const bool quantized = x_type == 2;
+    const int most = Shape<kQuantized>::kCols, grain = quantized ? 64 : 32, terms = quantized ? 1 : x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>;
     const long long features = (N + kFeatures - 1) / kFeatures;
     RowCuts best = {};
     long long least = 0;
     for (int size = most; size >= grain; size -= grain) {
-        const long long cuts = (M + size - 1) / size, rounds = (cuts * features + pairs - 1) / pairs;
-        const int columns = cuts == 1 ? (M + 31) / 32 * 32 : size;
-        const long long time = rounds * (clocks * columns < 500 ? 500 : clocks * columns);
+        const int cuts = (M + size - 1) / size, columns = cuts == 1 ? (M + 31) / 32 * 32 : size;
+        const long long rounds = (cuts * features + pairs - 1) / pairs, products = 2 * terms * columns;
+        const long long loads = (16384 + terms * columns * 64) / 64;
+        const long long time = rounds * (products < loads ? loads : products);
         if (best.cuts == 0 || time < least) {
-            best = {(int)cuts, size, quantized ? size : (size + 127) / 128 * 128};
+            best = {cuts, columns, quantized ? columns : (columns + 127) / 128 * 128};
             least = time;
         }
     }
@@ -477,7 +480,7 @@ static RowCuts cuts_for(bool quantized, int M, int N, int pairs) {
 // The bytes of `terms` that M rows of a type need by N outputs.
 static long long terms_needed(int x_type, int M, int N, int K) {
     if (x_type == 2) return 0;
-    const RowCuts c = cuts_for(false, M, N, pair_count());
+    const RowCuts c = cuts_for(x_type, M, N, pair_count());
     const long long rows = (long long)c.cuts * c.pitch * (x_type == THN_F32 ? kTerms<float> : kTerms<__nv_bfloat16>), padded = mx4_padded(K);
     return rows * padded + rows / 128 * (padded / kMx4Atom) * kMx4AtomBytes;
 }
@@ -511,7 +514,7 @@ THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_
     args.atoms = (int)(mx4_padded(K) / kMx4Atom);
     args.err = err;
     args.skip_loads = skip_loads;
-    const RowCuts rows = cuts_for(x_type == 2, M, N, pair_count());
+    const RowCuts rows = cuts_for(x_type, M, N, pair_count());
     args.cuts = rows.cuts;
     args.size = rows.size;
     args.pitch = rows.pitch;
