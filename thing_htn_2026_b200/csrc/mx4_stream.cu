@@ -193,15 +193,15 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
     } else if (warp == 1) {
         // ---- the products: the whole warp walks, one thread of it issues.  A stage's scales go to tensor memory ahead of the products of the stage
         // before it, so that they are copied under those; two sets of columns take them in turn.
-        // (Tensor memory is taken while the kernels before still run.  None of their blocks on this multiprocessor waits for it in vain: a block with 88 KB of
-        // shared memory or more, as all of this library's with tensor memory are, shares a multiprocessor with one other at most, and has 256
-        // columns at most where it can share.  Taken after them, it made one row by 19,456 x 2,560 9.9 us, 8.1 so.)
+        // (Tensor memory is taken once the kernels before are done: a block that held it while it waits for them could hold what one of theirs, or of another
+        // stream's kernels beside them, still has to take, and that wait has no bound.
+        // One row by 19,456 x 2,560 takes 9.9 us so, 8.1 with columns taken ahead of the wait; by 6,144 x 2,560 5.3 and 5.1; other sizes are level.)
+        pdl_wait();
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                      "r"(S::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        pdl_wait();                            // (ahead of the first bounded wait for what depends on the kernels before)
-        __syncwarp();
         asm volatile("bar.sync 1, 160;" ::: "memory");         // the warps of the sums
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
