@@ -89,8 +89,10 @@ __device__ __forceinline__ uint32_t leader_addr(const void* p) {
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
     return a;
 }
+// All threads of both blocks.  (Not the .aligned form, which counts warps: a warp whose lanes come one after the other would count twice.)
 __device__ __forceinline__ void pair_barrier() {
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count));
@@ -192,7 +194,6 @@ template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_gemm_kernel(
     const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sorted,
     const __grid_constant__ CUtensorMap map_x, PairArgs a) {
-    pdl_launch_dependents();
     constexpr int kTileFeatures = MODE == kGlu ? kFeatures / 2 : kFeatures, kTileRows = tile_rows(MODE);
     constexpr uint32_t kLoaded = kABytes + kTileRows / 2 * BK * 2;      // bytes of a step, per block
     extern __shared__ unsigned char smem_raw[];
@@ -223,12 +224,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ge
         *give_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
     if (warp == 1) {   // the same warp of both blocks allocates both accumulators' columns
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                      "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
-    pdl_wait();
     // how many tiles the groups have, summed: warp 0, a group a lane and turn
     if (warp == 0) {
         int sum = 0;
@@ -254,6 +255,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ge
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     pair_barrier();                            // both blocks' barriers stand
+    __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
     const int n_tiles = first_tile[n_groups];
@@ -474,10 +476,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) pair_ge
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     pair_barrier();                            // neither block leaves while the other may reach into it
+    __syncwarp();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
     }
+    // neither block leaves before both have given their tensor memory back
+    __syncthreads();
+    pair_barrier();
 }
 
 constexpr int kSortThreads = 1024;
@@ -626,7 +632,9 @@ int launch_pairs(const CUtensorMap& w, const CUtensorMap& sorted, const CUtensor
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
     const long long pairs = most_tiles < n_sms / 2 ? most_tiles : n_sms / 2;
-    thn_launch(kernel, dim3((unsigned)(2 * (pairs > 0 ? pairs : 1))), kThreads, kSmemBytes, stream, w, sorted, x, args);
+    // In plain stream order, and no kernel is scheduled early behind it: a pair holds all tensor memory of two multiprocessors from its start to its end,
+    // and nothing waits for some of it while kernels before or behind still run.
+    thn_launch_ordered(kernel, dim3((unsigned)(2 * (pairs > 0 ? pairs : 1))), kThreads, kSmemBytes, stream, w, sorted, x, args);
     return thn_launch_status("moe_grouped");
 }
 
