@@ -1005,9 +1005,10 @@ class Mx4:
     scale, a power of two held in a byte (``2^(byte - 127)``; 255: the block is not a number), and an entry is one of 0, 1/2, 1, 3/2,
     2, 3, 4, 6 with a sign, held in four bits.  :func:`quantize_mx4` makes one from numbers, :func:`mx4_from_parts` from stored codes
     and scales.  ``data`` holds the codes and behind them the scales, laid out for the tensor cores (``csrc/mx4.cuh``).
-    ``quantizes_rows``: as a weight of :func:`linear`, the rows that it multiplies are brought to 4 bits first."""
+    ``quantizes_rows``: as a weight of :func:`linear`, the rows that it multiplies are brought to 4 bits first.  ``only_rows``: made to be
+    multiplied (:func:`quantize_mx4`), and refused as a weight."""
 
-    __slots__ = ("data", "rows", "columns", "code_bytes", "quantizes_rows")
+    __slots__ = ("data", "rows", "columns", "code_bytes", "quantizes_rows", "only_rows")
 
     def __init__(self, data: torch.Tensor, rows: int, columns: int, quantizes_rows: bool = False):
         _need(data, "Mx4 data", torch.uint8)
@@ -1017,8 +1018,8 @@ class Mx4:
                               f"columns: {_mx4_bytes(rows, columns)} bytes at a multiple of 32, please")
         self._set(data, rows, columns, quantizes_rows)
 
-    def _set(self, data: torch.Tensor, rows: int, columns: int, quantizes_rows: bool = False) -> "Mx4":
-        self.data, self.rows, self.columns, self.quantizes_rows = data, rows, columns, quantizes_rows
+    def _set(self, data: torch.Tensor, rows: int, columns: int, quantizes_rows: bool = False, only_rows: bool = False) -> "Mx4":
+        self.data, self.rows, self.columns, self.quantizes_rows, self.only_rows = data, rows, columns, quantizes_rows, only_rows
         self.code_bytes = rows * ((columns + 127) // 128 * 64)
         return self
 
@@ -1065,8 +1066,8 @@ def quantize_mx4(x: torch.Tensor, to_multiply: bool = False) -> Mx4:
     """``x [rows, columns]`` (bfloat16 or float32) in microscaled 4-bit floating point.  A block's scale is
     ``2^(floor(log2 max|x|) - 2)``, at least 2^-127, and an entry becomes the nearest magnitude, of two equally near ones that with
     the even code; what lies above 6 scales becomes 6.  A block that holds an infinity or a NaN is not a number as a whole.
-    ``to_multiply``: the result is multiplied by a weight and is never a weight itself (which a product reads while the kernels before it are still at
-    work); the kernel after this one may then be scheduled while it runs."""
+    ``to_multiply``: the result is multiplied by a weight and is refused as a weight itself, which a product reads while the kernels before it are still at
+    work (its bytes, ``data``, are no weight either); the kernel after this one may then be scheduled while it runs."""
     _need(x, "quantize_mx4 x")
     shape = x.shape
     if len(shape) != 2 or shape[1] < 1:
@@ -1075,7 +1076,7 @@ def quantize_mx4(x: torch.Tensor, to_multiply: bool = False) -> Mx4:
     stream = _mx4_stream_for(x, "quantize_mx4 x")
     rows, columns = shape
     data = x.new_empty((_mx4_bytes(rows, columns),), dtype=torch.uint8)
-    out = Mx4.__new__(Mx4)._set(data, rows, columns)
+    out = Mx4.__new__(Mx4)._set(data, rows, columns, False, bool(to_multiply))
     at = data.data_ptr()
     _call("thn_mx4_quantize", at, at + out.code_bytes, x.data_ptr(), rows, columns, code, 1 if to_multiply else 0, stream)
     return out
@@ -1137,6 +1138,9 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     leaves is NaN in any case)."""
     if weight.__class__ is not Mx4:
         raise KernelError(f"linear_mx4: a weight in 4 bits (Mx4), please, not {type(weight).__name__}")
+    if weight.only_rows:
+        raise KernelError("linear_mx4: a weight that was quantised with to_multiply, which its kernel may still be writing when a product reads it: "
+                          "quantize_mx4(w), please")
     if x.__class__ is Mx4:
         kind, data, m, k = 2, x.data, x.rows, x.columns
         at = data.data_ptr()
