@@ -40,13 +40,15 @@ class Engine:
         fixes the size of the cache; left out, the cache is sized by the first call that
         needs more (as the reference sizes its cache per shape, engine/engine.py:830-846).
         ``weights="mx4"``: the layers' products hold their weights in microscaled 4-bit floating
-        point, and with ``activations="mx4"`` they multiply rows brought to 4 bits as well."""
+        point, and with ``activations="mx4"`` they multiply rows brought to 4 bits as well.  (A ``model`` that an engine
+        computes with already keeps its weights: refused.)"""
         if not torch.cuda.is_available():
             raise RuntimeError("Engine needs a CUDA device; this library has no CPU path")
         self.dtype = parse_dtype(dtype)
         self.device = torch.device(device)
         self.model = model if model is not None else load_model(model_path, self.dtype, device)
         self.model.quantize(weights, activations)
+        self.model.used_by(self)
         self.use_graphs = _env_flag("DRYFT_ENGINE_GRAPHS", True) if graphs is None else bool(graphs)
         self.depth = max(1, int(os.environ.get("DRYFT_ENGINE_DEPTH", 3) if depth is None else depth))
         self.max_batch = int(max_batch)

@@ -37,6 +37,7 @@ class StepRunner:
         self.cache = cache
         self.device = model.device
         self.err = ops.new_error_word(self.device)
+        model.used_by(self)
         model.ensure_positions(cache.max_pages_per_seq * cache.page_size)
         for name, (shape, dtype) in model.sequence_states().items():     # before any step is captured as a graph
             cache.sequence_state(name, shape, dtype)

@@ -5,6 +5,7 @@ engine/engine.py:1101-1121)."""
 
 from __future__ import annotations
 
+import weakref
 from dataclasses import replace
 from typing import Dict, Iterable, List, Optional
 
@@ -29,6 +30,8 @@ def tensor_specs_of_plan(plan: ModelPlan) -> List[TensorSpec]:
 
 
 class DecoderModel:
+    _users = ()
+
     def __init__(self, config: ModelConfig, tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device):
         self.config = config
         self.plan = plan = config.plan()
@@ -44,6 +47,7 @@ class DecoderModel:
         self.vocab_size = plan.vocab_size
         self.adds_start = any(entry.adds_start for entry in plan.schedule)
         runtime.tensors = {}   # parts hold what they need; fused copies replace the originals
+        self._users = weakref.WeakSet()
 
     # ------------------------------------------------------------------ construction
 
@@ -61,16 +65,23 @@ class DecoderModel:
                                            matrix_std, gain_std)
         return cls(config, tensors, dtype, device)
 
+    def used_by(self, user) -> None:
+        """``user`` (an engine, a step runner) computes with this model, and may have recorded where its weights lie."""
+        self._users.add(user)
+
     def quantize(self, weights: Optional[str], activations: Optional[str] = None) -> None:
         """``weights`` "mx4": the weights of the layers' products are held in microscaled 4-bit floating point from here on
         (:class:`ops.Mx4`); the embedding, the head, norms, routers, gates, convolutions and routed experts stay as they
         are.  ``activations`` "mx4": what these products multiply is brought to 4 bits too, a row at a time, at every step.  None:
-        nothing is changed."""
+        nothing is changed.  Refused while an engine or a step runner that was made before computes with the weights that would go."""
         if weights is None and activations is None:
             return
         if weights != "mx4" or activations not in (None, "mx4"):
             raise ValueError(f"weights {weights!r} with activations {activations!r}: weights are 'mx4' or None, activations 'mx4' "
                              f"(with such weights) or None")
+        if len(self._users) and any(isinstance(w, torch.Tensor) for layer in self.layers for _, _, w in layer.products()):
+            raise ValueError(f"an engine or step runner ({type(next(iter(self._users))).__name__}) computes with this model's weights as they are: "
+                             f"weights='mx4' needs a model of its own, or one whose engines are gone")
         if not sum(layer.quantize_products(activations == "mx4") for layer in self.layers):
             raise ValueError("no layer of this model has products whose weights can be held in 4 bits")
 

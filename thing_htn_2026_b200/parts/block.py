@@ -94,23 +94,22 @@ class Block:
         mixer = getattr(self, "mixer", None)
         return mixer.cache_need() if mixer is not None else None
 
+    def products(self) -> List[Tuple[object, str, object]]:
+        """(part, name, weight) of the block's and its members' products (their ``PRODUCTS``: names of weights that only
+        :func:`ops.linear` and :func:`ops.linear_swiglu` read)."""
+        held = [(part, name, getattr(part, name)) for part in [self] + self.parts() for name in getattr(part, "PRODUCTS", ())]
+        return [(part, name, weight) for part, name, weight in held if weight is not None]
+
     def quantize_products(self, quantize_rows: bool = False) -> int:
-        """Bring the weights of the members' products (their ``PRODUCTS``: names of weights that only :func:`ops.linear`
-        and :func:`ops.linear_swiglu` read) to 4 bits; ``quantize_rows``: the rows that they multiply too, at every step.
+        """Bring the weights of the products to 4 bits; ``quantize_rows``: the rows that they multiply too, at every step.
         Returns how many there are."""
-        count = 0
-        for part in [self] + self.parts():
-            for name in getattr(part, "PRODUCTS", ()):
-                weight = getattr(part, name)
-                if isinstance(weight, torch.Tensor):
-                    quantized = ops.quantize_mx4(weight.contiguous())
-                    quantized.quantizes_rows = bool(quantize_rows)
-                    setattr(part, name, quantized)
-                    count += 1
-                elif isinstance(weight, ops.Mx4):
-                    weight.quantizes_rows = bool(quantize_rows)
-                    count += 1
-        return count
+        held = self.products()
+        for part, name, weight in held:
+            if isinstance(weight, torch.Tensor):
+                weight = ops.quantize_mx4(weight.contiguous())
+                setattr(part, name, weight)
+            weight.quantizes_rows = bool(quantize_rows)
+        return len(held)
 
     def step_inputs(self, batch: HostBatch, out: Dict[str, List[int]]) -> None:
         """Integer inputs that members want computed on the host for this step, by name."""
