@@ -36,16 +36,17 @@ class _Handle:
 
 class DeviceBackend:
     def __init__(self, model, cache: SequenceCache, *, max_batch: int = 64, use_graphs: bool = True,
-                 ring: int = 8):
+                 ring: int = 8, rows_quantized=None):
         """``ring``: pinned token buffers for steps whose tokens the host has not fetched yet;
         a generation loop of depth d keeps d + 1 such steps, so it needs ``ring >= d + 1``.
-        Sending one more than the ring holds raises instead of overwriting."""
+        Sending one more than the ring holds raises instead of overwriting.
+        ``rows_quantized``: see :class:`StepRunner`."""
         self.model, self.cache = model, cache
         self.device = model.device
         self.page_size = cache.page_size
         self._max_batch = min(int(max_batch), cache.max_slots - 1)
         self.use_graphs = bool(use_graphs)
-        self.runner = StepRunner(model, cache)
+        self.runner = StepRunner(model, cache, rows_quantized)
         self.err = self.runner.err
         self.chooser = TokenChooser(cache)
         self.last_token = self.chooser.last_token

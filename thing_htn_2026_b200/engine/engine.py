@@ -41,7 +41,7 @@ class Engine:
         needs more (as the reference sizes its cache per shape, engine/engine.py:830-846).
         ``weights="mx4"``: the layers' products hold their weights in microscaled 4-bit floating
         point, and with ``activations="mx4"`` they multiply rows brought to 4 bits as well.  (A ``model`` that an engine
-        computes with already keeps its weights: refused.)"""
+        computes with already keeps its weights: refused.  Over weights in 4 bits, each engine keeps its own choice of rows.)"""
         if not torch.cuda.is_available():
             raise RuntimeError("Engine needs a CUDA device; this library has no CPU path")
         self.dtype = parse_dtype(dtype)
@@ -49,6 +49,7 @@ class Engine:
         self.model = model if model is not None else load_model(model_path, self.dtype, device)
         self.model.quantize(weights, activations)
         self.model.used_by(self)
+        self._rows_quantized = self.model.rows_quantized()
         self.use_graphs = _env_flag("DRYFT_ENGINE_GRAPHS", True) if graphs is None else bool(graphs)
         self.depth = max(1, int(os.environ.get("DRYFT_ENGINE_DEPTH", 3) if depth is None else depth))
         self.max_batch = int(max_batch)
@@ -75,7 +76,7 @@ class Engine:
         cache = SequenceCache(self.model.cache_needs(), max_tokens=pages * page, dtype=self.dtype,
                               device=self.device, max_slots=max(2, min(pages, self.max_batch + 1)))
         self.backend = DeviceBackend(self.model, cache, max_batch=self.max_batch, use_graphs=self.use_graphs,
-                                     ring=self.depth + 2)
+                                     ring=self.depth + 2, rows_quantized=self._rows_quantized)
         self.loop = GenerationLoop(self.backend, self.depth)
 
     def _ensure_cache(self, requests: Sequence[Request], whole_queue_in_one_batch: bool) -> None:

@@ -13,7 +13,7 @@ The reference has two functions with equal lengths only: ``_prefill_slice`` for 
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, FrozenSet, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -30,14 +30,16 @@ class StepEntry:
 
 
 class StepRunner:
-    """Owns the device error word and drives ``model`` over ``cache``."""
+    """Owns the device error word and drives ``model`` over ``cache``.  ``rows_quantized``: the weights in 4 bits whose rows
+    its steps bring to 4 bits too (None: as the model says now)."""
 
-    def __init__(self, model, cache: SequenceCache):
+    def __init__(self, model, cache: SequenceCache, rows_quantized: Optional[FrozenSet[ops.Mx4]] = None):
         self.model = model
         self.cache = cache
         self.device = model.device
         self.err = ops.new_error_word(self.device)
         model.used_by(self)
+        self.rows_quantized = model.rows_quantized() if rows_quantized is None else rows_quantized
         model.ensure_positions(cache.max_pages_per_seq * cache.page_size)
         for name, (shape, dtype) in model.sequence_states().items():     # before any step is captured as a graph
             cache.sequence_state(name, shape, dtype)
@@ -76,10 +78,11 @@ class StepRunner:
         rows = ops.step_rows(cu_seqlens, slots, self.cache.seq_lens, n_rows, max_q_len, out=row_out,
                              max_context=max_context, lengths_differ=lengths_differ)
         ctx = StepContext(rows=rows, cache=self.cache, err=self.err, inputs=inputs or {})
-        h, d = self.model.hidden(tokens, ctx)
         logits = None
-        if want_rows is None or want_rows.shape[0]:
-            logits = self.model.logits(h, d, want_rows, self.err)
+        with ops.quantizing_rows_of(self.rows_quantized):
+            h, d = self.model.hidden(tokens, ctx)
+            if want_rows is None or want_rows.shape[0]:
+                logits = self.model.logits(h, d, want_rows, self.err)
         ops.advance(self.cache.seq_lens, slots, cu_seqlens)
         return logits
 

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import weakref
 from dataclasses import replace
-from typing import Dict, Iterable, List, Optional
+from typing import Dict, FrozenSet, Iterable, List, Optional
 
 import torch
 
@@ -73,7 +73,8 @@ class DecoderModel:
         """``weights`` "mx4": the weights of the layers' products are held in microscaled 4-bit floating point from here on
         (:class:`ops.Mx4`); the embedding, the head, norms, routers, gates, convolutions and routed experts stay as they
         are.  ``activations`` "mx4": what these products multiply is brought to 4 bits too, a row at a time, at every step.  None:
-        nothing is changed.  Refused while an engine or a step runner that was made before computes with the weights that would go."""
+        nothing is changed.  Refused while an engine or a step runner that was made before computes with the weights that would go;
+        over weights in 4 bits already, the choice of rows holds for engines and step runners that are made from here on."""
         if weights is None and activations is None:
             return
         if weights != "mx4" or activations not in (None, "mx4"):
@@ -84,6 +85,10 @@ class DecoderModel:
                              f"weights='mx4' needs a model of its own, or one whose engines are gone")
         if not sum(layer.quantize_products(activations == "mx4") for layer in self.layers):
             raise ValueError("no layer of this model has products whose weights can be held in 4 bits")
+
+    def rows_quantized(self) -> FrozenSet[ops.Mx4]:
+        """The weights whose rows are brought to 4 bits (an engine keeps the choice that it was made with)."""
+        return frozenset(w for layer in self.layers for _, _, w in layer.products() if isinstance(w, ops.Mx4) and w.quantizes_rows)
 
     # ------------------------------------------------------------------ cache and positions
 

@@ -8,8 +8,10 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
+from contextlib import contextmanager
 from dataclasses import dataclass
-from typing import Dict, NamedTuple, Optional, Tuple
+from typing import Dict, FrozenSet, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -941,7 +943,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out_dtype: Optional[torch.dtyp
     in the vendor product's epilogue (float32, before the one rounding), or by a kernel of its own
     after the FFMA product.  ``weight`` may be an :class:`Mx4` (:func:`linear_mx4`)."""
     if isinstance(weight, Mx4):
-        return linear_mx4(quantize_mx4(x, to_multiply=True) if weight.quantizes_rows else x, weight, out_dtype or x.dtype, err, bias)
+        chosen = getattr(_rows_chosen, "weights", None)
+        quantizes = weight.quantizes_rows if chosen is None else weight in chosen
+        return linear_mx4(quantize_mx4(x, to_multiply=True) if quantizes else x, weight, out_dtype or x.dtype, err, bias)
     if bias is not None:
         _need(bias, "linear bias", x.dtype)
         if bias.shape[0] != weight.shape[0]:
@@ -1005,7 +1009,8 @@ class Mx4:
     scale, a power of two held in a byte (``2^(byte - 127)``; 255: the block is not a number), and an entry is one of 0, 1/2, 1, 3/2,
     2, 3, 4, 6 with a sign, held in four bits.  :func:`quantize_mx4` makes one from numbers, :func:`mx4_from_parts` from stored codes
     and scales.  ``data`` holds the codes and behind them the scales, laid out for the tensor cores (``csrc/mx4.cuh``).
-    ``quantizes_rows``: as a weight of :func:`linear`, the rows that it multiplies are brought to 4 bits first.  ``only_rows``: made to be
+    ``quantizes_rows``: as a weight of :func:`linear`, the rows that it multiplies are brought to 4 bits first (unless
+    :func:`quantizing_rows_of` says for which weights).  ``only_rows``: made to be
     multiplied (:func:`quantize_mx4`), and refused as a weight."""
 
     __slots__ = ("data", "rows", "columns", "code_bytes", "quantizes_rows", "only_rows")
@@ -1044,6 +1049,21 @@ class Mx4:
     @property
     def nbytes(self) -> int:
         return self.data.numel()
+
+
+_rows_chosen = threading.local()
+
+
+@contextmanager
+def quantizing_rows_of(weights: FrozenSet[Mx4]):
+    """In this context, and on this thread, :func:`linear` brings the rows that these weights multiply to 4 bits, and no others': several engines can
+    share a model, each with a choice of its own."""
+    before = getattr(_rows_chosen, "weights", None)
+    _rows_chosen.weights = weights
+    try:
+        yield
+    finally:
+        _rows_chosen.weights = before
 
 
 # (The checks below are written out rather than called one by one: a product of a few rows takes the device 4 to 10 us, about what its call takes
