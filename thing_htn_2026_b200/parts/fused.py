@@ -50,20 +50,20 @@ class PhasedMixer:
     inner_width: int = 0
     state_base: int = 0
 
+    def hold(self, in_rows: Tuple[torch.Tensor, Optional[torch.Tensor]], out_rows: Tuple[torch.Tensor, Optional[torch.Tensor]]) -> None:
+        """The weights (and biases) of this mixer's own products.  Nothing else of it keeps them, so that they are gone once they are replaced."""
+        self.w_in, self.b_in = in_rows
+        self.w_out, self.b_out = out_rows
+
     def in_rows(self) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-        raise NotImplementedError
+        return self.w_in, self.b_in
 
     def out_rows(self) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-        raise NotImplementedError
+        return self.w_out, self.b_out
 
     def inner(self, x: torch.Tensor, proj: torch.Tensor, offset: int, ctx: StepContext, entry: ScheduleEntry,
               out: torch.Tensor, out_offset: int, scale: float) -> None:
         raise NotImplementedError
-
-    def finish(self) -> None:
-        """Called once the weights are where they will be used: alone, this mixer's own products."""
-        self.w_in, self.b_in = self.in_rows()
-        self.w_out, self.b_out = self.out_rows()
 
     def forward(self, x: torch.Tensor, ctx: StepContext, entry: ScheduleEntry) -> torch.Tensor:
         proj = ops.linear(x, self.w_in, err=ctx.err, bias=self.b_in)
@@ -110,6 +110,7 @@ class MixerPair:
             need = member.cache_need()
             states += sum(not isinstance(one, KVSpec) for one in (need if isinstance(need, tuple) else (need,))
                           if one is not None)
+            member.hold((None, None), (None, None))            # the pair's products are over copies of them
         self.inner_width = at_out
 
     def cache_need(self) -> CacheNeed:

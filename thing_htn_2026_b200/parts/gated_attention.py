@@ -93,16 +93,9 @@ class GatedAttention(PhasedMixer):
                 for n in ("q", "k", "v")]
         if self.gated:
             rows.append((self._runtime_tensor("g_proj"), None))
-        self._in = (torch.cat([w for w, _ in rows], dim=0).contiguous(), cat_bias(rows))
-        self._out = (self._runtime_tensor("o_proj"), self._runtime_tensor("o_bias") if self.biased else None)
+        self.hold((torch.cat([w for w, _ in rows], dim=0).contiguous(), cat_bias(rows)),
+                  (self._runtime_tensor("o_proj"), self._runtime_tensor("o_bias") if self.biased else None))
         self._runtime_tensor = None
-        self.finish()
-
-    def in_rows(self):
-        return self._in
-
-    def out_rows(self):
-        return self._out
 
     def cache_need(self) -> CacheNeed:
         return KVSpec(self.n_kv, self.head_dim, self.window, 0, None, self.value_dim)

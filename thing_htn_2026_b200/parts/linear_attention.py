@@ -100,15 +100,7 @@ class LinearAttention(PhasedMixer):
         self.out_gain = f32(runtime.tensor(spec, "norm"))
         self.inner_width = h * e
         self.gate_offset = 2 * h * d + h * e
-        self._in = (torch.cat([runtime.tensor(spec, n) for n in ("q", "k", "v", "g")], dim=0).contiguous(), None)
-        self._out = (runtime.tensor(spec, "o"), None)
-        self.finish()
-
-    def in_rows(self):
-        return self._in
-
-    def out_rows(self):
-        return self._out
+        self.hold((torch.cat([runtime.tensor(spec, n) for n in ("q", "k", "v", "g")], dim=0).contiguous(), None), (runtime.tensor(spec, "o"), None))
 
     def cache_need(self) -> CacheNeed:
         return StateSpec((self.n_heads, self.value_dim, self.key_dim), torch.float32)

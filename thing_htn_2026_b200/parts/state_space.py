@@ -65,7 +65,7 @@ class StateSpaceMixer:
         f32 = lambda t: t.to(torch.float32).contiguous()
         w_in = runtime.tensor(spec, "in")
         wide = 2 * self.inner + 2 * g * n
-        self.w_in, self.w_dt = w_in[:wide].contiguous(), w_in[wide:].contiguous()
+        self.w_in, self.w_dt = w_in[:wide], w_in[wide:].clone()      # (a slice of it would keep all of it once w_in is held in 4 bits)
         rate = torch.exp(runtime.tensor(spec, "A_log").to(torch.float64)).to(torch.float32).contiguous()
         self.shape = ops.StateSpace(h, e, n, g, f32(runtime.tensor(spec, "conv")), f32(runtime.tensor(spec, "conv_bias")),
                                     f32(runtime.tensor(spec, "dt_bias")), rate, f32(runtime.tensor(spec, "D")))
