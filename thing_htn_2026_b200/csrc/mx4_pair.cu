@@ -12,7 +12,7 @@
 //    products that use them.  A tile's rows of x begin at a multiple of 64 rows of its operand, two columns of scales.
 //
 // A row's result depends on its own entries and its place in a tile alone.  Every wait on an mbarrier is bounded: after
-// kWaitLimitNs the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, what is left to store becomes NaN, and tensor
+// kWaitLimitNs, and more for the stages of a sum, the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, what is left to store becomes NaN, and tensor
 // memory is given back.  A pair's two blocks are one cluster and always resident together; no wait depends on another pair.
 #include "mx4_tcgen05.cuh"
 
@@ -315,7 +315,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
             const bool there = feature < a.N;
             const float bias = bias_of(a.bias, a.bias_dtype, feature, a.N);
             if (!dead) {
-                const bool came = mbar_wait(acc_full + buf, (local / S::kBuffers) & 1);
+                const bool came = mbar_wait(acc_full + buf, (local / S::kBuffers) & 1, sum_limit_ns(n_k));
                 dead = !__all_sync(0xffffffffu, came && !*give_up);      // all lanes together before tcgen05.ld
                 if (dead) {
                     if (lane == 0 && a.err) atomicOr(a.err, THN_ERR_WAIT_TIMEOUT);

@@ -14,8 +14,9 @@
 //  * W of the first stages is asked for while the kernels before still run; those that write a weight in this form (mx4.cu) let nothing run ahead of
 //    their end.
 //
-// Every wait on an mbarrier is bounded: after kWaitLimitNs the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's error word, the
-// block's partial sums become NaN, and tensor memory is given back.  No wait depends on another block.
+// Every wait on an mbarrier is bounded: after kWaitLimitNs, and more for the stages of a sum, the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's
+// error word, the block's partial sums become NaN, and tensor memory is given back.  These waits are for the block's own copies and products.  The
+// blocks of a cluster, which are resident together, wait for one another at its barrier, without a limit of its own: each comes there after bounded waits.
 #include <atomic>
 
 #include "mx4_tcgen05.cuh"
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
             const int buf = local & 1, out_n = tile * BW + r;
             const float bias = bias_of(a.bias, a.bias_dtype, out_n, a.N);
             if (!dead) {
-                const bool came = mbar_wait(acc_full + buf, (local >> 1) & 1);
+                const bool came = mbar_wait(acc_full + buf, (local >> 1) & 1, sum_limit_ns(n));
                 dead = !__all_sync(0xffffffffu, came && !*give_up);              // all lanes together before tcgen05.ld
                 if (dead && lane == 0) give_up_at();
             }

@@ -11,7 +11,10 @@ int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K
 
 namespace {
 
-constexpr unsigned long long kWaitLimitNs = 20ull * 1000 * 1000;   // a wait gives up after 20 ms
+// A wait gives up after 20 ms.  One for an accumulator waits for all stages of its sum, and a stage takes 2.3 us of a float32 tile's products at 1 GHz, or 4 us
+// where all pairs bring theirs from memory at half its rate: 10 us more for each (1.3 s for 2^24 columns, the most that a product takes).
+constexpr unsigned long long kWaitLimitNs = 20ull * 1000 * 1000, kStageLimitNs = 10ull * 1000;
+__device__ __forceinline__ unsigned long long sum_limit_ns(int stages) { return kWaitLimitNs + (unsigned)stages * kStageLimitNs; }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -35,11 +38,12 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-// Bounded wait for the phase with the given parity.  Returns false when it gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
+// Bounded wait for the phase with the given parity.  Returns false when it gave up.  (A try may sleep for as long as the hardware lets it; the clock, which
+// counts a part of a long step alone, is looked at after each.)
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsigned long long limit_ns = kWaitLimitNs) {
     const uint32_t addr = smem_addr(bar);
     WaitClock clock;
-    for (int spin = 0;; ++spin) {
+    for (;;) {
         uint32_t done;
         asm volatile(
             "{\n"
@@ -51,7 +55,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
             : "r"(addr), "r"(parity)
             : "memory");
         if (done) return true;
-        if ((spin & 15) == 15 && clock.ran_out(kWaitLimitNs)) return false;
+        if (clock.ran_out(limit_ns)) return false;
     }
 }
 // Whether that phase is over, without waiting.
