@@ -5,7 +5,7 @@
 //    brings half), so that a multiprocessor brings half of what a block alone would for the same products.
 //  * Rows in 4 bits (kQuantized): both operands as they lie, 256 columns of the sum in 128 bytes a row, kind::mxf4, four times
 //    the rate of bfloat16.
-//  * Rows in bfloat16 or float32 (kRows2, kRows6): two or six terms of 8-bit floats (mx4_tcgen05.cuh) that mx4_terms_kernel has
+//  * Rows in bfloat16 or float32 (kRows2, kRows2Apart, kRows6): two or six terms of 8-bit floats (mx4_tcgen05.cuh) that mx4_terms_kernel has
 //    prepared, 128 columns of the sum at a time, kind::mxf8f6f4; W's codes are spread over 8-bit containers by TMA as they are
 //    copied.  Two terms at twice the rate of bfloat16 cost what a bfloat16 product costs; W is a quarter of the bytes.
 //  * Scales: 512 bytes for 128 rows and 128 columns, by TMA like the operands, to tensor memory by tcgen05.cp just ahead of the
@@ -18,19 +18,22 @@
 
 namespace {
 
-enum Mode { kQuantized, kRows2, kRows6 };
+// Rows in 4 bits; bfloat16 rows for a result in bfloat16 (kRows2) and in float32 (kRows2Apart); float32 rows.
+enum Mode { kQuantized, kRows2, kRows2Apart, kRows6 };
 
 constexpr int kFeatures = 256;                             // of a pair
 constexpr int kEpilogueWarps = 8, kThreads = 64 + 32 * kEpilogueWarps;      // warp 0: TMA, warp 1: products and tensor memory
 
 template <int MODE>
 struct Shape {
-    static constexpr int kT = MODE == kQuantized ? 1 : MODE == kRows2 ? 2 : 6;
+    static constexpr int kT = MODE == kQuantized ? 1 : MODE == kRows6 ? 6 : 2;
     static constexpr int kCols = 192;                                        // of an accumulator
     // Accumulators of a tile, and tiles that are held at once.  The tensor core cuts a sum's last bits off at every step of 32 columns, and six terms in one
     // accumulator would be six times as many cuts: 300 float32 rows, K = 4,096: 6.8e-6 off in relation to the result, 1.1e-6 for products
-    // added one after the other in float32.  So float32's first terms have an accumulator of their own.
-    static constexpr int kSums = MODE == kRows6 ? 2 : 1, kBuffers = 2 / kSums;
+    // added one after the other in float32.  So float32's first terms have an accumulator of their own, and a bfloat16's where the result keeps what it
+    // saves: 300 bfloat16 rows, K = 12,288, 4.1e-6 off in one accumulator, 0.8e-6 in two, 2.7e-6 for float32 additions; 2,048 by 24,576 x 4,096 269
+    // and 331 us.  A bfloat16 result is rounded by 2^-9 and takes one.
+    static constexpr int kSums = MODE == kRows6 || MODE == kRows2Apart ? 2 : 1, kBuffers = 2 / kSums;
     static constexpr int kSteps = MODE == kQuantized ? 2 : 1;                // pieces of 128 columns of the sum that a stage holds
     static constexpr int kAtoms = (kCols + 64 + 127) / 128;                  // of scales that a tile's rows of x can touch
     static constexpr uint32_t kASmem = 128 * 128, kBSmem = kCols / 2 * 128;  // of one block, a term
@@ -445,7 +448,9 @@ int run(Args args, const void* codes, const void* scales, const void* x, const v
         thn_set_error("mx4_pair: cuTensorMapEncodeTiled failed for M=%d N=%d and %d pieces of K", args.M, args.N, args.atoms);
         return THN_BAD_ARGUMENT;
     }
-    return out_dtype == THN_F32 ? launch<MODE, float>(maps, args, stream) : launch<MODE, __nv_bfloat16>(maps, args, stream);
+    if constexpr (MODE == kRows2) return launch<MODE, __nv_bfloat16>(maps, args, stream);
+    else if constexpr (MODE == kRows2Apart) return launch<MODE, float>(maps, args, stream);
+    else return out_dtype == THN_F32 ? launch<MODE, float>(maps, args, stream) : launch<MODE, __nv_bfloat16>(maps, args, stream);
 }
 
 }  // namespace
@@ -527,5 +532,6 @@ THN_API int thn_mx4_pair(void* out, int out_dtype, const void* x, const void* x_
     const int status = mx4_terms(bytes, term_scales, x, x_type, M, K, (int)plane, rows.size, rows.pitch, stream);
     if (status != THN_OK) return status;
     if (x_type == THN_F32) return run<kRows6>(args, codes, scales, bytes, term_scales, out_dtype, stream);
+    if (out_dtype == THN_F32) return run<kRows2Apart>(args, codes, scales, bytes, term_scales, out_dtype, stream);
     return run<kRows2>(args, codes, scales, bytes, term_scales, out_dtype, stream);
 }
