@@ -1151,9 +1151,11 @@ def _mx4_terms_need(entry: str, kind: int, m: int, n: int, k: int) -> int:
 
 def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``x [M, K] @ weight[N, K]^T`` (+ ``bias [N]``) with a weight in 4 bits: float32 sums, one rounding to ``out_dtype`` (bfloat16 or
-    float32).  ``x`` is a tensor in bfloat16 or float32, which is multiplied as it is and whose type is the default
-    ``out_dtype``, or an :class:`Mx4` (default: bfloat16).  A row of ``x`` that holds an infinity or a NaN comes out as NaN, and so does the
+    """``x [M, K] @ weight[N, K]^T`` (+ ``bias [N]``) with a weight in 4 bits: float32 sums, rounded to ``out_dtype`` (bfloat16 or
+    float32).  ``x`` is an :class:`Mx4` (default ``out_dtype``: bfloat16), or a tensor in bfloat16 or float32, whose type is the default
+    ``out_dtype``.  A tensor's entries are multiplied as they are down to 2^-13 of the largest in their block of 32 neighbours; what is
+    smaller is rounded, by at most 2^-21 (bfloat16) or 2^-37 (float32) of that largest (``linear(x, dequantize_mx4(weight, x.dtype))`` takes all of
+    them as they are).  A row of ``x`` that holds an infinity or a NaN comes out as NaN, and so does the
     column of a weight row that does.  ``err``: the step's device error word for the kernel's bounded waits (what a wait that gave up
     leaves is NaN in any case)."""
     if weight.__class__ is not Mx4:
