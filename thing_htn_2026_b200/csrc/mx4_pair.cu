@@ -307,7 +307,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mx4_pai
             *give_up = 1;
         }
     } else if (warp >= 2) {
-        // ---- epilogue: a warp reads tensor-memory lanes 32 * (warp % 4) .. + 31 (= features), every fourth chunk of 32 columns (= rows)
+        // ---- epilogue: a warp reads tensor-memory lanes 32 * (warp % 4) .. + 31 (= features), its group every second chunk of 32 columns (= rows)
         const int quarter = warp & 3, group = (warp - 2) >> 2;
         int local = 0;
         bool dead = false;
@@ -407,12 +407,9 @@ int pair_count() {
 
 template <int MODE, typename OutT>
 int launch(const CUtensorMap (&maps)[4], const Args& args, cudaStream_t stream) {
-    auto kernel = mx4_pair_kernel<MODE, OutT>;
-    static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE>::kSmemBytes);
-    if (configured != cudaSuccess) {
-        thn_set_error("mx4_pair: cannot reserve %zu bytes of shared memory: %s", Shape<MODE>::kSmemBytes, cudaGetErrorString(configured));
-        return (int)configured;
-    }
+    constexpr auto kernel = mx4_pair_kernel<MODE, OutT>;
+    const int status = reserve_smem<kernel>("mx4_pair", Shape<MODE>::kSmemBytes);
+    if (status != 0) return status;
     const int most = pair_count(), pairs = args.n_tiles < most ? args.n_tiles : most;
     // In plain stream order, and no kernel is scheduled early behind it: a pair holds all tensor memory of two multiprocessors from its start to its end,
     // and a long chain of such kernels and small ones, each scheduled under the one before, was seen to stop for good.

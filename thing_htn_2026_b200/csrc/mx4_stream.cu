@@ -17,8 +17,6 @@
 // Every wait on an mbarrier is bounded: after kWaitLimitNs, and more for the stages of a sum, the waiter sets THN_ERR_WAIT_TIMEOUT in the caller's
 // error word, the block's partial sums become NaN, and tensor memory is given back.  These waits are for the block's own copies and products.  The
 // blocks of a cluster, which are resident together, wait for one another at its barrier, without a limit of its own: each comes there after bounded waits.
-#include <atomic>
-
 #include "mx4_tcgen05.cuh"
 
 namespace {
@@ -441,12 +439,11 @@ __global__ void __launch_bounds__(kTermThreads) mx4_terms_kernel(uint8_t* __rest
     });
 }
 
-// Clusters of `c` blocks that are resident together, `blocks` a multiprocessor.
-template <typename S, typename Kernel>
-int resident_clusters(Kernel kernel, int c, int blocks) {
-    static std::atomic<int> held[2][kMaxCluster + 1];      // one more than the number; 0: not asked for yet
-    std::atomic<int>& n = held[blocks - 1][c];
-    if (n == 0) {
+// Clusters of `c` blocks that are resident together on the current device, `blocks` a multiprocessor.
+template <typename S, auto KERNEL>
+int resident_clusters(int device, int c, int blocks) {
+    static NumberPerDevice held[2][kMaxCluster + 1];
+    return held[blocks - 1][c](device, [&] {
         cudaLaunchConfig_t config = {};
         config.gridDim = dim3((unsigned)(c * 512));
         config.blockDim = dim3(S::kThreads);
@@ -459,13 +456,12 @@ int resident_clusters(Kernel kernel, int c, int blocks) {
         config.attrs = attribute;
         config.numAttrs = 1;
         int found = 0;
-        if (cudaOccupancyMaxActiveClusters(&found, kernel, &config) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&found, KERNEL, &config) != cudaSuccess) {
             cudaGetLastError();
-            found = 0;
+            return -1;
         }
-        n = found + 1;
-    }
-    return n - 1;
+        return found;
+    });
 }
 
 // How a weight is cut: blocks of a cluster, and blocks a multiprocessor.
@@ -476,18 +472,18 @@ struct Cut {
 // Few tiles: the largest cluster of which all are resident together and that has a piece of K a block, two blocks a multiprocessor where a half of
 // its shared memory holds four stages, else one.  More tiles: blocks alone, two a multiprocessor where there are more tiles than those and four
 // stages fit (34,816 x 5,120 is 272 tiles: 1.84 rounds of single blocks, of which the second leaves the memory idle in part).
-template <typename S, typename Kernel>
-Cut cut_for(Kernel kernel, int n_tiles, int chunks, int n_sms) {
+template <typename S, auto KERNEL>
+Cut cut_for(int device, int n_tiles, int chunks, int n_sms) {
     if (n_tiles <= n_sms) {
         const int most = chunks < kMaxCluster ? chunks : kMaxCluster;
         if (S::stages_for(2, true) >= 4)
             for (int c = most; c >= 2; --c)
-                if (n_tiles * c <= 2 * n_sms && resident_clusters<S>(kernel, c, 2) >= n_tiles) return {c, 2};
+                if (n_tiles * c <= 2 * n_sms && resident_clusters<S, KERNEL>(device, c, 2) >= n_tiles) return {c, 2};
         for (int c = most; c >= 2; --c)
-            if (n_tiles * c <= n_sms && resident_clusters<S>(kernel, c, 1) >= n_tiles) return {c, 1};
+            if (n_tiles * c <= n_sms && resident_clusters<S, KERNEL>(device, c, 1) >= n_tiles) return {c, 1};
         if (S::stages_for(2, true) >= S::kMinStages)
             for (int c = most; c >= 2; --c)
-                if (n_tiles * c <= 2 * n_sms && resident_clusters<S>(kernel, c, 2) >= n_tiles) return {c, 2};
+                if (n_tiles * c <= 2 * n_sms && resident_clusters<S, KERNEL>(device, c, 2) >= n_tiles) return {c, 2};
     }
     return {1, n_tiles > n_sms && S::stages_for(2, false) >= 4 ? 2 : 1};
 }
@@ -495,16 +491,13 @@ Cut cut_for(Kernel kernel, int n_tiles, int chunks, int n_sms) {
 template <typename RT, int MR, int PAIRS, typename OutT>
 int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, Args args, cudaStream_t stream) {
     using S = Shape<RT, MR, PAIRS>;
-    auto kernel = mx4_stream_kernel<RT, MR, PAIRS, OutT>;
-    static const cudaError_t configured = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
-    if (configured != cudaSuccess) {
-        thn_set_error("mx4_stream: cannot reserve %d bytes of shared memory: %s", 226 * 1024, cudaGetErrorString(configured));
-        return (int)configured;
-    }
+    constexpr auto kernel = mx4_stream_kernel<RT, MR, PAIRS, OutT>;
+    const int status = reserve_smem<kernel>("mx4_stream", 226 * 1024);
+    if (status != 0) return status;
     int device = 0, n_sms = 0;
     cudaGetDevice(&device);
     cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
-    const Cut cut = cut_for<S>(kernel, args.n_tiles, args.chunks, n_sms);
+    const Cut cut = cut_for<S, kernel>(device, args.n_tiles, args.chunks, n_sms);
     args.stages = S::stages_for(cut.blocks, cut.cluster > 1);
     const size_t smem = args.stages * S::kStageStride + S::kFixed + S::recv_bytes(cut.cluster > 1);
     const int slots = n_sms * cut.blocks;

@@ -4,6 +4,7 @@
 #include <cuda.h>
 
 #include "mx4.cuh"
+#include "per_device.h"
 
 // Rows x [M, K] of a type (THN_F32, THN_BF16) as terms of 8-bit floats, see below: term t of row r is row t * plane + r / size * pitch + r % size of a
 // matrix of bytes [terms * plane, padded], whose scales lie as mx4.cuh says (mx4_stream.cu).
@@ -266,6 +267,20 @@ inline EncodeTiled encode_tiled() {
         return (EncodeTiled)p;
     }();
     return fn;
+}
+
+// Lets a kernel take so much dynamic shared memory on the current device.
+template <auto KERNEL>
+int reserve_smem(const char* what, size_t bytes) {
+    static OncePerDevice reserved;
+    int device = -1;
+    cudaGetDevice(&device);
+    const int status = reserved(device, [&] { return (int)cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes); });
+    if (status != 0) {
+        cudaGetLastError();
+        thn_set_error("%s: cannot reserve %zu bytes of shared memory: %s", what, bytes, cudaGetErrorString((cudaError_t)status));
+    }
+    return status;
 }
 
 // Codes [rows][padded / 2] for boxes of 128 columns x box_rows, which arrive as 8-bit containers of 16 bytes for 16 entries, the
