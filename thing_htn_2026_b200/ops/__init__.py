@@ -1137,16 +1137,21 @@ def dequantize_mx4(q: Mx4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
 
 
 _MX4_MOST = 1 << 24       # rows, outputs or columns of a product
-_mx4_terms_needs: Dict[Tuple[str, int, int, int, int], int] = {}
+_MX4_KEPT = 4096          # sizes of scratch that are remembered; then they are asked for again
+_mx4_terms_needs: Dict[Tuple[str, int, int, int, int, int], int] = {}
 
 
 def _mx4_terms_need(entry: str, kind: int, m: int, n: int, k: int) -> int:
-    key = (entry, kind, m, n, k)
-    if key not in _mx4_terms_needs:
+    """The bytes of scratch of a product on the current device."""
+    key = (entry, torch._C._cuda_getDevice(), kind, m, n, k)
+    need = _mx4_terms_needs.get(key)
+    if need is None:
         size = c_longlong(0)
         getattr(lib(), entry)(kind, m, n, k, ctypes.byref(size))
-        _mx4_terms_needs[key] = size.value
-    return _mx4_terms_needs[key]
+        if len(_mx4_terms_needs) >= _MX4_KEPT:
+            _mx4_terms_needs.clear()
+        need = _mx4_terms_needs[key] = size.value
+    return need
 
 
 def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Optional[torch.Tensor] = None,
