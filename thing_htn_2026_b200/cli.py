@@ -80,6 +80,8 @@ def _engine(args):
     from .engine.engine import Engine
     if bool(args.model) == bool(args.random_config):
         raise SystemExit("give exactly one of --model DIR and --random-config NAME")
+    if args.activations and not args.weights:
+        raise SystemExit("--activations mx4 goes with --weights mx4")
     if args.model:
         return Engine(args.model, dtype=args.dtype, device=args.device, weights=args.weights, activations=args.activations)
     return Engine.from_config(_named_config(args), seed=args.seed, dtype=args.dtype, device=args.device, weights=args.weights,

@@ -19,6 +19,7 @@ import torch
 
 from ..cache.sequence_cache import SequenceCache
 from ..config import ModelConfig
+from ..models.decoder import check_formats
 from .device_backend import DeviceBackend
 from .generation import Completion, GenerationLoop, Request, tokens_needed
 from .loading import load_model, parse_dtype, random_model
@@ -42,6 +43,7 @@ class Engine:
         ``weights="mx4"``: the layers' products hold their weights in microscaled 4-bit floating
         point, and with ``activations="mx4"`` they multiply rows brought to 4 bits as well.  (A ``model`` that an engine
         computes with already keeps its weights: refused.  Over weights in 4 bits, each engine keeps its own choice of rows.)"""
+        check_formats(weights, activations)
         if not torch.cuda.is_available():
             raise RuntimeError("Engine needs a CUDA device; this library has no CPU path")
         self.dtype = parse_dtype(dtype)
@@ -63,6 +65,7 @@ class Engine:
     def from_config(cls, config: ModelConfig, seed: int = 0, *, dtype="bfloat16", device: str = "cuda:0",
                     matrix_std: float = 0.02, gain_std: float = 0.02, **kwargs) -> "Engine":
         """Random weights of the configuration's shapes, drawn on the device."""
+        check_formats(kwargs.get("weights"), kwargs.get("activations"))
         model = random_model(config, seed, dtype, device, matrix_std=matrix_std, gain_std=gain_std)
         return cls(None, dtype=dtype, device=device, model=model, **kwargs)
 

@@ -29,6 +29,13 @@ def tensor_specs_of_plan(plan: ModelPlan) -> List[TensorSpec]:
     return specs
 
 
+def check_formats(weights: Optional[str], activations: Optional[str]) -> None:
+    """Raises where these are no formats in which a model's layers can hold their weights and take their rows."""
+    if (weights, activations) not in ((None, None), ("mx4", None), ("mx4", "mx4")):
+        raise ValueError(f"weights {weights!r} with activations {activations!r}: weights are 'mx4' or None, activations 'mx4' "
+                         f"(with such weights) or None")
+
+
 class DecoderModel:
     _users = ()
 
@@ -75,11 +82,9 @@ class DecoderModel:
         are.  ``activations`` "mx4": what these products multiply is brought to 4 bits too, a row at a time, at every step.  None:
         nothing is changed.  Refused while an engine or a step runner that was made before computes with the weights that would go;
         over weights in 4 bits already, the choice of rows holds for engines and step runners that are made from here on."""
-        if weights is None and activations is None:
+        check_formats(weights, activations)
+        if weights is None:
             return
-        if weights != "mx4" or activations not in (None, "mx4"):
-            raise ValueError(f"weights {weights!r} with activations {activations!r}: weights are 'mx4' or None, activations 'mx4' "
-                             f"(with such weights) or None")
         if len(self._users) and any(isinstance(w, torch.Tensor) for layer in self.layers for _, _, w in layer.products()):
             raise ValueError(f"an engine or step runner ({type(next(iter(self._users))).__name__}) computes with this model's weights as they are: "
                              f"weights='mx4' needs a model of its own, or one whose engines are gone")
