@@ -95,3 +95,23 @@ def test_bytes_of_a_model_on_the_device(name):
     gc.collect()
     held = sum(-(-w.nbytes // piece) * piece for layer in model.layers for _, _, w in layer.products())
     assert torch.cuda.memory_allocated() <= before - sum(gone.values()) + held
+
+
+# What stays in 16 bits, as :meth:`DecoderModel.quantize` says.
+STAYS = {"routers and routed experts": {"w_route", "w_up", "w_gate_up", "w_down"},
+         "decays, step sizes, input and forget gates": {"w_a1", "w_a2", "w_gates", "w_bc", "w_dt", "w_low", "w1", "w2"},
+         "time mixing's input projections": {"w_wide"}, "token rows": {"table", "w_gate", "w_proj"}}
+EXPERTS = {"RoutedExperts", "RoutedGLUExperts", "RoutedClampedExperts"}
+
+
+@pytest.mark.parametrize("name", DESIGNS)
+def test_what_stays_in_16_bits(name, monkeypatch):
+    monkeypatch.setattr(block, "PARALLEL_STREAMS", False)
+    for layer in layers_of(name):
+        for part in [layer] + layer.parts():
+            products = getattr(part, "PRODUCTS", ())
+            stays = {n for n, t in vars(part).items() if isinstance(t, torch.Tensor) and t.dim() > 1 and t.dtype == torch.bfloat16} - set(products)
+            if type(part).__name__ in EXPERTS:
+                assert stays and stays <= STAYS["routers and routed experts"]
+            else:
+                assert stays <= set.union(*STAYS.values()) - STAYS["routers and routed experts"], (type(part).__name__, stays)

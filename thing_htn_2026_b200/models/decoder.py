@@ -78,15 +78,18 @@ class DecoderModel:
 
     def quantize(self, weights: Optional[str], activations: Optional[str] = None) -> None:
         """``weights`` "mx4": the weights of the layers' products are held in microscaled 4-bit floating point from here on
-        (:class:`ops.Mx4`); the embedding, the head, norms, routers, gates, convolutions and routed experts stay as they
-        are.  ``activations`` "mx4": what these products multiply is brought to 4 bits too, a row at a time, at every step.  None:
+        (:class:`ops.Mx4`): the mixers' wide input projections, output gates among them, and output projections, and the dense
+        feed-forwards.  As they are stay the embedding and the head, norms and convolutions, routers and routed experts, the narrow products
+        of decays, step sizes, input and forget gates, time mixing's input projections (r, k, v, g), and token rows' two products.
+        ``activations`` "mx4": what these products multiply is brought to 4 bits too, a row at a time, at every step.  None:
         nothing is changed.  Refused while an engine or a step runner that was made before computes with the weights that would go;
         over weights in 4 bits already, the choice of rows holds for engines and step runners that are made from here on."""
         check_formats(weights, activations)
         if weights is None:
             return
-        if len(self._users) and any(isinstance(w, torch.Tensor) for layer in self.layers for _, _, w in layer.products()):
-            raise ValueError(f"an engine or step runner ({type(next(iter(self._users))).__name__}) computes with this model's weights as they are: "
+        users = list(self._users)
+        if users and any(isinstance(w, torch.Tensor) for layer in self.layers for _, _, w in layer.products()):
+            raise ValueError(f"an engine or step runner ({type(users[0]).__name__}) computes with this model's weights as they are: "
                              f"weights='mx4' needs a model of its own, or one whose engines are gone")
         if not sum(layer.quantize_products(activations == "mx4") for layer in self.layers):
             raise ValueError("no layer of this model has products whose weights can be held in 4 bits")
