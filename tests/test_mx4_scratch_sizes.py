@@ -32,3 +32,10 @@ def test_sizes_are_remembered(monkeypatch):
     for m in range(1, 500):
         assert need(m) == m
         assert len(ops._mx4_terms_needs) <= 50
+
+
+def test_the_rows_of_the_product_of_few_rows_stand_once():
+    """Scratch is asked of the product that takes the rows; the library says which that is."""
+    for kind in range(3):
+        most = ops._mx4_few_rows(kind)
+        assert most == ops.lib().thn_mx4_stream_rows(kind) and most >= 8

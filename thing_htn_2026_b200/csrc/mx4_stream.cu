@@ -550,6 +550,7 @@ int mx4_terms(void* bytes, void* scales, const void* x, int x_type, int M, int K
 
 // How many rows of a type (THN_F32, THN_BF16, 2: 4 bits) thn_mx4_stream takes.
 static int rows_taken(int x_type) { return x_type == THN_F32 ? 32 : 64; }
+THN_API int thn_mx4_stream_rows(int x_type) { return rows_taken(x_type); }
 
 // The bytes of `terms` that M rows of a type need.
 static long long terms_needed(int x_type, int M, int N, int K) {

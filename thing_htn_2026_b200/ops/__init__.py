@@ -7,6 +7,7 @@ else, and every product of the 32-bit path, is this library's own kernel.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 from contextlib import contextmanager
@@ -157,6 +158,7 @@ _SIGNATURES = {
     "thn_mx4_pair_scratch": [c_int, c_int, c_int, c_int, c_void_p],
     "thn_mx4_pair": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                      c_int, c_void_p, c_void_p],
+    "thn_mx4_stream_rows": [c_int],
     "thn_mx4_stream_scratch": [c_int, c_int, c_int, c_int, c_void_p],
     "thn_mx4_stream": [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_int,
                        c_int, c_void_p, c_void_p],
@@ -1154,6 +1156,12 @@ def _mx4_terms_need(entry: str, kind: int, m: int, n: int, k: int) -> int:
     return need
 
 
+@functools.lru_cache(maxsize=None)
+def _mx4_few_rows(kind: int) -> int:
+    """How many rows of a kind (a type's code, 2: in 4 bits) the product of few rows takes."""
+    return lib().thn_mx4_stream_rows(kind)
+
+
 def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [M, K] @ weight[N, K]^T`` (+ ``bias [N]``) with a weight in 4 bits: float32 sums, rounded to ``out_dtype`` (bfloat16 or
@@ -1208,7 +1216,7 @@ def linear_mx4(x, weight: Mx4, out_dtype: Optional[torch.dtype] = None, err: Opt
     if m == 0 or n == 0:
         return out
     codes = held.data_ptr()
-    few = m <= (32 if kind == 0 else 64)          # the rows that thn_mx4_stream takes
+    few = m <= _mx4_few_rows(kind)
     terms_at, size = None, 0
     if kind != 2:
         size = _mx4_terms_need("thn_mx4_stream_scratch" if few else "thn_mx4_pair_scratch", kind, m, n, k)
