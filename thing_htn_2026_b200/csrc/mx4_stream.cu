@@ -28,7 +28,7 @@ constexpr int kMaxCluster = 8;
 // Rows that the kernel itself brings to terms.  Five to eight float32 rows, with six terms to compute, only by a weight of few pieces (four pieces of
 // K a block): by 19,456 x 2,560 eight of them took 26 us so and 13.7 us prepared, five by 1,333 x 1,000 4.6 us either way, a launch more.
 constexpr int kConverted = 8;
-constexpr long long kFewPieces = 4 * 296;
+constexpr long long kFewPieces = 4 * 296;      // (two blocks on each of 148 multiprocessors)
 inline bool converts(int x_type, int M, int N, int K) {
     return M <= 4 || (M <= kConverted && (x_type != THN_F32 || (N + 127LL) / 128 * ((K + 127) / 128) <= kFewPieces));
 }
