@@ -115,3 +115,22 @@ def test_what_stays_in_16_bits(name, monkeypatch):
                 assert stays and stays <= STAYS["routers and routed experts"]
             else:
                 assert stays <= set.union(*STAYS.values()) - STAYS["routers and routed experts"], (type(part).__name__, stays)
+
+
+def test_a_mixer_that_says_its_rows_itself():
+    """A mixer in phases of a user's own: ``in_rows`` and ``out_rows`` of its own, and ``finish``."""
+    from thing_htn_2026_b200.parts.fused import PhasedMixer
+
+    class Own(PhasedMixer):
+        def __init__(self):
+            self.rows = [(torch.ones(8, 4), None), (torch.ones(4, 8), torch.zeros(4))]
+            self.finish()
+
+        def in_rows(self):
+            return self.rows[0]
+
+        def out_rows(self):
+            return self.rows[1]
+
+    own = Own()
+    assert own.w_in is own.rows[0][0] and own.b_in is None and own.w_out is own.rows[1][0] and own.b_out is own.rows[1][1]

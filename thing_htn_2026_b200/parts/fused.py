@@ -61,6 +61,10 @@ class PhasedMixer:
     def out_rows(self) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         return self.w_out, self.b_out
 
+    def finish(self) -> None:
+        """For a mixer whose ``in_rows`` and ``out_rows`` are its own: once they can be asked, its products alone are over what they say."""
+        self.hold(self.in_rows(), self.out_rows())
+
     def inner(self, x: torch.Tensor, proj: torch.Tensor, offset: int, ctx: StepContext, entry: ScheduleEntry,
               out: torch.Tensor, out_offset: int, scale: float) -> None:
         raise NotImplementedError
