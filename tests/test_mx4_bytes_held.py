@@ -66,6 +66,21 @@ def test_nothing_keeps_the_weights_that_were_replaced(name, monkeypatch):
     assert sum(t.numel() * t.element_size() for t in kept) < sum(gone.values()) / 4
 
 
+def test_one_weight_at_a_time_is_held_in_both_forms(monkeypatch):
+    monkeypatch.setattr(block, "PARALLEL_STREAMS", False)
+    gone = []
+
+    def quantize(w):
+        assert all(ref() is None for ref in gone)
+        gone.append(weakref.ref(w))
+        return ops.Mx4.__new__(ops.Mx4)._set(torch.empty(0, dtype=torch.uint8), *w.shape)
+
+    monkeypatch.setattr(ops, "quantize_mx4", quantize)
+    for layer in layers_of("tiny-a"):
+        layer.quantize_products()
+    assert len(gone) > 4
+
+
 @pytest.mark.parametrize("name", DESIGNS)
 def test_a_weight_is_held_once(name, monkeypatch):
     """In 16 bits, too: a mixer pair's members do not keep what the pair's products have copies of."""

@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(Shape<RT, MR, PAIRS>::kThreads) mx4_stream_ker
         // before it, so that they are copied under those; two sets of columns take them in turn.
         // (Tensor memory is taken once the kernels before are done: a block that held it while it waits for them could hold what one of theirs, or of another
         // stream's kernels beside them, still has to take, and that wait has no bound.
-        // One row by 19,456 x 2,560 takes 9.9 us so, 8.1 with columns taken ahead of the wait; by 6,144 x 2,560 5.3 and 5.1; other sizes are level.)
+        // Blocks that walk alone, two a multiprocessor, pay for it: one row by 19,456 x 2,560 9.9 us, 8.1 with columns taken ahead of the wait, eight rows 10.9 and
+        // 9.7, 32 by 34,816 x 5,120 23.1 and 22.3; clusters are level, 5.3 and 5.1 by 6,144 x 2,560.)
         pdl_wait();
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),

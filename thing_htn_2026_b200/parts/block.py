@@ -103,13 +103,12 @@ class Block:
     def quantize_products(self, quantize_rows: bool = False) -> int:
         """Bring the weights of the products to 4 bits; ``quantize_rows``: the rows that they multiply too, at every step.
         Returns how many there are."""
-        held = self.products()
-        for part, name, weight in held:
-            if isinstance(weight, torch.Tensor):
-                weight = ops.quantize_mx4(weight.contiguous())
-                setattr(part, name, weight)
-            weight.quantizes_rows = bool(quantize_rows)
-        return len(held)
+        places = [(part, name) for part, name, _ in self.products()]
+        for part, name in places:                  # (one weight at a time is held in both forms)
+            if isinstance(getattr(part, name), torch.Tensor):
+                setattr(part, name, ops.quantize_mx4(getattr(part, name).contiguous()))
+            getattr(part, name).quantizes_rows = bool(quantize_rows)
+        return len(places)
 
     def step_inputs(self, batch: HostBatch, out: Dict[str, List[int]]) -> None:
         """Integer inputs that members want computed on the host for this step, by name."""
